@@ -716,6 +716,67 @@ int mi355q_decode_attention_fused(
     int kv_fp8, const float* k_scale, const float* v_scale, mi355q_stream_t stream);
 
 /* ------------------------------------------------------------------ */
+/* 8-bit KV cache with a scale for each block and head; windowed attention */
+/* ------------------------------------------------------------------ */
+/* what a cache element is: 16 bits of the activation dtype, or a code (value = code * scale) */
+enum { MI355Q_KV_16 = 0, MI355Q_KV_FP8 = 1, MI355Q_KV_INT8 = 2 };
+
+/*
+ * Append to a paged cache held in 8 bits with one fp32 scale for each (block, kv head) of K and of V, the position
+ * rotation applied on the way (rot_dim 0: none, positions and cos_sin_cache unused; num_heads 0: no query).
+ * K cache [num_blocks, kv_heads, head/16, block_size, 16], V cache [num_blocks, kv_heads, head, block_size], blocks
+ * block_stride bytes apart (heads contiguous inside a block); scale of (b, h) at [b * scale_block_stride + h *
+ * scale_head_stride].  code_type MI355Q_KV_INT8 (largest code 127) or MI355Q_KV_FP8 (e4m3fn, 448).
+ *   query_out = rotated query (may be `query` itself); `key` is left as it was, the cache takes it rotated and rounded
+ *   to dtype.  For a block that the call writes from offset `first` on:
+ *     scale' = max(first > 0 ? scale : 0, largest |x| of the new tokens / largest code)
+ *     codes below `first`: round(code * (scale / scale')) where the scale grew; new codes: round(x / scale').
+ *   Writing offset 0 restarts a block.  A value that is not finite makes the scale NaN.
+ * slot_mapping int64 [num_tokens]; slots outside [0, num_blocks * block_size) are skipped (their query is rotated all the
+ * same).  The tokens of one block follow one another in slot_mapping, as a scheduler lays a sequence's new tokens (skipped
+ * ones may stand between them); of several with the same slot the last one stays.  Positions are clamped to the table's max_position rows.
+ * head_size 64 or 128, block_size 16, 32, 48 or 64; rows of 16-byte alignment take the wide loads, others work too.
+ * No counterpart in the reference, whose 8-bit caches have one scale per tensor or per head
+ * (csrc/cache_kernels.cu:254-400; rope and cache write in one hook: vllm/v1/attention/backends/rocm_attn.py:522-562).
+ */
+int mi355q_rope_and_cache_blocks(const int64_t* positions, const void* query, int64_t query_stride, void* query_out,
+                                 int64_t query_out_stride, const void* key, int64_t key_stride, const void* value,
+                                 int64_t value_stride, int head_size, int num_heads, int num_kv_heads,
+                                 const void* cos_sin_cache, int rot_dim, int max_position, int cos_dtype, int is_neox,
+                                 void* key_cache, void* value_cache, int num_blocks, int block_size, int64_t block_stride,
+                                 float* k_scales, float* v_scales, int64_t scale_block_stride, int64_t scale_head_stride,
+                                 const int64_t* slot_mapping, int num_tokens, int dtype, int code_type,
+                                 mi355q_stream_t stream);
+
+/*
+ * Causal attention of rows of any query length over the paged cache, with an optional sliding window and first tokens
+ * that stay visible: row j of sequence s stands at p = seq_lens[s] - query_len[s] + j and sees token t where
+ *   t <= p and (window == 0 or t > p - window or t < sinks).
+ * A row that sees nothing is written as zeros; rows behind the last sequence are not touched.  kv_type MI355Q_KV_16:
+ * cache of dtype elements (k_scale / v_scale unused); MI355Q_KV_FP8 / MI355Q_KV_INT8: codes whose scale is read at
+ * [block * scale_block_stride + kv_head * scale_head_stride] -- strides 0 give the one-scale cache of
+ * mi355q_reshape_and_cache, the caches of mi355q_rope_and_cache_blocks have one for each.
+ * Only pages that some row sees are looked up (those behind the window may have been given away); a page number outside
+ * [0, num_blocks) reads as tokens that nobody sees.  query_start_loc int32 [num_seqs + 1], or NULL: one row each.
+ * max_query_len bounds the query lengths; max_seq_len only chooses how the work is cut.
+ * workspace: device scratch of mi355q_paged_window_attention_workspace_bytes(...) bytes (0: may be NULL), used by this
+ * call alone; nothing in it has to be cleared.  head_size 64 or 128; 1 to 16 query heads to a kv head; block_size a
+ * multiple of 16 up to 256.
+ * Stands for the reference's windowed attention (sliding_window of AttentionImpl, vllm/v1/attention/backends/
+ * rocm_attn.py:271-300; ops/prefix_prefill.py SLIDING_WINDOW); visible first tokens and block scales have no counterpart there.
+ */
+size_t mi355q_paged_window_attention_workspace_bytes(int num_seqs, int num_rows, int num_heads, int num_kv_heads,
+                                                     int head_size, int max_query_len, int max_seq_len, int window, int sinks);
+int mi355q_paged_window_attention(void* out, int64_t out_stride, const void* query, int64_t q_stride, const void* key_cache,
+                                  const void* value_cache, int64_t kv_block_stride, int64_t kv_head_stride, int num_blocks,
+                                  int num_rows, int num_seqs, int num_heads, int num_kv_heads, int head_size, float scale,
+                                  const int32_t* block_tables, int max_blocks_per_seq, const int32_t* seq_lens,
+                                  const int32_t* query_start_loc, int max_query_len, int block_size, int max_seq_len,
+                                  int window, int sinks, int dtype, int kv_type, const float* k_scale, const float* v_scale,
+                                  int64_t scale_block_stride, int64_t scale_head_stride, void* workspace,
+                                  size_t workspace_bytes, mi355q_stream_t stream);
+
+/* ------------------------------------------------------------------ */
 /* Sampler inner loop                                                  */
 /* ------------------------------------------------------------------ */
 /* ids[b] = first index of max(float(logits[b, :])).  Replaces

@@ -1,0 +1,667 @@
+"""8-bit KV cache with a scale for each (block, kv head), and attention with a sliding window and visible first tokens:
+ops.rope_and_cache_blocks, ops.reshape_and_cache_blocks and ops.paged_window_attention against plain restatements.
+
+The append is compared bit for bit: the restatement does the documented fp32 operations one at a time.  Attention is compared
+with a 64-bit evaluation of the formula on the very codes the kernel reads; the tolerance is the sum of what the kernel's
+roundings can do (see `attention_bound`)."""
+import numpy as np
+import pytest
+import torch
+
+from mi355q import ops
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda"
+QMAX = {"block_int8": 127.0, "block_fp8": 448.0}
+CODE = {"block_int8": torch.int8, "block_fp8": torch.float8_e4m3fn, "fp8": torch.float8_e4m3fn}
+UNIT = {torch.bfloat16: 2.0 ** -8, torch.float16: 2.0 ** -11}
+
+
+# ---------------------------------------------------------------------------------------------------------------------
+# append
+# ---------------------------------------------------------------------------------------------------------------------
+def cpu(t):
+    return t.detach().cpu()
+
+
+def encode(x, form):
+    """fp32 -> the values the codes stand for (before the scale)."""
+    return torch.round(x) if form == "block_int8" else x.clamp(-448, 448).to(torch.float8_e4m3fn).float()
+
+
+def rotate_ref(x, positions, cos_sin, rot, neox, dtype):
+    """x [T, heads, D]; fp32 with one rounding per operation, rounded to dtype at the end."""
+    if not rot:
+        return x.clone()
+    y = x.float().clone()
+    row = cos_sin.float()[positions.clamp(0, cos_sin.shape[0] - 1)][:, None]
+    e = rot // 2
+    c, s = row[..., :e], row[..., e:]
+    i, j = (slice(0, e), slice(e, rot)) if neox else (slice(0, rot, 2), slice(1, rot, 2))
+    a, b = x.float()[..., i], x.float()[..., j]
+    y[..., i] = a * c - b * s
+    y[..., j] = b * c + a * s
+    return y.to(dtype)
+
+
+def append_ref(codes, scales, x, slots, bs, form):
+    """codes: fp32 values [blocks, KVH, bs, D] (changed in place); scales [blocks, KVH]; x [T, KVH, D] in the model's type.
+    One run of tokens in one block after the other (at most 64 positions each), as documented."""
+    n = codes.shape[0] * bs
+    t, T = 0, len(slots)
+    while t < T:
+        if not 0 <= slots[t] < n:
+            t += 1
+            continue
+        b, end, run = slots[t] // bs, t, []
+        while end < min(T, t + 64):
+            if 0 <= slots[end] < n:
+                if slots[end] // bs != b:
+                    break
+                run.append(end)
+            end += 1
+        stands = {slots[i] % bs: i for i in run}       # the last of several for one slot
+        first = min(stands)
+        take = x[sorted(stands.values())].float()
+        top = take.abs().amax((0, 2)) / torch.tensor(QMAX[form])
+        top = torch.where(torch.isfinite(take).all(2).all(0), top, torch.nan)
+        for h in range(x.shape[1]):
+            old = scales[b, h].item() if first > 0 else 0.0
+            new = top[h].item() if top[h] > old or torch.isnan(top[h]) else old
+            if new > old:
+                ratio = torch.tensor(old) / torch.tensor(new)
+                codes[b, h, :first] = encode(codes[b, h, :first] * ratio, form)
+            for o, i in stands.items():
+                codes[b, h, o] = encode(x[i, h].float() / torch.tensor(new), form) if new > 0 else 0.0
+            scales[b, h] = new
+        t = end
+
+
+class Cache:
+    """A paged 8-bit cache with stale contents, and the restatement's copy of it."""
+
+    def __init__(self, blocks, kvh, D, bs, form, seed=0):
+        g = torch.Generator().manual_seed(seed)
+        self.form, self.bs, self.D = form, bs, D
+        stale = torch.randint(-127, 128, (2, blocks, kvh, bs, D), generator=g).float()
+        stale = encode(stale, form)
+        self.k_ref, self.v_ref = stale[0].clone(), stale[1].clone()
+        self.ks_ref, self.vs_ref = (torch.rand(blocks, kvh, generator=g) * 0.02 for _ in range(2))
+        self.kc = self.pack_k(self.k_ref).to(DEV)
+        self.vc = self.pack_v(self.v_ref).to(DEV)
+        self.ks, self.vs = self.ks_ref.to(DEV), self.vs_ref.to(DEV)
+
+    def pack_k(self, x):
+        n, h, bs, D = x.shape
+        return x.view(n, h, bs, D // 16, 16).transpose(2, 3).contiguous().to(CODE[self.form]).view(torch.uint8)
+
+    def pack_v(self, x):
+        return x.transpose(2, 3).contiguous().to(CODE[self.form]).view(torch.uint8)
+
+    def append(self, k, v, slots):
+        append_ref(self.k_ref, self.ks_ref, k, slots, self.bs, self.form)
+        append_ref(self.v_ref, self.vs_ref, v, slots, self.bs, self.form)
+
+    def check(self):
+        """Codes compared as values (e4m3 has two zeros), scales bit for bit."""
+        for got, want in ((self.kc, self.pack_k(self.k_ref)), (self.vc, self.pack_v(self.v_ref))):
+            a, b = cpu(got).view(CODE[self.form]).float(), want.view(CODE[self.form]).float()
+            assert torch.equal(a, b), f"{int((a != b).sum())} of {a.numel()} codes differ"
+        for got, want in ((self.ks, self.ks_ref), (self.vs, self.vs_ref)):
+            assert torch.equal(torch.nan_to_num(cpu(got), nan=-1.0), torch.nan_to_num(want, nan=-1.0))
+
+
+def qkv_rows(T, H, KVH, D, dtype, seed, loud=1.0):
+    g = torch.Generator().manual_seed(seed)
+    x = torch.randn(T, (H + 2 * KVH) * D, generator=g)
+    x[:, H * D:] *= torch.exp(torch.randn(T, 1, generator=g) * loud)     # tokens of different size: scales grow as they come
+    return x.to(dtype)
+
+
+def angles(rot, rows, dtype):
+    inv = 10000.0 ** (-torch.arange(0, rot, 2, dtype=torch.float64) / rot)
+    a = torch.arange(rows, dtype=torch.float64)[:, None] * inv
+    return torch.cat([a.cos(), a.sin()], 1).to(dtype)
+
+
+def run_append(c, qkv, H, KVH, D, positions, cos_sin, rot, neox, slots, in_place=False):
+    x = qkv.to(DEV)
+    q, k, v = x[:, :H * D], x[:, H * D:(H + KVH) * D], x[:, (H + KVH) * D:]
+    out = q if in_place else torch.full(q.shape, 7.0, dtype=q.dtype, device=DEV)
+    ops.rope_and_cache_blocks(positions.to(DEV), q, k, v, D, cos_sin.to(DEV), neox, c.kc, c.vc, c.ks, c.vs,
+                              torch.tensor(slots, device=DEV), c.form, query_out=None if in_place else out)
+    torch.cuda.synchronize()
+    T = qkv.shape[0]
+    q, k, v = (t.unflatten(1, (-1, D)) for t in (qkv[:, :H * D], qkv[:, H * D:(H + KVH) * D], qkv[:, (H + KVH) * D:]))
+    want = rotate_ref(q, positions, cos_sin, rot, neox, qkv.dtype).flatten(1)
+    assert torch.equal(cpu(out), want)
+    assert torch.equal(cpu(x[:, H * D:]).contiguous().view(torch.int16), qkv[:, H * D:].contiguous().view(torch.int16))   # key and value as they were
+    c.append(rotate_ref(k, positions, cos_sin, rot, neox, qkv.dtype), v, slots)
+    c.check()
+
+
+@pytest.mark.parametrize("form", ["block_int8", "block_fp8"])
+@pytest.mark.parametrize("H,KVH,D,bs,rot,neox,dtype,table", [
+    (8, 2, 128, 16, 128, True, torch.bfloat16, torch.bfloat16),
+    (4, 4, 64, 32, 64, True, torch.float16, torch.float32),
+    (6, 2, 64, 16, 32, False, torch.bfloat16, torch.bfloat16),      # half the head, interleaved pairs
+    (3, 1, 128, 64, 64, True, torch.float16, torch.float16),
+    (5, 1, 128, 48, 36, True, torch.bfloat16, torch.float32),       # a rotation that no 16-element chunk holds
+    (16, 1, 64, 16, 6, False, torch.float16, torch.bfloat16),
+])
+def test_append_prompts_then_tokens(form, H, KVH, D, bs, rot, neox, dtype, table):
+    """Three sequences: prompts that end inside a block, a second chunk, then single tokens: every step bit for bit."""
+    c = Cache(24, KVH, D, bs, form)
+    cs = angles(rot, 4 * bs + 64, table)
+    pages = torch.randperm(24, generator=torch.Generator().manual_seed(5)).tolist()
+    filled = [0, 0, 0]
+    own = [pages[:8], pages[8:16], pages[16:24]]
+    for step, new in enumerate([(bs + 5, 1, 2 * bs), (3, 2 * bs - 1, 1), (1, 1, 1), (1, 0, 1), (bs - 2, 1, 1)]):
+        pos, slots = [], []
+        for s, n in enumerate(new):
+            for t in range(filled[s], filled[s] + n):
+                pos.append(t)
+                slots.append(own[s][t // bs] * bs + t % bs)
+            filled[s] += n
+        pos += [0, 0]                                                     # graph padding behind the batch
+        slots += [-1, -1]
+        qkv = qkv_rows(len(pos), H, KVH, D, dtype, seed=step)
+        run_append(c, qkv, H, KVH, D, torch.tensor(pos), cs, rot, neox, slots, in_place=step % 2 == 1)
+
+
+@pytest.mark.parametrize("form", ["block_int8", "block_fp8"])
+def test_append_many_tokens(form):
+    """The many-token variant of the launch (over 512 tokens), ragged, slots skipped inside the batch."""
+    H, KVH, D, bs = 4, 2, 128, 16
+    c = Cache(80, KVH, D, bs, form)
+    cs = angles(D, 1300, torch.bfloat16)
+    pages = torch.randperm(80, generator=torch.Generator().manual_seed(1)).tolist()
+    pos = list(range(7, 607)) + list(range(0, 431))
+    slots = [pages[t // bs] * bs + t % bs for t in range(7, 607)] + [pages[40 + t // bs] * bs + t % bs for t in range(431)]
+    for t in list(range(590, 600)) + [100 + 9, 900, 902]:                 # the second sequence's block 18 has gaps
+        slots[t] = -1
+    qkv = qkv_rows(len(pos), H, KVH, D, torch.bfloat16, 3)
+    run_append(c, qkv, H, KVH, D, torch.tensor(pos), cs, D, True, slots)
+
+
+@pytest.mark.parametrize("form", ["block_int8", "block_fp8"])
+def test_append_odd_slots(form):
+    """Slots outside the cache, repeated slots (the last stays), slots in falling order, zeros, values that are not finite."""
+    KVH, D, bs = 2, 64, 16
+    c = Cache(6, KVH, D, bs, form)
+    cs = angles(D, 64, torch.bfloat16)
+    slots = [-5, 6 * bs, 1 << 40, 17, 17, 17, 35, 34, 33, 40, 38, 3, -1, 50, 48, 50, 64]
+    qkv = qkv_rows(len(slots), 2, KVH, D, torch.bfloat16, 11)
+    qkv[11] = 0.0
+    qkv[16, 2 * D + 3] = float("inf")                                     # key of kv head 0
+    qkv[16, 2 * D + KVH * D + D + 1] = float("nan")                       # value of kv head 1
+    pos = torch.arange(len(slots))
+    pos[1], pos[2] = -3, 1 << 40                                          # outside the table: clamped
+    run_append(c, qkv, 2, KVH, D, pos, cs, D, True, slots)
+    assert torch.isnan(c.ks_ref[4]).tolist() == [True, False] and torch.isnan(c.vs_ref[4]).tolist() == [False, True]
+    # a poisoned block stays so until it starts over
+    run_append(c, qkv_rows(1, 2, KVH, D, torch.bfloat16, 12), 2, KVH, D, torch.tensor([1]), cs, D, True, [65])
+    assert torch.isnan(c.ks_ref[4, 0])
+    run_append(c, qkv_rows(1, 2, KVH, D, torch.bfloat16, 13), 2, KVH, D, torch.tensor([0]), cs, D, True, [64])
+    assert torch.isfinite(c.ks_ref[4]).all() and torch.isfinite(c.vs_ref[4]).all()
+
+
+def test_append_behind_long_gaps():
+    """Runs that go on behind more than 64, and more than 512, tokens without a slot."""
+    KVH, D, bs = 1, 64, 16
+    c = Cache(8, KVH, D, bs, "block_int8")
+    slots = [-1] * 700 + [19, 20] + [-1] * 90 + [21] + [-1] * 600 + [22, 23, 48] + [-1] * 20 + [49, 70] + [-1] * 70
+    qkv = qkv_rows(len(slots), 1, KVH, D, torch.bfloat16, 6)
+    run_append(c, qkv, 1, KVH, D, torch.arange(len(slots)), angles(D, len(slots), torch.bfloat16), D, True, slots)
+
+
+def test_append_one_slot_named_many_times():
+    """More neighbours in one block than a stretch of 64."""
+    KVH, D, bs = 1, 128, 16
+    c = Cache(4, KVH, D, bs, "block_int8")
+    slots = [16 + (i * 7) % 16 for i in range(150)]
+    qkv = qkv_rows(150, 1, KVH, D, torch.float16, 2)
+    run_append(c, qkv, 1, KVH, D, torch.arange(150), angles(D, 150, torch.float16), D, True, slots)
+
+
+def test_append_unaligned_rows_and_strided_scales():
+    H, KVH, D, bs = 3, 2, 64, 16
+    c = Cache(5, KVH, D, bs, "block_int8")
+    qkv = qkv_rows(20, H, KVH, D, torch.bfloat16, 4)
+    wide = torch.zeros(20, (H + 2 * KVH) * D + 3, dtype=torch.bfloat16, device=DEV)
+    wide[:, 1:-2] = qkv.to(DEV)
+    q, k, v = wide[:, 1:1 + H * D], wide[:, 1 + H * D:1 + (H + KVH) * D], wide[:, 1 + (H + KVH) * D:-2]
+    ks, vs = torch.zeros(KVH, 5, device=DEV).t(), torch.zeros(KVH, 5, device=DEV).t()
+    ks.copy_(c.ks)
+    vs.copy_(c.vs)
+    c.ks, c.vs = ks, vs
+    cs, pos, slots = angles(D, 64, torch.bfloat16), torch.arange(20), list(range(30, 50))
+    out = torch.empty(20, H * D, dtype=torch.bfloat16, device=DEV)
+    ops.rope_and_cache_blocks(pos.to(DEV), q, k, v, D, cs.to(DEV), True, c.kc, c.vc, c.ks, c.vs, torch.tensor(slots, device=DEV),
+                              c.form, query_out=out)
+    x = [t.unflatten(1, (-1, D)) for t in (qkv[:, :H * D], qkv[:, H * D:(H + KVH) * D], qkv[:, (H + KVH) * D:])]
+    assert torch.equal(cpu(out), rotate_ref(x[0], pos, cs, D, True, torch.bfloat16).flatten(1))
+    c.append(rotate_ref(x[1], pos, cs, D, True, torch.bfloat16), x[2], slots)
+    c.check()
+
+
+@pytest.mark.parametrize("form", ["block_int8", "block_fp8"])
+def test_reshape_and_cache_blocks(form):
+    """The append alone, with more key rows than slots (graph padding); and how far the held values may be off: half a step
+    for each time a value was rounded (once when written, once each time its block's scale grew)."""
+    KVH, D, bs = 3, 128, 32
+    c = Cache(4, KVH, D, bs, form)
+    written, grew = torch.zeros(bs, KVH, D), torch.zeros(bs, KVH)
+    scale = torch.zeros(KVH)
+    for t in range(bs):
+        x = qkv_rows(2, 0, KVH, D, torch.bfloat16, 40 + t)
+        k, v = x[:, :KVH * D].view(2, KVH, D), x[:, KVH * D:].view(2, KVH, D)
+        ops.reshape_and_cache_blocks(k.to(DEV), v.to(DEV), c.kc, c.vc, c.ks, c.vs, torch.tensor([64 + t], device=DEV), form)
+        c.append(k[:1], v[:1], [64 + t])
+        c.check()
+        written[t] = v[0].float()
+        grew[:t] += (c.vs_ref[2] > scale).float()
+        scale = c.vs_ref[2].clone()
+    held = c.v_ref[2].transpose(0, 1) * scale[None, :, None]            # [bs, KVH, D]
+    off = (held - written).abs()
+    if form == "block_int8":   # half a code each time, at a scale no larger than the last
+        bound = (grew + 1)[..., None] * 0.5 * scale[None, :, None] * (1 + 2 ** -20)
+    else:                      # 2^-4 of the value each time, or half the smallest e4m3 step
+        n = (grew + 1)[..., None]
+        bound = n * (written.abs() * 2 ** -4 * (1 + 2 ** -4) ** n + 2 ** -10 * scale[None, :, None])
+    assert (off <= bound).all()
+
+
+def test_append_captured_in_a_graph():
+    H, KVH, D, bs = 8, 2, 128, 16
+    c = Cache(8, KVH, D, bs, "block_int8")
+    cs = angles(D, 128, torch.bfloat16)
+    x = torch.zeros(2, (H + 2 * KVH) * D, dtype=torch.bfloat16, device=DEV)
+    pos, slots = torch.zeros(2, dtype=torch.int64, device=DEV), torch.full((2,), -1, dtype=torch.int64, device=DEV)
+    out, table = torch.empty(2, H * D, dtype=torch.bfloat16, device=DEV), cs.to(DEV)
+
+    def step():
+        ops.rope_and_cache_blocks(pos, x[:, :H * D], x[:, H * D:(H + KVH) * D], x[:, (H + KVH) * D:], D, table, True, c.kc, c.vc, c.ks, c.vs,
+                                  slots, c.form, query_out=out)
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        step()
+    for t in range(20):
+        rows = qkv_rows(2, H, KVH, D, torch.bfloat16, 60 + t)
+        p, s = torch.tensor([t, t]), [16 + t, -1 if t % 3 else 80 + t]
+        x.copy_(rows)
+        pos.copy_(p)
+        slots.copy_(torch.tensor(s))
+        g.replay()
+        torch.cuda.synchronize()
+        q, k, v = (r.unflatten(1, (-1, D)) for r in (rows[:, :H * D], rows[:, H * D:(H + KVH) * D], rows[:, (H + KVH) * D:]))
+        assert torch.equal(cpu(out), rotate_ref(q, p, cs, D, True, torch.bfloat16).flatten(1))
+        c.append(rotate_ref(k, p, cs, D, True, torch.bfloat16), v, s)
+        c.check()
+
+
+# ---------------------------------------------------------------------------------------------------------------------
+# attention
+# ---------------------------------------------------------------------------------------------------------------------
+class Batch:
+    """Sequences "context + new" over a paged cache; everything a call of paged_window_attention takes, and the formula in
+    64 bits on the same codes."""
+
+    def __init__(self, lens, H, KVH, D, bs, form, dtype, window=0, sinks=0, seed=0, loud=1.0, spare=2):
+        g = torch.Generator().manual_seed(seed)
+        self.lens, self.H, self.KVH, self.D, self.bs, self.form, self.dtype, self.window, self.sinks = lens, H, KVH, D, bs, form, dtype, window, sinks
+        total = [c + n for c, n in lens]
+        pages = [max(1, -(-t // bs)) for t in total]
+        self.blocks = sum(pages) + spare
+        order = torch.randperm(self.blocks, generator=g)
+        self.tables = torch.full((len(lens), max(pages) + 1), -7, dtype=torch.int32)       # never a page of anybody's
+        at = 0
+        for s, n in enumerate(pages):
+            self.tables[s, :n] = order[at:at + n].to(torch.int32)
+            at += n
+        self.rows = sum(n for _, n in lens)
+        self.qkv = torch.randn(self.rows + 1, H * D, generator=g).to(dtype)                 # one row behind the last sequence
+        self.q = self.qkv.view(-1, H, D)
+        shape = (self.blocks, KVH, bs, D)
+        k = torch.randn(shape, generator=g) * torch.exp(torch.randn(1, KVH, 1, D, generator=g) * 0.5)
+        v = torch.randn(shape, generator=g) * torch.exp(torch.randn(self.blocks, KVH, 1, 1, generator=g) * loud)
+        x = 8 if form == "auto" else 16
+        if form == "auto":
+            self.k, self.v = k.to(dtype).double(), v.to(dtype).double()
+            kk, vv = k.to(dtype), v.to(dtype)
+            self.ks = self.vs = None
+        else:
+            if form == "fp8":
+                self.ks, self.vs = torch.tensor(0.03), torch.tensor(0.02)
+                sk, sv = self.ks, self.vs
+            else:
+                self.ks, self.vs = k.abs().amax((2, 3)) / QMAX[form], v.abs().amax((2, 3)) / QMAX[form]
+                sk, sv = self.ks[..., None, None], self.vs[..., None, None]
+            kk, vv = ((torch.round(t) if form == "block_int8" else t.clamp(-448, 448)).to(CODE[form]) for t in (k / sk, v / sv))
+            self.k, self.v = kk.double() * sk.double(), vv.double() * sv.double()
+        byte = kk if form == "auto" else kk.view(torch.uint8)
+        self.kc = byte.view(self.blocks, KVH, bs, D // x, x).transpose(2, 3).contiguous().to(DEV)
+        byte = vv if form == "auto" else vv.view(torch.uint8)
+        self.vc = byte.transpose(2, 3).contiguous().to(DEV)
+        self.scale = D ** -0.5
+        self.dev = {n: (None if t is None else t.to(DEV)) for n, t in dict(q=self.q, tables=self.tables, ks=self.ks, vs=self.vs).items()}
+        self.seq_lens = torch.tensor(total, dtype=torch.int32, device=DEV)
+        self.starts = torch.tensor([0] + np.cumsum([n for _, n in lens]).tolist(), dtype=torch.int32, device=DEV)
+        self.max_query, self.max_len = max(1, max(n for _, n in lens)), max(1, max(total))
+
+    def run(self, **more):
+        out = torch.full(self.q.shape, 3.0, dtype=self.dtype, device=DEV)
+        d = self.dev
+        a = dict(out=out, query=d["q"], key_cache=self.kc, value_cache=self.vc, num_kv_heads=self.KVH, scale=self.scale, block_tables=d["tables"],
+                 seq_lens=self.seq_lens, query_start_loc=self.starts, max_query_len=self.max_query, max_seq_len=self.max_len,
+                 kv_cache_dtype=self.form, k_scale=d["ks"], v_scale=d["vs"], sliding_window=self.window, sink_tokens=self.sinks)
+        a.update(more)
+        ops.paged_window_attention(**a)
+        return a["out"]
+
+    def visible(self, s, j):
+        c, n = self.lens[s]
+        p = c + j
+        t = torch.arange(c + n)
+        keep = t <= p
+        if self.window:
+            keep &= (t > p - self.window) | (t < self.sinks)
+        return t[keep]
+
+    def reference(self):
+        """(out, bound) in 64 bits, [rows, H, D]."""
+        out, bound = torch.zeros(self.rows, self.H, self.D, dtype=torch.float64), torch.zeros(self.rows, self.H, self.D, dtype=torch.float64)
+        G, row = self.H // self.KVH, 0
+        for s, (c, n) in enumerate(self.lens):
+            table = self.tables[s].long()
+            for j in range(n):
+                t = self.visible(s, j)
+                if len(t):
+                    page, off = table[t // self.bs], t % self.bs
+                    inside = (page >= 0) & (page < self.blocks)
+                    page, off = page[inside], off[inside]
+                    k, v = self.k[page, :, off].transpose(0, 1), self.v[page, :, off].transpose(0, 1)         # [KVH, L, D]
+                    q = self.q[row].double().view(self.KVH, G, self.D)
+                    z = q @ k.transpose(1, 2) * self.scale
+                    w = torch.softmax(z, 2)
+                    o = w @ v
+                    slip = (q.abs() @ k.abs().transpose(1, 2) * self.scale).amax(2, keepdim=True)
+                    out[row] = o.reshape(self.H, self.D)
+                    bound[row] = self.attention_bound(o, w @ v.abs(), v.abs().amax(1, keepdim=True), slip, len(t)).reshape(self.H, self.D)
+                row += 1
+        return out, bound
+
+    def attention_bound(self, o, mass, vmax, slip, n):
+        """What the roundings add up to.  mass = sum w |v|:
+          probabilities rounded to fp16 (8-bit caches) or the model's type: one half step of each, u_p * mass
+          logits: products summed in fp32 over the head, at most (D + 8) 2^-24 of sum |q k| each, and the base-2 exponent's own
+            error of about 2^-22; both as relative errors of the weights, in numerator and denominator: 2 * (...) * mass
+          the sums over n tokens in fp32, and the scale factors: (n / 16 + 32) 2^-24 * mass (products are added 16 and more at a time)
+          fp16 probabilities below its normal range: n * 2^-32 of the largest |v| (times 4 for the headroom of the scales)
+          the result rounded to the model's type: u_out * (|o| + the above)"""
+        u_p = UNIT[self.dtype] if self.form == "auto" else 2.0 ** -11
+        weights = 2 * ((self.D + 8) * 2.0 ** -24 * slip * 1.5 + 2.0 ** -21)
+        e = (u_p + weights + (n / 16 + 32) * 2.0 ** -24) * mass + n * 2.0 ** -30 * vmax
+        return e + UNIT[self.dtype] * (o.abs() + e) + 2.0 ** -25
+
+    def check(self, out=None):
+        got = cpu(self.run() if out is None else out).double()
+        want, bound = self.reference()
+        assert torch.equal(got[self.rows:], torch.full_like(got[self.rows:], 3.0)), "rows behind the last sequence"
+        off = (got[:self.rows] - want).abs()
+        worst = (off / bound).nan_to_num(0.0).max().item() if self.rows else 0.0
+        assert torch.isfinite(got).all() and (off <= bound).all(), f"{worst:.2f} of the bound"
+
+
+FORMS = ["auto", "fp8", "block_int8", "block_fp8"]
+HEADS = [(8, 2, 128, 16, torch.bfloat16), (4, 4, 64, 32, torch.float16), (16, 1, 128, 48, torch.float16), (7, 1, 64, 16, torch.bfloat16),
+         (6, 2, 128, 64, torch.bfloat16)]
+
+
+@pytest.mark.parametrize("form", FORMS)
+@pytest.mark.parametrize("H,KVH,D,bs,dtype", HEADS)
+def test_decode_rows(form, H, KVH, D, bs, dtype):
+    lens = [(0, 1), (1, 1), (15, 1), (16, 1), (62, 1), (63, 1), (64, 1), (200, 1), (301, 1), (575, 1)]
+    b = Batch(lens, H, KVH, D, bs, form, dtype, seed=1)
+    b.check()
+    b.check(b.run(query_start_loc=None, query=b.dev["q"], max_query_len=1))
+
+
+@pytest.mark.parametrize("form", FORMS)
+@pytest.mark.parametrize("H,KVH,D,bs,dtype", HEADS)
+def test_mixed_rows(form, H, KVH, D, bs, dtype):
+    """Prompts, chunks over a context, drafts and decode rows in one batch; a sequence without new rows."""
+    b = Batch([(0, 37), (130, 5), (64, 70), (90, 1), (33, 0), (0, 1), (255, 2)], H, KVH, D, bs, form, dtype, seed=2)
+    b.check()
+
+
+@pytest.mark.parametrize("form", FORMS)
+@pytest.mark.parametrize("window,sinks", [(1, 0), (1, 1), (16, 4), (63, 0), (64, 4), (65, 70), (100, 17), (4096, 4)])
+def test_window_and_sinks(form, window, sinks):
+    b = Batch([(0, 150), (299, 1), (200, 9), (0, 1), (40, 60), (333, 1)], 4, 2, 64, 16, form, torch.bfloat16, window=window, sinks=sinks, seed=3)
+    b.check()
+
+
+@pytest.mark.parametrize("form", FORMS)
+@pytest.mark.parametrize("window,sinks", [(0, 0), (600, 4)])
+def test_long_contexts_are_cut_and_joined(form, window, sinks):
+    lens = [(4999, 1), (2047, 3), (64, 1)]
+    b = Batch(lens, 4, 1, 128, 16, form, torch.float16, window=window, sinks=sinks, seed=4)
+    if not window:
+        assert ops.paged_window_attention_workspace_bytes(3, b.rows + 1, 4, 1, 128, 3, 5000) > 0
+    b.check()
+    # a bound on the lengths that is far off changes how the work is cut, not what comes out of it
+    b.check(b.run(max_seq_len=64))
+    b.check(b.run(max_seq_len=1 << 17))
+
+
+@pytest.mark.parametrize("form", FORMS)
+@pytest.mark.parametrize("window,sinks", [(0, 0), (70, 4)])
+def test_longer_prompts(form, window, sinks):
+    """Prompt rows past several tiles and column blocks, with a context whose end is inside a page."""
+    Batch([(0, 333), (77, 260), (500, 129)], 8, 2, 128, 16, form, torch.bfloat16, window=window, sinks=sinks, seed=5).check()
+    Batch([(0, 300), (13, 200)], 3, 1, 64, 32, form, torch.float16, window=window, sinks=sinks, seed=6).check()
+
+
+@pytest.mark.parametrize("form", FORMS)
+def test_masked_places_hold_anything(form):
+    """Pages behind the window given away (numbers outside the cache), stale places after a sequence's end full of NaN, scales of
+    pages that nobody sees NaN: none of it shows."""
+    b = Batch([(300, 1), (130, 1), (200, 40), (5, 20)], 4, 2, 64, 16, form, torch.float16, window=50, sinks=3, seed=7)
+    want = cpu(b.run())
+    for s, (c, n) in enumerate(b.lens):
+        low = max(0, c + 1 - 50)
+        for page in range((c + n + 15) // 16):
+            if page * 16 >= 3 and (page + 1) * 16 <= low:
+                b.tables[s, page] = [-1, 1 << 30, b.blocks, -(1 << 31)][page % 4]
+    b.dev["tables"] = b.tables.to(DEV)
+    used = torch.zeros(b.blocks, dtype=torch.bool)
+    used[b.tables[(b.tables >= 0) & (b.tables < b.blocks)].long()] = True
+    nan = {"auto": 0x7e00, "fp8": 0x7f, "block_fp8": 0x7f, "block_int8": 0x80}[form]
+    kc, vc = (t.view(torch.int16 if form == "auto" else torch.uint8) for t in (b.kc, b.vc))
+    kc[~used] = nan
+    vc[~used] = nan
+    for s, (c, n) in enumerate(b.lens):
+        end, page = (c + n) % 16, int(b.tables[s, (c + n - 1) // 16])
+        if end:
+            kc[page, :, :, end:] = nan
+            vc[page, :, :, end:] = nan
+    if form.startswith("block"):
+        b.dev["ks"][~used] = float("nan")
+        b.dev["vs"][~used] = float("nan")
+    got = cpu(b.run())
+    assert torch.equal(got, want)
+    b.check(got.to(DEV))
+
+
+@pytest.mark.parametrize("form", ["auto", "fp8"])
+@pytest.mark.parametrize("shape", [(0, 40), (60, 7), (0, 200)])
+def test_not_finite_tokens_reach_only_the_rows_that_see_them(form, shape):
+    """A key or value that is not finite: rows before it (and behind the window) are as if it were not there."""
+    c, n = shape
+    b = Batch([shape], 4, 2, 64, 16, form, torch.bfloat16, window=24, sinks=2, seed=8)
+    clean = cpu(b.run()).double()
+    t, end = c + n // 2, c + n
+    page, off = int(b.tables[0, t // 16]), t % 16
+    if form == "auto":
+        b.vc[page, 0, 5, off] = float("inf")
+        b.vc[page, 1, 9, off] = float("nan")
+    else:
+        b.vc[page, 0, 5, off] = 0x7f
+        b.vc[page, 1, 9, off] = 0x7f
+    got = cpu(b.run()).double()
+    for j in range(n):
+        sees = t in b.visible(0, j).tolist()
+        for h in range(4):
+            d = 5 if h < 2 else 9
+            rest = [i for i in range(64) if i != d]
+            # other head dims: the same sums in another order at most
+            assert torch.allclose(got[j, h, rest], clean[j, h, rest], rtol=2 ** -6, atol=2 ** -7)
+            if not sees:
+                assert torch.isfinite(got[j, h, d]) and abs(got[j, h, d] - clean[j, h, d]) <= 2 ** -6 * abs(clean[j, h, d]) + 2 ** -7
+            elif form == "auto" and h < 2:
+                assert got[j, h, d] == float("inf")
+            else:
+                assert torch.isnan(got[j, h, d])
+    # keys: a NaN logit makes its row NaN, and no other
+    b = Batch([shape], 4, 2, 64, 16, form, torch.bfloat16, window=24, sinks=2, seed=8)
+    b.kc[page, 0, 0, off, 0] = float("nan") if form == "auto" else 0x7f
+    got = cpu(b.run()).double()
+    for j in range(n):
+        sees = t in b.visible(0, j).tolist()
+        assert torch.isnan(got[j, :2]).all() if sees else torch.allclose(got[j, :2], clean[j, :2], rtol=2 ** -6, atol=2 ** -7)
+        assert torch.equal(got[j, 2:], clean[j, 2:])
+
+
+@pytest.mark.parametrize("form", ["block_int8", "block_fp8"])
+def test_poisoned_block_reads_as_nan(form):
+    b = Batch([(50, 1), (70, 1), (100, 3)], 4, 2, 128, 16, form, torch.bfloat16, window=32, sinks=0, seed=9)
+    clean = cpu(b.run())
+    b.dev["ks"][int(b.tables[0, 3]), 0] = float("nan")       # tokens 48 .. 63 of sequence 0
+    b.dev["vs"][int(b.tables[1, 1]), 1] = float("nan")       # tokens 16 .. 31 of sequence 1: behind its window
+    b.dev["vs"][int(b.tables[2, 4]), 1] = float("nan")       # tokens 64 .. 79 of sequence 2
+    got = cpu(b.run())
+    assert torch.isnan(got[0, :2]).all() and torch.equal(got[0, 2:], clean[0, 2:])
+    assert torch.equal(got[1], clean[1])
+    assert torch.equal(got[2:5, :2], clean[2:5, :2]) and torch.isnan(got[2:5, 2:]).all()
+
+
+def test_rows_that_see_nothing():
+    """A sequence of length zero, and rows before the sequence's first token (query longer than the sequence)."""
+    for form in FORMS:
+        b = Batch([(0, 3), (20, 2), (0, 4)], 4, 2, 64, 16, form, torch.bfloat16, seed=10)
+        b.seq_lens.copy_(torch.tensor([0, 22, 2]))
+        got = cpu(b.run())
+        assert torch.equal(got[:3], torch.zeros_like(got[:3])) and torch.equal(got[5:7], torch.zeros_like(got[5:7]))
+        assert got[3:5].abs().sum() > 0 and got[7:9].abs().sum() > 0
+        b2 = Batch([(0, 3), (20, 2), (0, 4)], 4, 2, 64, 16, form, torch.bfloat16, seed=10)
+        assert torch.equal(cpu(b2.run())[3:5], got[3:5])
+
+
+@pytest.mark.parametrize("form", ["block_int8", "block_fp8"])
+def test_scales_far_apart(form):
+    """Blocks whose V scales differ by factors of up to e^30: the probabilities in between keep their bits."""
+    b = Batch([(700, 1), (300, 6)], 4, 2, 128, 16, form, torch.bfloat16, seed=11, loud=6.0)
+    b.check()
+
+
+@pytest.mark.parametrize("form", ["block_int8", "fp8", "auto"])
+def test_large_and_small_queries(form):
+    """Query rows from 2^-40 to 2^30 (bf16): the power of two that brings them to fp16 comes off again."""
+    b = Batch([(100, 1), (60, 3), (200, 1)], 4, 2, 64, 16, form, torch.bfloat16, seed=12)
+    b.q *= torch.exp2(torch.tensor([-40.0, 0.0, 3.0, 1.0, 2.0, 0.0]))[:, None, None].to(torch.bfloat16)
+    b.q[2, 1] = 0.0
+    b.dev["q"] = b.q.to(DEV)
+    b.check()
+    b.q.mul_(2.0 ** 30)
+    b.scale *= 2.0 ** -30
+    b.dev["q"] = b.q.to(DEV)
+    b.check()
+
+
+def test_strided_rows_tables_and_cache_heads():
+    """Query rows inside a wider projection, output rows inside a wider buffer, a cache whose head pages lie apart."""
+    b = Batch([(100, 1), (60, 30), (200, 1)], 4, 2, 64, 16, "block_int8", torch.float16, seed=13)
+    wide = torch.zeros(b.rows + 1, 4 * 64 + 128, dtype=torch.float16, device=DEV)
+    wide[:, 64:-64] = b.dev["q"].flatten(1)
+    out = torch.full((b.rows + 1, 4 * 64 + 32), 3.0, dtype=torch.float16, device=DEV)
+    kc = torch.zeros(b.blocks, 4, *b.kc.shape[2:], dtype=torch.uint8, device=DEV)[:, ::2]
+    vc = torch.zeros(b.blocks, 4, *b.vc.shape[2:], dtype=torch.uint8, device=DEV)[:, ::2]
+    kc.copy_(b.kc)
+    vc.copy_(b.vc)
+    scales = [torch.empty(2, b.blocks, device=DEV).t().copy_(b.dev[n]) for n in ("ks", "vs")]
+    got = b.run(query=wide[:, 64:-64].unflatten(1, (4, 64)), out=out[:, :256].unflatten(1, (4, 64)), key_cache=kc, value_cache=vc,
+                k_scale=scales[0], v_scale=scales[1])
+    assert torch.equal(out[:, 256:], torch.full_like(out[:, 256:], 3.0))
+    b.check(got)
+
+
+def test_streams_graphs_and_a_workspace_of_ones_own():
+    b = Batch([(2999, 1), (700, 3)], 4, 1, 128, 16, "block_int8", torch.bfloat16, seed=14)
+    want = cpu(b.run())
+    need = ops.paged_window_attention_workspace_bytes(2, b.rows + 1, 4, 1, 128, b.max_query, b.max_len)
+    ws = torch.empty(need, dtype=torch.uint8, device=DEV)
+    assert torch.equal(cpu(b.run(workspace=ws)), want)
+    with pytest.raises(RuntimeError, match="workspace"):
+        b.run(workspace=ws[:need - 16])
+    streams = [torch.cuda.Stream() for _ in range(4)]
+    outs = []
+    for s in streams:
+        s.wait_stream(torch.cuda.current_stream())
+    for i in range(12):
+        with torch.cuda.stream(streams[i % 4]):
+            outs.append(b.run())
+    torch.cuda.synchronize()
+    assert all(torch.equal(cpu(o), want) for o in outs)
+    # two graphs over the same inputs, replayed at once on two streams
+    out = [torch.empty_like(b.dev["q"]) for _ in range(2)]
+    graphs = []
+    for o in out:
+        o.fill_(3.0)
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            b.run(out=o)
+        graphs.append(g)
+    for _ in range(5):
+        for o in out:
+            o.fill_(3.0)
+        torch.cuda.synchronize()
+        for s, g in zip(streams, graphs):
+            with torch.cuda.stream(s):
+                g.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(cpu(o), want) for o in out)
+
+
+# ---------------------------------------------------------------------------------------------------------------------
+# as they are used: append, then attend, step after step
+# ---------------------------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("form", ["block_int8", "block_fp8"])
+@pytest.mark.parametrize("window,sinks", [(0, 0), (40, 4)])
+def test_generation_over_the_block_scaled_cache(form, window, sinks):
+    """Two conversations: prompt, second chunk, decode steps.  Each step's attention is checked against the formula on what the
+    cache then holds; the cache itself against the restated append."""
+    H, KVH, D, bs, dtype = 4, 2, 64, 16, torch.bfloat16
+    c = Cache(20, KVH, D, bs, form)
+    cs = angles(D, 256, dtype)
+    own = [[3, 9, 1, 17, 5, 8, 0, 11], [2, 4, 19, 6, 7, 10, 12, 13]]
+    filled = [0, 0]
+    for step, new in enumerate([(45, 20), (0, 33), (1, 1), (1, 1), (1, 4), (1, 1)]):
+        pos = [t for s in range(2) for t in range(filled[s], filled[s] + new[s])]
+        slots = [own[s][t // bs] * bs + t % bs for s in range(2) for t in range(filled[s], filled[s] + new[s])]
+        qkv = qkv_rows(len(pos), H, KVH, D, dtype, 90 + step, loud=0.3)
+        run_append(c, qkv, H, KVH, D, torch.tensor(pos), cs, D, True, slots)
+        b = Batch([(filled[s], new[s]) for s in range(2)], H, KVH, D, bs, form, dtype, window=window, sinks=sinks)
+        b.q = torch.cat([rotate_ref(qkv[:, :H * D].unflatten(1, (H, D)), torch.tensor(pos), cs, D, True, dtype), b.q[-1:]])
+        b.k, b.v = c.k_ref.double() * c.ks_ref.double()[..., None, None], c.v_ref.double() * c.vs_ref.double()[..., None, None]
+        b.tables = torch.tensor(own, dtype=torch.int32)
+        b.blocks, b.kc, b.vc = 20, c.kc, c.vc
+        b.dev = dict(q=b.q.to(DEV), tables=b.tables.to(DEV), ks=c.ks, vs=c.vs)
+        filled = [f + n for f, n in zip(filled, new)]
+        b.check()

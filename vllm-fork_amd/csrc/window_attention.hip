@@ -1,0 +1,633 @@
+// Attention over the paged cache with a sliding window and visible first tokens (sinks), over 16-bit caches, 8-bit caches
+// with one scale per tensor and 8-bit caches with a scale for each (block, kv head).
+//   K cache [blocks, kv_heads, head/x, block_size, x] (x = 16 bytes of elements), V cache [blocks, kv_heads, head, block_size]
+//
+// Query row j of a sequence sits at position p = seq_len - query_len + j and sees token t where
+//   t <= p  and  (no window, or t > p - window, or t < sinks);
+// a row that sees nothing comes out as zeros.  Rows of several query heads that share a kv head are flattened into
+// columns, (row, head) = (c / G, c % G): decode rows, drafts and prompts differ only in how many columns there are.
+//
+//   S^T = K Q^T, O^T = V^T P^T on the matrix cores, running maximum and sum per column.
+//
+// 8-bit codes become fp16 (every int8 and every e4m3 value is one) and are multiplied with fp16 queries: a bf16 query row is
+// first brought to [2^13, 2^14) by a power of two, which keeps all 8 bits of every element within 2^-28 of the row's
+// largest.  Scales stay outside the products: the 16 tokens of a lane group lie in one block, so K's scale is one factor
+// per lane on the logits and V's one factor per lane on the probabilities, relative to the largest V scale met so far
+// (vref, rescaled like the running maximum) so that fp16 holds them.
+#include <limits.h>
+#include <math.h>
+
+#include <algorithm>
+
+#include "common.h"
+
+namespace mi355q {
+
+typedef __attribute__((ext_vector_type(2))) _Float16 wa_f16x2;
+typedef __attribute__((ext_vector_type(2))) __bf16 wa_bf16x2;
+
+constexpr float WA_LOG2E = 1.44269504088896f;
+// Probabilities are kept as 2^(x - m + 7): fp16 then resolves a probability down to 2^-31 of the largest, and the running
+// maximum m may lag behind by up to 8 before the sums are rescaled (the largest value is 2^15).
+constexpr float WA_SHIFT = 7.0f, WA_LAG = 8.0f;
+
+struct WindowParams {
+  uint16_t* out;
+  const uint16_t* q;
+  const unsigned char* kc;
+  const unsigned char* vc;
+  const float* ks;
+  const float* vs;
+  const int32_t* tables;
+  const int32_t* seq_lens;
+  const int32_t* starts;        // query_start_loc, or null: one row per sequence
+  float* part_o;                // [rows, heads, splits, head] partial sums
+  float* part_ml;               // [rows, heads, splits, 2] their maxima (base 2) and sums
+  int64_t out_stride, q_stride;
+  int64_t block_stride, head_stride;   // bytes
+  int64_t scale_block_stride, scale_head_stride;
+  float scale;
+  int num_seqs, num_rows, num_heads, num_kv_heads, group;
+  int num_blocks, table_width;
+  int bs, page_magic;
+  int window, sinks;            // window 0: none
+  int splits, split_tiles;      // the context in stretches of split_tiles 64-token tiles, at most `splits` of them
+  int col_tiles;                // column tiles of the longest query
+};
+
+__device__ inline int wa_page(int n, int magic) { return magic ? (int)__umulhi((unsigned)n, (unsigned)magic) : n; }
+
+// a load whose address is the same for the whole wave and whose memory no store of the launch touches: scalar cache
+template <typename T>
+__device__ inline T sload(const T* p) {
+  return *(const __attribute__((address_space(4))) T*)(uintptr_t)p;
+}
+
+// what a sequence's rows [first column, last column] see: sink tokens [0, sink_end) and [low, end), 64 at a time
+struct Span {
+  int sink_end, low, end, sink_tiles, tiles;
+  __device__ inline int base(int i) const { return i < sink_tiles ? 64 * i : low + 64 * (i - sink_tiles); }
+  __device__ inline int limit(int i) const { return i < sink_tiles ? sink_end : end; }
+};
+__device__ inline Span span_of(const WindowParams& p, int pos_first, int pos_last) {
+  Span s;
+  s.end = min(pos_last + 1, p.table_width * p.bs);
+  const int low = p.window ? max(0, pos_first - p.window + 1) : 0;
+  s.low = min(low, max(s.end, 0)) & ~15;
+  s.sink_end = min(p.sinks, s.low);
+  s.sink_tiles = (s.sink_end + 63) >> 6;
+  s.tiles = s.sink_tiles + (s.end > s.low ? (s.end - s.low + 63) >> 6 : 0);
+  return s;
+}
+
+enum { KV16 = MI355Q_KV_16, KVF8 = MI355Q_KV_FP8, KVI8 = MI355Q_KV_INT8 };
+
+// type of the products
+template <typename DT, int KV>
+struct MathOf { typedef FP16 T; };
+template <typename DT>
+struct MathOf<DT, KV16> { typedef DT T; };
+
+// 4 codes -> 4 fp16
+template <int KV>
+__device__ inline u32x2 widen4(uint32_t w) {
+  u32x2 r;
+  if constexpr (KV == KVF8) {
+    r[0] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w, 1.0f, false));
+    r[1] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w, 1.0f, true));
+  } else {
+    // 0x6400 + u is the fp16 number 1024 + u: the code biased by 128 in the low byte, then 1152 taken off, exactly
+    const uint32_t u = w ^ 0x80808080u;
+    const wa_f16x2 bias = {(_Float16)1152.0f, (_Float16)1152.0f};
+    r[0] = __builtin_bit_cast(uint32_t, __builtin_bit_cast(wa_f16x2, __builtin_amdgcn_perm(0x64646464u, u, 0x04010400u)) - bias);
+    r[1] = __builtin_bit_cast(uint32_t, __builtin_bit_cast(wa_f16x2, __builtin_amdgcn_perm(0x64646464u, u, 0x04030402u)) - bias);
+  }
+  return r;
+}
+// half h (8 codes) of a 16-byte piece
+template <int KV>
+__device__ inline u32x4 widen8(u32x4 w, int h) {
+  const u32x2 a = widen4<KV>(w[2 * h]), b = widen4<KV>(w[2 * h + 1]);
+  return u32x4{a[0], a[1], b[0], b[1]};
+}
+
+// max over the four lanes that share a column
+__device__ inline float group_max(float v) {
+  auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  v = fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+  r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
+__device__ inline float group_sum(float v) {
+  auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  v = __uint_as_float(r[0]) + __uint_as_float(r[1]);
+  r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return __uint_as_float(r[0]) + __uint_as_float(r[1]);
+}
+__device__ inline float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }
+
+// whether one of eight 16-bit values is an infinity or NaN
+template <typename MT>
+__device__ inline bool not_finite(u32x4 v) {
+  const uint32_t e = MT::id == MI355Q_BF16 ? 0x7f80u : 0x7c00u;
+  bool bad = false;
+#pragma unroll
+  for (int i = 0; i < 4; i++) bad |= (v[i] & e) == e || ((v[i] >> 16) & e) == e;
+  return bad;
+}
+// value n of eight (none: n outside 0 .. 7), in lanes that are `here`; zeros elsewhere
+template <typename MT>
+__device__ inline u32x4 only(u32x4 v, bool here, int n) {
+#pragma unroll
+  for (int i = 0; i < 4; i++) v[i] &= here ? (n == 2 * i ? 0xffffu : n == 2 * i + 1 ? 0xffff0000u : 0u) : 0u;
+  return v;
+}
+
+// ---------------------------------------------------------------------------------------------------------------------
+// Few columns (decode rows, drafts): one workgroup of 4 waves per (sequence, 16 columns, kv head, stretch of the context);
+// the waves take the stretch's 64-token tiles in turn, each with a running softmax of its own, and meet once in LDS.
+// Bound by HBM: a wave keeps a tile of K or V on the way while it works on the other (K of the next tile is requested as
+// soon as this tile's logits stand, V as soon as its products do).
+//
+// Token order inside a tile: row i of 16-row MFMA tile T is token 16 (i / 4) + 4 T + i % 4, so the 16 logits that a lane of
+// group g = lane / 16 holds after S^T are tokens 16 g .. 16 g + 15: one block, one scale, and the B operand of O^T as
+// they stand; V comes in its own order, 16 tokens of a head dim per lane.
+// ---------------------------------------------------------------------------------------------------------------------
+template <typename DT, int KV, int HEAD>
+__global__ __launch_bounds__(256, 2) void window_rows_kernel(const WindowParams p) {
+  typedef typename MathOf<DT, KV>::T MT;
+  constexpr int EB = KV == KV16 ? 2 : 1;
+  constexpr int DS = HEAD / 32, DT16 = HEAD / 16;
+  constexpr int KP = EB == 1 ? DS / 2 : DS;      // 16-byte pieces of K per lane and row tile
+  constexpr int VP = EB == 1 ? 1 : 2;            // of V per lane and 16 head dims
+  constexpr int LD = HEAD + 4;
+  __shared__ __attribute__((aligned(16))) float acc[4][16 * LD];
+  __shared__ float stat[4][2][16];
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int g = lane >> 4, col = lane & 15;
+
+  const int kvh = blockIdx.x % p.num_kv_heads;
+  int b = blockIdx.x / p.num_kv_heads;
+  const int split = b % p.splits;
+  b /= p.splits;
+  const int ct = b % p.col_tiles, seq = b / p.col_tiles;
+  const int G = p.group;
+
+  const int start = p.starts ? p.starts[seq] : seq;
+  const int qlen = p.starts ? p.starts[seq + 1] - start : 1;
+  const int cols = min(qlen, p.num_rows - start) * G;
+  if (start < 0 || ct * 16 >= cols) return;
+  const int seq_len = p.seq_lens[seq];
+  const int c0 = ct * 16, c1 = min(c0 + 16, cols) - 1;
+  const int pos0 = seq_len - qlen + c0 / G, pos1 = seq_len - qlen + c1 / G;
+  const Span span = span_of(p, pos0, pos1);
+  // (a context longer than the caller's bound: the last stretch takes the rest)
+  const int begin = split == 0 ? 0 : split * p.split_tiles;
+  const int end = split == p.splits - 1 ? span.tiles : min(begin + p.split_tiles, span.tiles);
+  if (split > 0 && begin >= end) return;      // nothing here; the merge knows how many stretches there are
+  const bool whole = span.tiles <= p.split_tiles;
+
+  const int c = min(c0 + col, c1);
+  const int row = start + c / G, head = kvh * G + c % G;
+  const int pos = seq_len - qlen + c / G;
+  const int low = p.window ? pos - p.window + 1 : INT_MIN;
+
+  // ---- this lane's query column -------------------------------------------------------------------------------------
+  u32x4 qf[DS];
+  float qscale = p.scale * WA_LOG2E;
+  {
+    const uint16_t* qp = p.q + (int64_t)row * p.q_stride + (int64_t)head * HEAD;
+#pragma unroll
+    for (int ds = 0; ds < DS; ds++) {
+      const int d0 = EB == 1 ? 16 * (4 * (ds >> 1) + g) + 8 * (ds & 1) : 32 * ds + 8 * g;
+      qf[ds] = *reinterpret_cast<const u32x4*>(qp + d0);
+    }
+    if constexpr (EB == 1 && DT::id == MI355Q_BF16) {
+      float top = 0.f;
+#pragma unroll
+      for (int ds = 0; ds < DS; ds++)
+#pragma unroll
+        for (int e = 0; e < 4; e++)
+          top = fmaxf(top, fmaxf(fabsf(BF16::to_f32((uint16_t)qf[ds][e])), fabsf(BF16::to_f32((uint16_t)(qf[ds][e] >> 16)))));
+      top = group_max(top);
+      int ex = (int)(__float_as_uint(top) >> 23);            // biased exponent; 255: not finite, 0: zero or subnormal
+      ex = ex == 255 ? 140 : max(ex, 20);
+      const float up = __uint_as_float((uint32_t)(127 + 140 - ex) << 23);   // 2^(13 - exponent)
+      qscale *= __uint_as_float((uint32_t)(ex - 13) << 23);
+#pragma unroll
+      for (int ds = 0; ds < DS; ds++)
+#pragma unroll
+        for (int e = 0; e < 4; e++)
+          qf[ds][e] = pack2<FP16>(BF16::to_f32((uint16_t)qf[ds][e]) * up, BF16::to_f32((uint16_t)(qf[ds][e] >> 16)) * up);
+    }
+  }
+
+  const int32_t* table = p.tables + (int64_t)seq * p.table_width;
+  const int pieces = p.bs >> 4;
+  const unsigned char* kc = p.kc + (int64_t)kvh * p.head_stride;
+  const unsigned char* vc = p.vc + (int64_t)kvh * p.head_stride;
+  const int64_t klane = ((int64_t)g * p.bs + (col & 3)) * 16;
+  const int64_t vlane = (int64_t)col * p.bs * EB;
+
+  // one tile's four 16-token stretches: where their block lies, what scales it, whether anything of it is seen
+  auto place_of = [&](int tile, const unsigned char*& kp, const unsigned char*& vp, float& ks, float& vs, bool& ok) {
+    const int t0 = span.base(tile), lim = span.limit(tile);
+    int blk[4], off[4];
+#pragma unroll
+    for (int j = 0; j < 4; j++) {
+      const int n = min(t0 + 16 * j, (lim - 1) & ~15) >> 4;   // past the end: the last stretch again, masked
+      const int pg = wa_page(n, p.page_magic);
+      blk[j] = sload(table + pg);
+      off[j] = (n - pg * pieces) * 16;
+    }
+    kp = kc, vp = vc, ks = 0.f, vs = 0.f, ok = false;
+#pragma unroll
+    for (int j = 0; j < 4; j++) {
+      const bool in = (unsigned)blk[j] < (unsigned)p.num_blocks;
+      const int64_t at = in ? blk[j] : 0;
+      const unsigned char* kj = kc + at * p.block_stride + (int64_t)off[j] * 16;
+      const unsigned char* vj = vc + at * p.block_stride + off[j] * EB;
+      if ((col >> 2) == j) kp = kj;
+      if constexpr (KV != KV16) {
+        const int64_t si = at * p.scale_block_stride + kvh * p.scale_head_stride;
+        const float a = sload(p.ks + si), b = sload(p.vs + si);
+        ks = g == j ? a : ks;
+        vs = g == j ? b : vs;
+      }
+      if (g == j) {
+        vp = vj;
+        ok = in && t0 + 16 * j < lim;
+      }
+    }
+  };
+
+  u32x4 kf[4][KP], vf[DT16][VP];
+  auto load_k = [&](const unsigned char* kp) {
+#pragma unroll
+    for (int T = 0; T < 4; T++)
+#pragma unroll
+      for (int s = 0; s < KP; s++)
+        kf[T][s] = *reinterpret_cast<const u32x4*>(kp + klane + T * 64 + (int64_t)s * 64 * p.bs);
+  };
+  auto load_v = [&](const unsigned char* vp) {
+#pragma unroll
+    for (int d = 0; d < DT16; d++)
+#pragma unroll
+      for (int s = 0; s < VP; s++)
+        vf[d][s] = *reinterpret_cast<const u32x4*>(vp + vlane + (int64_t)d * 16 * p.bs * EB + s * 16);
+  };
+
+  f32x4 o[DT16];
+#pragma unroll
+  for (int d = 0; d < DT16; d++) o[d] = f32x4{0.f, 0.f, 0.f, 0.f};
+  float m = -INFINITY, l = 0.f, vref = 0.f;
+
+  int tile = begin + wave;
+  const unsigned char *kp, *vp;
+  float ks, vs;
+  bool ok;
+  if (tile < end) {
+    place_of(tile, kp, vp, ks, vs, ok);
+    load_k(kp);
+    load_v(vp);
+  }
+  for (; tile < end; tile += 4) {
+    const int t0 = span.base(tile), lim = span.limit(tile);
+    const float ks_now = ks, vs_now = vs;
+    const bool ok_now = ok, more = tile + 4 < end;
+    if (more) place_of(tile + 4, kp, vp, ks, vs, ok);
+
+    f32x4 s[4];
+#pragma unroll
+    for (int T = 0; T < 4; T++) {
+      s[T] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int ds = 0; ds < DS; ds++) {
+        u32x4 a;
+        if constexpr (EB == 1) a = widen8<KV>(kf[T][ds >> 1], ds & 1);
+        else a = kf[T][ds];
+        s[T] = mfma16<MT>(a, qf[ds], s[T]);
+      }
+    }
+    if (more) load_k(kp);
+
+    // ---- running softmax -------------------------------------------------------------------------------------------
+    const int tg = t0 + 16 * g;
+    const float f = KV == KV16 ? qscale : qscale * ks_now;
+    // every column sees every token of the tile?
+    const bool inner = __all(ok_now) && t0 + 64 <= lim && t0 + 63 <= pos0 && (!p.window || t0 > pos1 - p.window);
+    uint32_t seen = 0xffffu;
+    if (!inner) {
+      seen = 0;
+#pragma unroll
+      for (int i = 0; i < 16; i++) {
+        const int t = tg + i;
+        if (ok_now && t < lim && t <= pos && (t >= low || t < p.sinks)) seen |= 1u << i;
+      }
+    }
+    float x[16], mx = -INFINITY;
+#pragma unroll
+    for (int i = 0; i < 16; i++) {
+      x[i] = s[i >> 2][i & 3] * f;
+      if (!inner) x[i] = (seen >> i) & 1 ? x[i] : -INFINITY;
+      mx = fmaxf(mx, x[i]);
+    }
+    mx = group_max(mx);
+    float vtop = 0.f;
+    if constexpr (KV != KV16) vtop = group_max(ok_now ? vs_now : 0.f);
+    if (__any(mx > m + WA_LAG || vtop > vref)) {
+      const float mn = fmaxf(m, mx);
+      float a = m == -INFINITY ? 0.f : exp2_fast(m - mn);
+      l *= a;
+      if (vtop > vref) {        // headroom of 2: the next slightly larger scale needs no rescaling
+        a *= vref / (2.f * vtop);
+        vref = 2.f * vtop;
+      }
+#pragma unroll
+      for (int d = 0; d < DT16; d++) o[d] *= a;
+      m = mn;
+    }
+    const float ms = (m == -INFINITY ? 0.f : m) - WA_SHIFT;
+    float w[16];
+#pragma unroll
+    for (int i = 0; i < 16; i++) {
+      w[i] = exp2_fast(x[i] - ms);
+      l += w[i];
+    }
+    if constexpr (KV != KV16) {
+      const float r = vref > 0.f ? vs_now / vref : (vs_now == 0.f ? 0.f : vs_now);
+#pragma unroll
+      for (int i = 0; i < 16; i++) {
+        w[i] *= r;
+        if (!inner) w[i] = (seen >> i) & 1 ? w[i] : 0.f;   // whatever the scale of a block that is not seen
+      }
+    }
+    u32x4 pf[2];
+#pragma unroll
+    for (int i = 0; i < 8; i++) pf[i >> 2][i & 3] = pack2<MT>(w[2 * i], w[2 * i + 1]);
+
+    // ---- O^T += V^T P^T ----------------------------------------------------------------------------------------------
+    auto fragment = [&](int d, int h) {
+      if constexpr (EB == 1) return widen8<KV>(vf[d][0], h);
+      else return vf[d][h];
+    };
+    if (inner || KV == KVI8) {
+#pragma unroll
+      for (int d = 0; d < DT16; d++)
+#pragma unroll
+        for (int h = 0; h < 2; h++) o[d] = mfma16<MT>(fragment(d, h), pf[h], o[d]);
+    } else {
+      // tokens that no column sees count for nothing, whatever bytes their places hold
+      uint32_t any = 0;
+#pragma unroll
+      for (int i = 0; i < 16; i++) {
+        const int t = tg + i;
+        const bool some = ok_now && t < lim && t <= pos1 && (!p.window || t > pos0 - p.window || t < p.sinks);
+        any |= some ? 1u << i : 0u;
+      }
+      bool bad = false;
+      auto seen_fragment = [&](int d, int h) {
+        u32x4 v = fragment(d, h);
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+          const uint32_t two = any >> (8 * h + 2 * e);
+          v[e] &= (two & 1 ? 0xffffu : 0u) | (two & 2 ? 0xffff0000u : 0u);
+        }
+        return v;
+      };
+#pragma unroll
+      for (int d = 0; d < DT16; d++)
+#pragma unroll
+        for (int h = 0; h < 2; h++) {
+          const u32x4 v = seen_fragment(d, h);
+          bad |= not_finite<MT>(v);
+        }
+      if (!__any(bad)) {
+#pragma unroll
+        for (int d = 0; d < DT16; d++)
+#pragma unroll
+          for (int h = 0; h < 2; h++) o[d] = mfma16<MT>(seen_fragment(d, h), pf[h], o[d]);
+      } else {
+        // an infinity or NaN that some columns may see and others must not: one token at a time, added where it is seen
+#pragma unroll 1
+        for (int n = 0; n < 64; n++) {
+          const int gn = n >> 4, i = n & 15;
+          const bool here = g == gn;
+          const bool counts = (__shfl((int)seen, gn * 16 + col, 64) >> i) & 1;
+#pragma unroll
+          for (int d = 0; d < DT16; d++) {
+            f32x4 r = o[d];
+#pragma unroll
+            for (int h = 0; h < 2; h++) r = mfma16<MT>(only<MT>(seen_fragment(d, h), here, i - 8 * h), only<MT>(pf[h], here, i - 8 * h), r);
+            if (counts) o[d] = r;
+          }
+        }
+      }
+    }
+    if (more) load_v(vp);
+  }
+
+  // ---- the four waves meet -------------------------------------------------------------------------------------------
+  l = group_sum(l);
+  if (g == 0) {
+    stat[wave][0][col] = m;
+    stat[wave][1][col] = l;
+  }
+  __syncthreads();
+  const float mall = fmaxf(fmaxf(stat[0][0][col], stat[1][0][col]), fmaxf(stat[2][0][col], stat[3][0][col]));
+  {
+    float a = m == -INFINITY ? 0.f : exp2_fast(m - mall);
+    if constexpr (KV != KV16) a *= vref;
+#pragma unroll
+    for (int d = 0; d < DT16; d++) *reinterpret_cast<f32x4*>(&acc[wave][col * LD + 16 * d + 4 * g]) = o[d] * a;
+  }
+  __syncthreads();
+  constexpr int PER = HEAD / 16;
+  const int cc = threadIdx.x >> 4, d0 = (threadIdx.x & 15) * PER;
+  if (c0 + cc > c1) return;
+  float top = -INFINITY, sum = 0.f;
+#pragma unroll
+  for (int w = 0; w < 4; w++) top = fmaxf(top, stat[w][0][cc]);
+#pragma unroll
+  for (int w = 0; w < 4; w++) sum += stat[w][0][cc] == -INFINITY ? 0.f : stat[w][1][cc] * exp2_fast(stat[w][0][cc] - top);
+  float v[PER];
+#pragma unroll
+  for (int i = 0; i < PER; i++) v[i] = (acc[0][cc * LD + d0 + i] + acc[1][cc * LD + d0 + i]) + (acc[2][cc * LD + d0 + i] + acc[3][cc * LD + d0 + i]);
+  const int orow = start + (c0 + cc) / G, ohead = kvh * G + (c0 + cc) % G;
+  if (whole) {
+    const float inv = top == -INFINITY ? 0.f : 1.f / sum;
+    uint32_t* out = reinterpret_cast<uint32_t*>(p.out + (int64_t)orow * p.out_stride + (int64_t)ohead * HEAD + d0);
+#pragma unroll
+    for (int i = 0; i < PER / 2; i++) out[i] = top == -INFINITY ? 0u : pack2<DT>(v[2 * i] * inv, v[2 * i + 1] * inv);
+  } else {
+    const int64_t at = ((int64_t)orow * p.num_heads + ohead) * p.splits + split;
+#pragma unroll
+    for (int i = 0; i < PER; i += 4) *reinterpret_cast<f32x4*>(p.part_o + at * HEAD + d0 + i) = f32x4{v[i], v[i + 1], v[i + 2], v[i + 3]};
+    if (d0 == 0) {
+      p.part_ml[2 * at] = top;
+      p.part_ml[2 * at + 1] = sum;
+    }
+  }
+}
+
+// Joins the stretches of a long context: one wave per column (query row and head).
+template <typename DT, int HEAD>
+__global__ __launch_bounds__(256) void window_merge_kernel(const WindowParams p) {
+  constexpr int PER = HEAD / 64;
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  int b = blockIdx.x;
+  const int per_seq = (p.col_tiles * 16 + 3) / 4;
+  const int c = (b % per_seq) * 4 + wave;
+  b /= per_seq;
+  const int kvh = b % p.num_kv_heads, seq = b / p.num_kv_heads;
+  const int start = p.starts ? p.starts[seq] : seq;
+  const int qlen = p.starts ? p.starts[seq + 1] - start : 1;
+  const int cols = min(qlen, p.num_rows - start) * p.group;
+  if (start < 0 || c >= cols) return;
+  const int seq_len = p.seq_lens[seq];
+  const int c0 = c & ~15, c1 = min(c0 + 16, cols) - 1;
+  const Span span = span_of(p, seq_len - qlen + c0 / p.group, seq_len - qlen + c1 / p.group);
+  if (span.tiles <= p.split_tiles) return;    // written by its only workgroup
+  const int n = min(p.splits, (span.tiles + p.split_tiles - 1) / p.split_tiles);
+  const int row = start + c / p.group, head = kvh * p.group + c % p.group;
+  const int64_t at = ((int64_t)row * p.num_heads + head) * p.splits;
+  const float* ml = p.part_ml + 2 * at;
+  const float* po = p.part_o + at * HEAD + lane * PER;
+  float top = -INFINITY;
+  for (int i = lane; i < n; i += 64) top = fmaxf(top, ml[2 * i]);
+  top = wave_max(top);
+  float sum = 0.f, v[PER];
+#pragma unroll
+  for (int j = 0; j < PER; j++) v[j] = 0.f;
+#pragma unroll 4
+  for (int i = 0; i < n; i++) {
+    const float mi = ml[2 * i];
+    const float w = mi == -INFINITY ? 0.f : exp2_fast(mi - top);
+    sum += ml[2 * i + 1] * w;
+#pragma unroll
+    for (int j = 0; j < PER; j++) v[j] += po[(int64_t)i * HEAD + j] * w;
+  }
+  uint16_t* out = p.out + (int64_t)row * p.out_stride + (int64_t)head * HEAD + lane * PER;
+#pragma unroll
+  for (int j = 0; j < PER; j++) out[j] = top == -INFINITY ? 0 : DT::from_f32(v[j] / sum);
+}
+
+// ---------------------------------------------------------------------------------------------------------------------
+// how a call is cut: host side, from what the caller bounds
+// ---------------------------------------------------------------------------------------------------------------------
+struct WindowPlan { int col_tiles, splits, split_tiles; };
+
+static WindowPlan window_plan(int num_seqs, int num_heads, int num_kv_heads, int max_query_len, int max_seq_len, int window, int sinks) {
+  WindowPlan w;
+  const int G = num_heads / num_kv_heads;
+  w.col_tiles = (int)(((int64_t)max_query_len * G + 15) / 16);
+  // tiles that 16 columns see: the window of their first row, their own rows, an unaligned start, the sinks
+  int64_t tiles = ((int64_t)max_seq_len + 63) / 64;
+  if (window) tiles = std::min(tiles + 1, ((int64_t)std::min(window, max_seq_len) + 16 + 15 + 63) / 64 + ((int64_t)std::min(sinks, max_seq_len) + 63) / 64);
+  tiles = std::max<int64_t>(tiles, 1);
+  const int64_t groups = (int64_t)num_seqs * num_kv_heads * w.col_tiles;
+  // enough workgroups for four on each of the 256 CUs, at least 4 tiles (one per wave) in each
+  const int64_t want = std::max<int64_t>(1, (1024 + groups - 1) / groups);
+  w.split_tiles = (int)std::max<int64_t>(4, (tiles + want - 1) / want);
+  w.splits = (int)((tiles + w.split_tiles - 1) / w.split_tiles);
+  return w;
+}
+
+static size_t window_workspace(const WindowPlan& w, int num_rows, int num_heads, int head_size) {
+  return w.splits == 1 ? 0 : (size_t)num_rows * num_heads * w.splits * (head_size + 2) * sizeof(float);
+}
+
+}  // namespace mi355q
+
+using namespace mi355q;
+
+extern "C" size_t mi355q_paged_window_attention_workspace_bytes(int num_seqs, int num_rows, int num_heads, int num_kv_heads, int head_size,
+                                                                int max_query_len, int max_seq_len, int window, int sinks) {
+  if (num_seqs <= 0 || num_rows <= 0 || num_kv_heads <= 0 || num_heads <= 0 || max_query_len <= 0 || max_seq_len <= 0) return 0;
+  return window_workspace(window_plan(num_seqs, num_heads, num_kv_heads, max_query_len, max_seq_len, window, sinks), num_rows, num_heads, head_size);
+}
+
+extern "C" int mi355q_paged_window_attention(void* out, int64_t out_stride, const void* query, int64_t q_stride, const void* key_cache,
+                                             const void* value_cache, int64_t kv_block_stride, int64_t kv_head_stride, int num_blocks,
+                                             int num_rows, int num_seqs, int num_heads, int num_kv_heads, int head_size, float scale,
+                                             const int32_t* block_tables, int max_blocks_per_seq, const int32_t* seq_lens,
+                                             const int32_t* query_start_loc, int max_query_len, int block_size, int max_seq_len,
+                                             int window, int sinks, int dtype, int kv_type, const float* k_scale, const float* v_scale,
+                                             int64_t scale_block_stride, int64_t scale_head_stride, void* workspace,
+                                             size_t workspace_bytes, mi355q_stream_t stream) {
+  MI355Q_REQUIRE(dtype == MI355Q_BF16 || dtype == MI355Q_FP16, "paged_window_attention: dtype must be bf16 or fp16");
+  MI355Q_REQUIRE(kv_type == MI355Q_KV_16 || kv_type == MI355Q_KV_FP8 || kv_type == MI355Q_KV_INT8, "paged_window_attention: bad cache type %d", kv_type);
+  MI355Q_REQUIRE(num_seqs >= 0 && num_rows >= 0, "paged_window_attention: bad sizes");
+  if (num_seqs == 0 || num_rows == 0) return MI355Q_OK;
+  MI355Q_REQUIRE(out && query && key_cache && value_cache && block_tables && seq_lens, "paged_window_attention: null pointer");
+  MI355Q_REQUIRE(kv_type == MI355Q_KV_16 || (k_scale && v_scale), "paged_window_attention: an 8-bit cache needs k_scale / v_scale");
+  MI355Q_REQUIRE(head_size == 64 || head_size == 128, "paged_window_attention: head_size %d (64 or 128)", head_size);
+  MI355Q_REQUIRE(num_heads > 0 && num_kv_heads > 0 && num_heads % num_kv_heads == 0 && num_heads / num_kv_heads <= 16,
+                 "paged_window_attention: %d query heads over %d kv heads (1 to 16 to each)", num_heads, num_kv_heads);
+  MI355Q_REQUIRE(block_size >= 16 && block_size <= 256 && block_size % 16 == 0, "paged_window_attention: block size %d (a multiple of 16 up to 256)", block_size);
+  MI355Q_REQUIRE(num_blocks > 0 && max_blocks_per_seq > 0 && (int64_t)max_blocks_per_seq * block_size < (int64_t)1 << 30,
+                 "paged_window_attention: bad block table");
+  MI355Q_REQUIRE(max_query_len > 0 && max_seq_len > 0 && window >= 0 && sinks >= 0, "paged_window_attention: negative or zero length");
+  MI355Q_REQUIRE(query_start_loc || num_seqs <= num_rows, "paged_window_attention: %d rows for %d sequences", num_rows, num_seqs);
+  const int eb = kv_type == MI355Q_KV_16 ? 2 : 1;
+  const int64_t page = (int64_t)head_size * block_size;
+  MI355Q_REQUIRE(kv_head_stride >= page && kv_block_stride >= page && kv_head_stride * eb % 16 == 0 && kv_block_stride * eb % 16 == 0,
+                 "paged_window_attention: cache strides");
+  MI355Q_REQUIRE((((uintptr_t)key_cache | (uintptr_t)value_cache | (uintptr_t)query) & 15) == 0 && q_stride % 8 == 0,
+                 "paged_window_attention: caches and query rows must be 16-byte aligned");
+  MI355Q_REQUIRE(((uintptr_t)out & 3) == 0 && out_stride % 2 == 0, "paged_window_attention: output rows must be 4-byte aligned");
+  const WindowPlan w = window_plan(num_seqs, num_heads, num_kv_heads, max_query_len, max_seq_len, window, sinks);
+  const size_t need = window_workspace(w, num_rows, num_heads, head_size);
+  if (need && (!workspace || workspace_bytes < need))
+    return set_error(MI355Q_ENOSPACE, "paged_window_attention: workspace of %zu bytes, %zu needed", workspace ? workspace_bytes : (size_t)0, need);
+  MI355Q_REQUIRE(!need || ((uintptr_t)workspace & 15) == 0, "paged_window_attention: workspace must be 16-byte aligned");
+  WindowParams p{};
+  p.out = (uint16_t*)out;
+  p.q = (const uint16_t*)query;
+  p.kc = (const unsigned char*)key_cache;
+  p.vc = (const unsigned char*)value_cache;
+  p.ks = k_scale, p.vs = v_scale;
+  p.tables = block_tables, p.seq_lens = seq_lens, p.starts = query_start_loc;
+  p.part_o = (float*)workspace;
+  p.part_ml = (float*)workspace + (size_t)num_rows * num_heads * w.splits * head_size;
+  p.out_stride = out_stride, p.q_stride = q_stride;
+  p.block_stride = kv_block_stride * eb, p.head_stride = kv_head_stride * eb;
+  p.scale_block_stride = scale_block_stride, p.scale_head_stride = scale_head_stride;
+  p.scale = scale;
+  p.num_seqs = num_seqs, p.num_rows = num_rows, p.num_heads = num_heads, p.num_kv_heads = num_kv_heads, p.group = num_heads / num_kv_heads;
+  p.num_blocks = num_blocks, p.table_width = max_blocks_per_seq;
+  p.bs = block_size;
+  const int pieces = block_size / 16;
+  p.page_magic = pieces == 1 ? 0 : (int)(((1ull << 32) + pieces - 1) / pieces);
+  p.window = std::min(window, 1 << 30), p.sinks = sinks;
+  p.splits = w.splits, p.split_tiles = w.splits == 1 ? INT_MAX : w.split_tiles, p.col_tiles = w.col_tiles;
+  const int64_t groups = (int64_t)num_seqs * num_kv_heads * w.col_tiles * w.splits;
+  const int64_t merges = (int64_t)num_seqs * num_kv_heads * (w.col_tiles * 4);
+  MI355Q_REQUIRE(groups < (int64_t)1 << 31 && merges < (int64_t)1 << 31, "paged_window_attention: too many workgroups");
+  hipStream_t s = (hipStream_t)stream;
+#define ROWS(DT, KV, HD) hipLaunchKernelGGL((window_rows_kernel<DT, KV, HD>), dim3((unsigned)groups), dim3(256), 0, s, p)
+#define MERGE(DT, HD) hipLaunchKernelGGL((window_merge_kernel<DT, HD>), dim3((unsigned)merges), dim3(256), 0, s, p)
+#define BY_KV(DT, HD)                                                \
+  do {                                                               \
+    if (kv_type == MI355Q_KV_16) ROWS(DT, KV16, HD);                 \
+    else if (kv_type == MI355Q_KV_FP8) ROWS(DT, KVF8, HD);           \
+    else ROWS(DT, KVI8, HD);                                         \
+    if (w.splits > 1) {                                              \
+      if (int e = check_launch("window_rows_kernel")) return e;      \
+      MERGE(DT, HD);                                                 \
+    }                                                                \
+  } while (0)
+  if (dtype == MI355Q_BF16) {
+    if (head_size == 128) BY_KV(BF16, 128);
+    else BY_KV(BF16, 64);
+  } else {
+    if (head_size == 128) BY_KV(FP16, 128);
+    else BY_KV(FP16, 64);
+  }
+#undef BY_KV
+#undef MERGE
+#undef ROWS
+  return check_launch("paged_window_attention");
+}

@@ -17,6 +17,7 @@ W_GPTQ, W_NSEQ, W_AWQ = 0, 1, 2
 W_PAIR_HALVES = 0x100
 ZP_CONST, ZP_NSEQ, ZP_AWQ, ZP_GPTQ_V1 = 0, 1, 2, 3
 PA_PARTITION = 256
+KV_16, KV_FP8, KV_INT8 = 0, 1, 2
 
 _lib = None
 
@@ -136,6 +137,13 @@ _SIGS = {
     "mi355q_decode_attention_fused": (c_int, [c_vp, c_vp, c_vp, c_vp, c_vp, c_i64, c_vp, c_vp, c_vp, c_vp, c_i64, c_i64,
                                               c_int, c_int, c_int, c_int, c_f32, c_vp, c_int, c_vp, c_int, c_int,
                                               c_int, c_int, c_vp, c_vp, c_vp]),
+    "mi355q_rope_and_cache_blocks": (c_int, [c_vp, c_vp, c_i64, c_vp, c_i64, c_vp, c_i64, c_vp, c_i64, c_int, c_int, c_int,
+                                             c_vp, c_int, c_int, c_int, c_int, c_vp, c_vp, c_int, c_int, c_i64, c_vp, c_vp,
+                                             c_i64, c_i64, c_vp, c_int, c_int, c_int, c_vp]),
+    "mi355q_paged_window_attention_workspace_bytes": (c_sz, [c_int] * 9),
+    "mi355q_paged_window_attention": (c_int, [c_vp, c_i64, c_vp, c_i64, c_vp, c_vp, c_i64, c_i64, c_int, c_int, c_int, c_int,
+                                              c_int, c_int, c_f32, c_vp, c_int, c_vp, c_vp, c_int, c_int, c_int, c_int, c_int,
+                                              c_int, c_int, c_vp, c_vp, c_i64, c_i64, c_vp, c_sz, c_vp]),
     "mi355q_argmax": (c_int, [c_vp, c_i64, c_vp, c_int, c_int, c_int, c_vp]),
     "mi355q_argmax_decode_step": (c_int, [c_vp, c_i64, c_vp, c_int, c_int, c_int, c_vp, c_vp, c_vp, c_i64, c_vp, c_i64,
                                           c_int, c_vp]),

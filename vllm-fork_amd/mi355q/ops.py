@@ -1250,6 +1250,197 @@ def decode_attention_fused(out, exp_sum, max_logits, tmp_out, qkv, positions, co
 
 
 # ---------------------------------------------------------------------------
+# 8-bit KV cache with a scale for each block and head; windowed attention
+# ---------------------------------------------------------------------------
+_BLOCK_CODES = {"block_int8": _lib.KV_INT8, "block_fp8": _lib.KV_FP8}
+
+
+def is_block_scaled(kv_cache_dtype: str) -> bool:
+    """Caches whose codes are scaled per (block, kv head): "block_int8" and "block_fp8" (e4m3fn)."""
+    return kv_cache_dtype in _BLOCK_CODES
+
+
+def _one_device(what: str, first: torch.Tensor, *ts) -> None:
+    for t in (first, *ts):
+        if t is not None and (not t.is_cuda or t.device != first.device):
+            raise RuntimeError(f"{what}: every tensor must be on one GPU (MI355X); no CPU fallback exists")
+
+
+def _launch(device: torch.device, fn, *args) -> None:
+    """fn(*args, stream) on the device the tensors live on, on torch's current stream there."""
+    if device.index == torch.cuda.current_device():
+        check(fn(*args, _stream()))
+    else:
+        with torch.cuda.device(device):
+            check(fn(*args, _stream()))
+
+
+def _paged_cache(what: str, key_cache: torch.Tensor, value_cache: torch.Tensor, head_size: int, element: int):
+    """(kv heads, block size) of K [blocks, kv_heads, head / x, block, x] and V [blocks, kv_heads, head, block]."""
+    x = 16 // element
+    if value_cache.dim() != 4 or key_cache.dim() != 5:
+        raise RuntimeError(f"{what}: key_cache must be [blocks, kv_heads, head / {x}, block, {x}], value_cache [blocks, kv_heads, head, block]")
+    n, kvh, d, bs = value_cache.shape
+    if d != head_size or key_cache.shape != (n, kvh, head_size // x, bs, x) or n == 0:
+        raise RuntimeError(f"{what}: cache shapes {tuple(key_cache.shape)} / {tuple(value_cache.shape)} for heads of {head_size}")
+    if key_cache.element_size() != element or value_cache.element_size() != element:
+        raise RuntimeError(f"{what}: cache elements must have {element} bytes")
+    if key_cache.stride()[2:] != (bs * x, x, 1) or value_cache.stride()[2:] != (bs, 1) or key_cache.stride()[:2] != value_cache.stride()[:2]:
+        raise RuntimeError(f"{what}: the pages of a head must be contiguous, and both caches laid out alike")
+    return kvh, bs
+
+
+def _block_scales(what: str, k_scales: torch.Tensor, v_scales: torch.Tensor, blocks: int, kvh: int) -> None:
+    for s in (k_scales, v_scales):
+        if s.dtype != torch.float32 or s.shape != (blocks, kvh):
+            raise RuntimeError(f"{what}: scales must be fp32 [{blocks}, {kvh}]")
+    if k_scales.stride() != v_scales.stride():
+        raise RuntimeError(f"{what}: k_scales and v_scales must have the same strides")
+
+
+def rope_and_cache_blocks(positions: torch.Tensor, query: torch.Tensor, key: torch.Tensor, value: torch.Tensor, head_size: int,
+                          cos_sin_cache: torch.Tensor, is_neox: bool, key_cache: torch.Tensor, value_cache: torch.Tensor,
+                          k_scales: torch.Tensor, v_scales: torch.Tensor, slot_mapping: torch.Tensor, kv_cache_dtype: str,
+                          query_out: torch.Tensor | None = None) -> None:
+    """RoPE and the append to an 8-bit cache with one scale per (block, kv head), in one launch: the block-scaled form of
+    `rope_and_cache`.  query [T, heads * head] is rotated into query_out (default: in place); key is left as it was,
+    the cache takes it rotated.  kv_cache_dtype "block_int8" or "block_fp8"; k_scales / v_scales fp32 [blocks, kv_heads].
+    A block's scale grows with its tokens (earlier codes are rescaled) and starts over when offset 0 is written.
+    slot_mapping int64 [T]: negative slots and slots past the cache are skipped; the tokens of one block follow one
+    another (skipped ones may stand between them).  Not idempotent on `query` when in place, and tokens must be appended in their order."""
+    what = "rope_and_cache_blocks"
+    _one_device(what, key, positions, query, value, cos_sin_cache, key_cache, value_cache, k_scales, v_scales, slot_mapping, query_out)
+    T = slot_mapping.numel()
+    if positions.dtype != torch.int64 or slot_mapping.dtype != torch.int64 or positions.numel() != T:
+        raise RuntimeError(f"{what}: positions and slot_mapping must be int64 [T]")
+    if not positions.is_contiguous() or not slot_mapping.is_contiguous():
+        raise RuntimeError(f"{what}: positions and slot_mapping must be contiguous")
+    q2 = query.view(T, -1)
+    o2 = q2 if query_out is None else query_out.view(T, -1)
+    if cos_sin_cache.dim() != 2 or not cos_sin_cache.is_contiguous() or cos_sin_cache.shape[1] > head_size or cos_sin_cache.shape[1] % 2:
+        raise RuntimeError(f"{what}: cos_sin_cache must be contiguous [positions, rot_dim] with an even rot_dim of at most {head_size}")
+    if q2.shape != o2.shape or q2.shape[1] % head_size or o2.dtype != key.dtype or q2.dtype != key.dtype:
+        raise RuntimeError(f"{what}: query and query_out must be [T, heads * {head_size}] of the key's dtype")
+    if T and (q2.stride(1) != 1 or o2.stride(1) != 1):
+        raise RuntimeError(f"{what}: query rows must be contiguous")
+    _append_blocks(what, positions, q2, o2, key, value, head_size, cos_sin_cache, is_neox, key_cache, value_cache, k_scales, v_scales,
+                   slot_mapping, kv_cache_dtype)
+
+
+def reshape_and_cache_blocks(key: torch.Tensor, value: torch.Tensor, key_cache: torch.Tensor, value_cache: torch.Tensor,
+                             k_scales: torch.Tensor, v_scales: torch.Tensor, slot_mapping: torch.Tensor, kv_cache_dtype: str) -> None:
+    """The append of `rope_and_cache_blocks` without a rotation: the block-scaled form of `reshape_and_cache`.
+    key / value [T, kv_heads, head]; T may exceed slot_mapping's length (graph padding)."""
+    what = "reshape_and_cache_blocks"
+    _one_device(what, key, value, key_cache, value_cache, k_scales, v_scales, slot_mapping)
+    if slot_mapping.dtype != torch.int64 or not slot_mapping.is_contiguous():
+        raise RuntimeError(f"{what}: slot_mapping must be contiguous int64 [T]")
+    T, head_size = slot_mapping.numel(), value_cache.shape[2] if value_cache.dim() == 4 else 0
+    if key.dim() != 3 or key.shape[0] < T or value.shape[0] < T:
+        raise RuntimeError(f"{what}: key and value must be [T, kv_heads, head] with a row for each slot")
+    if key.stride()[1:] != (key.shape[2], 1) or value.dim() != 3 or value.stride()[1:] != (value.shape[2], 1):
+        raise RuntimeError(f"{what}: key / value rows must be contiguous")
+    _append_blocks(what, None, None, None, key[:T].flatten(1), value[:T].flatten(1), head_size, None, False, key_cache, value_cache, k_scales,
+                   v_scales, slot_mapping, kv_cache_dtype)
+
+
+def _append_blocks(what, positions, q2, o2, key, value, head_size, cos_sin, is_neox, key_cache, value_cache, k_scales, v_scales,
+                   slot_mapping, kv_cache_dtype) -> None:
+    if kv_cache_dtype not in _BLOCK_CODES:
+        raise RuntimeError(f"{what}: unsupported kv_cache_dtype {kv_cache_dtype!r} (block_int8 or block_fp8)")
+    T = slot_mapping.numel()
+    kvh, bs = _paged_cache(what, key_cache, value_cache, head_size, 1)
+    if key_cache.stride(1) != head_size * bs:
+        raise RuntimeError(f"{what}: the heads of a block must be contiguous")
+    blocks = key_cache.shape[0]
+    _block_scales(what, k_scales, v_scales, blocks, kvh)
+    k2, v2 = key.view(T, -1), value.view(T, -1)
+    if T == 0:
+        return
+    if k2.shape[1] != kvh * head_size or v2.shape != k2.shape or k2.stride(1) != 1 or v2.stride(1) != 1 or v2.dtype != key.dtype:
+        raise RuntimeError(f"{what}: key and value must be [T, {kvh} * {head_size}] with contiguous rows")
+    _launch(key.device, _lib.lib().mi355q_rope_and_cache_blocks,
+            _ptr(positions), _ptr(q2), 0 if q2 is None else q2.stride(0), _ptr(o2), 0 if o2 is None else o2.stride(0), k2.data_ptr(),
+            k2.stride(0), v2.data_ptr(), v2.stride(0), head_size, 0 if q2 is None else q2.shape[1] // head_size, kvh, _ptr(cos_sin),
+            0 if cos_sin is None else cos_sin.shape[1], 0 if cos_sin is None else cos_sin.shape[0],
+            BF16 if cos_sin is None else _dt(cos_sin, True), int(is_neox), key_cache.data_ptr(), value_cache.data_ptr(), blocks, bs,
+            key_cache.stride(0), k_scales.data_ptr(), v_scales.data_ptr(), k_scales.stride(0), k_scales.stride(1),
+            slot_mapping.data_ptr(), T, _dt(key), _BLOCK_CODES[kv_cache_dtype])
+
+
+def paged_window_attention_workspace_bytes(num_seqs: int, num_rows: int, num_heads: int, num_kv_heads: int, head_size: int,
+                                           max_query_len: int, max_seq_len: int, sliding_window: int = 0, sink_tokens: int = 0) -> int:
+    """Scratch that `paged_window_attention` takes for a batch of these bounds (0 for many)."""
+    return _lib.lib().mi355q_paged_window_attention_workspace_bytes(num_seqs, num_rows, num_heads, num_kv_heads, head_size, max_query_len,
+                                                                    max_seq_len, sliding_window, sink_tokens)
+
+
+def paged_window_attention(out: torch.Tensor, query: torch.Tensor, key_cache: torch.Tensor, value_cache: torch.Tensor, num_kv_heads: int,
+                           scale: float, block_tables: torch.Tensor, seq_lens: torch.Tensor, query_start_loc: torch.Tensor | None,
+                           max_query_len: int, max_seq_len: int, kv_cache_dtype: str, k_scale: torch.Tensor | None,
+                           v_scale: torch.Tensor | None, sliding_window: int = 0, sink_tokens: int = 0,
+                           workspace: torch.Tensor | None = None) -> None:
+    """Causal attention of rows of any query length over the paged cache: decode rows, drafts and prompt rows in one call.
+    A row at position p sees token t <= p with t > p - sliding_window (0: no window) or t < sink_tokens; a row that sees
+    nothing becomes zeros, rows of `out` behind the last sequence stay as they are.
+    out / query [rows, heads, head]; kv_cache_dtype "auto" (16 bits), "fp8" (k_scale / v_scale hold one value) or
+    "block_int8" / "block_fp8" (fp32 [blocks, kv_heads], as `rope_and_cache_blocks` leaves them).
+    query_start_loc int32 [S + 1], or None: one row per sequence.  max_query_len must bound the query lengths; max_seq_len
+    only decides how the work is cut.  Pages that no row sees are never looked at.  workspace: uint8 scratch of
+    `paged_window_attention_workspace_bytes`, not shared with calls that may overlap; by default taken from the allocator."""
+    what = "paged_window_attention"
+    _one_device(what, query, out, key_cache, value_cache, block_tables, seq_lens, query_start_loc, workspace)
+    if query.dim() != 3 or out.shape != query.shape or out.dtype != query.dtype:
+        raise RuntimeError(f"{what}: out and query must be [rows, heads, head] of one dtype")
+    rows, H, D = query.shape
+    if rows and (query.stride()[1:] != (D, 1) or out.stride()[1:] != (D, 1)):
+        raise RuntimeError(f"{what}: the heads of a row must be contiguous")
+    if block_tables.dtype != torch.int32 or seq_lens.dtype != torch.int32 or block_tables.dim() != 2 or not block_tables.is_contiguous():
+        raise RuntimeError(f"{what}: block_tables must be contiguous int32 [S, pages], seq_lens int32 [S]")
+    S = block_tables.shape[0]
+    if seq_lens.shape != (S,) or not seq_lens.is_contiguous():
+        raise RuntimeError(f"{what}: seq_lens must be contiguous int32 [{S}]")
+    if query_start_loc is not None and (query_start_loc.dtype != torch.int32 or query_start_loc.shape != (S + 1,)
+                                        or not query_start_loc.is_contiguous()):
+        raise RuntimeError(f"{what}: query_start_loc must be contiguous int32 [{S + 1}]")
+    if sliding_window < 0 or sink_tokens < 0:
+        raise RuntimeError(f"{what}: sliding_window and sink_tokens must not be negative")
+    if kv_cache_dtype in _BLOCK_CODES:
+        kv, element = _BLOCK_CODES[kv_cache_dtype], 1
+    elif _is_fp8(kv_cache_dtype):
+        kv, element = _lib.KV_FP8, 1
+    else:
+        kv, element = _lib.KV_16, 2
+        if key_cache.dtype != query.dtype or value_cache.dtype != query.dtype:
+            raise RuntimeError(f"{what}: a 16-bit cache must have the query's dtype")
+    kvh, bs = _paged_cache(what, key_cache, value_cache, D, element)
+    if kvh != num_kv_heads:
+        raise RuntimeError(f"{what}: {num_kv_heads} kv heads over a cache of {kvh}")
+    strides = (0, 0)
+    if element == 1:
+        if k_scale is None or v_scale is None:
+            raise RuntimeError(f"{what}: an 8-bit cache needs k_scale and v_scale")
+        _one_device(what, query, k_scale, v_scale)
+        if kv_cache_dtype in _BLOCK_CODES:
+            _block_scales(what, k_scale, v_scale, key_cache.shape[0], kvh)
+            strides = k_scale.stride()
+        elif k_scale.numel() != 1 or v_scale.numel() != 1 or k_scale.dtype != torch.float32 or v_scale.dtype != torch.float32:
+            raise RuntimeError(f"{what}: k_scale and v_scale of an fp8 cache are single fp32 values")
+    if rows == 0 or S == 0:
+        return
+    L = _lib.lib()
+    need = L.mi355q_paged_window_attention_workspace_bytes(S, rows, H, kvh, D, max_query_len, max_seq_len, sliding_window, sink_tokens)
+    if need and workspace is None:
+        workspace = torch.empty(need, dtype=torch.uint8, device=query.device)
+    _launch(query.device, L.mi355q_paged_window_attention, out.data_ptr(), out.stride(0), query.data_ptr(), query.stride(0),
+            key_cache.data_ptr(), value_cache.data_ptr(), key_cache.stride(0), key_cache.stride(1), key_cache.shape[0], rows, S, H, kvh, D,
+            scale, block_tables.data_ptr(), block_tables.shape[1], seq_lens.data_ptr(), _ptr(query_start_loc), max_query_len, bs,
+            max_seq_len, sliding_window, sink_tokens, _dt(query), kv, _ptr(k_scale) if element == 1 else None,
+            _ptr(v_scale) if element == 1 else None, strides[0], strides[1], _ptr(workspace),
+            0 if workspace is None else workspace.numel() * workspace.element_size())
+
+
+# ---------------------------------------------------------------------------
 # sampler inner loop
 # ---------------------------------------------------------------------------
 def argmax(logits: torch.Tensor, out: torch.Tensor | None = None) -> torch.Tensor:
