@@ -729,7 +729,7 @@ enum { MI355Q_KV_16 = 0, MI355Q_KV_FP8 = 1, MI355Q_KV_INT8 = 2 };
  * scale_head_stride].  code_type MI355Q_KV_INT8 (largest code 127) or MI355Q_KV_FP8 (e4m3fn, 448).
  *   query_out = rotated query (may be `query` itself); `key` is left as it was, the cache takes it rotated and rounded
  *   to dtype.  For a block that the call writes from offset `first` on:
- *     scale' = max(first > 0 ? scale : 0, largest |x| of the new tokens / largest code)
+ *     scale' = max(first > 0 ? scale : 0, largest |x| of the new tokens * (1 / largest code))
  *     codes below `first`: round(code * (scale / scale')) where the scale grew; new codes: round(x / scale').
  *   Writing offset 0 restarts a block.  A value that is not finite makes the scale NaN.
  * slot_mapping int64 [num_tokens]; slots outside [0, num_blocks * block_size) are skipped (their query is rotated all the

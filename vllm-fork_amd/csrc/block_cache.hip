@@ -5,7 +5,7 @@
 //
 // For a block b and head h that a call writes, with first = the smallest offset written:
 //   s_old = first > 0 ? scale[b, h] : 0          offset 0 restarts a block: what it held before is void
-//   s_new = max(s_old, max |x| / QMAX)           over the call's tokens in b
+//   s_new = max(s_old, max |x| * (1 / QMAX))     over the call's tokens in b
 //   codes at offsets < first become round(c * (s_old / s_new)) where s_new > s_old
 //   new codes are round(x / s_new), 0 where s_new is 0; other offsets keep their bytes.
 // A value that is not finite makes its block's scale NaN: reads of the block are NaN until it is restarted.
@@ -207,7 +207,7 @@ __device__ inline uint32_t wave_umax(uint32_t v) {
 template <typename DT>
 __device__ inline float scale_of(uint32_t bits, float qmax) {
   const uint32_t inf = DT::id == MI355Q_BF16 ? 0x7f80u : 0x7c00u;
-  return bits >= inf ? __builtin_nanf("") : DT::to_f32((uint16_t)bits) / qmax;
+  return bits >= inf ? __builtin_nanf("") : DT::to_f32((uint16_t)bits) * (1.0f / qmax);
 }
 
 template <bool INT8>

@@ -49,10 +49,13 @@ struct WindowParams {
   float scale;
   int num_seqs, num_rows, num_heads, num_kv_heads, group;
   int num_blocks, table_width;
+  int out16;                    // output rows start on 16 bytes
   int bs, page_magic;
   int window, sinks;            // window 0: none
   int splits, split_tiles;      // the context in stretches of split_tiles 64-token tiles, at most `splits` of them
-  int col_tiles;                // column tiles of the longest query
+  int part_stride;              // partial sums are laid out for so many stretches
+  int col_tiles;                // column tiles of the longest query that this launch serves
+  int min_cols, max_cols;       // sequences with fewer or more columns (rows x heads per kv head) are another launch's
 };
 
 __device__ inline int wa_page(int n, int magic) { return magic ? (int)__umulhi((unsigned)n, (unsigned)magic) : n; }
@@ -177,7 +180,7 @@ __global__ __launch_bounds__(256, 2) void window_rows_kernel(const WindowParams 
   const int start = p.starts ? p.starts[seq] : seq;
   const int qlen = p.starts ? p.starts[seq + 1] - start : 1;
   const int cols = min(qlen, p.num_rows - start) * G;
-  if (start < 0 || ct * 16 >= cols) return;
+  if (start < 0 || ct * 16 >= cols || cols > p.max_cols) return;
   const int seq_len = p.seq_lens[seq];
   const int c0 = ct * 16, c1 = min(c0 + 16, cols) - 1;
   const int pos0 = seq_len - qlen + c0 / G, pos1 = seq_len - qlen + c1 / G;
@@ -461,7 +464,7 @@ __global__ __launch_bounds__(256, 2) void window_rows_kernel(const WindowParams 
 #pragma unroll
     for (int i = 0; i < PER / 2; i++) out[i] = top == -INFINITY ? 0u : pack2<DT>(v[2 * i] * inv, v[2 * i + 1] * inv);
   } else {
-    const int64_t at = ((int64_t)orow * p.num_heads + ohead) * p.splits + split;
+    const int64_t at = ((int64_t)orow * p.num_heads + ohead) * p.part_stride + split;
 #pragma unroll
     for (int i = 0; i < PER; i += 4) *reinterpret_cast<f32x4*>(p.part_o + at * HEAD + d0 + i) = f32x4{v[i], v[i + 1], v[i + 2], v[i + 3]};
     if (d0 == 0) {
@@ -471,28 +474,488 @@ __global__ __launch_bounds__(256, 2) void window_rows_kernel(const WindowParams 
   }
 }
 
-// Joins the stretches of a long context: one wave per column (query row and head).
+// ---------------------------------------------------------------------------------------------------------------------
+// Many columns (prompt rows): one workgroup of NW waves per (sequence, 32 NW columns, kv head, stretch of the context), 32
+// columns a wave.  The workgroup brings a 64-token tile of K and V into LDS once, as 16-bit MFMA operands in lane order (codes
+// are widened on the way: once per workgroup instead of once per wave), two tiles deep: the codes of the tile after the next
+// are on their way in registers while this one is worked on.
+//
+// v_mfma_f32_32x32x16.  Row r of a 32-token tile of S^T is token r with bits 2 and 3 exchanged: the 8 logits a lane then holds
+// of each 16-token stretch are tokens 8 h .. 8 h + 7 of it (h = lane / 32), the B operand of O^T as they stand.  A stretch lies
+// in one block, so K's scale is wave-uniform per 8 registers and joins the factor of the exponent; V's scale is applied while
+// widening, as a factor relative to vref, with 2^7 in hand (fp16 then resolves blocks whose scales are 10^-6 of the largest
+// to all 11 bits).
+// ---------------------------------------------------------------------------------------------------------------------
+typedef __attribute__((ext_vector_type(16))) float f32x16;
+
+template <typename MT>
+__device__ inline f32x16 mfma32(u32x4 a, u32x4 b, f32x16 c);
+template <>
+__device__ inline f32x16 mfma32<BF16>(u32x4 a, u32x4 b, f32x16 c) {
+  return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+}
+template <>
+__device__ inline f32x16 mfma32<FP16>(u32x4 a, u32x4 b, f32x16 c) {
+  return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+}
+// max / sum over the two lanes that share a column
+__device__ inline float pair_max(float v) {
+  auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
+__device__ inline float pair_sum(float v) {
+  auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return __uint_as_float(r[0]) + __uint_as_float(r[1]);
+}
+// c + the two 16-bit values of w
+template <typename MT>
+__device__ inline float add_pair(uint32_t w, float c);
+template <>
+__device__ inline float add_pair<BF16>(uint32_t w, float c) {
+  return __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2, w), __builtin_bit_cast(bf16x2, BF16::ones), c, false);
+}
+template <>
+__device__ inline float add_pair<FP16>(uint32_t w, float c) {
+  return __builtin_amdgcn_fdot2(__builtin_bit_cast(wa_f16x2, w), __builtin_bit_cast(wa_f16x2, FP16::ones), c, false);
+}
+
+constexpr float WA_VSHIFT = 128.0f;
+
+template <typename DT, int KV, int HEAD, int NW>
+__global__ __launch_bounds__(64 * NW, 2) void window_flash_kernel(const WindowParams p) {
+  typedef typename MathOf<DT, KV>::T MT;
+  constexpr int EB = KV == KV16 ? 2 : 1, NT = 64 * NW, COLS = 32 * NW;
+  constexpr int KS = HEAD / 16, DTL = HEAD / 32;
+  constexpr int KBYTES = 64 * HEAD * 2, STAGE = 2 * KBYTES;
+  constexpr int PIECES = 64 * HEAD * EB / 16;        // 16-byte pieces of K in a tile, and as many of V
+  constexpr int PP = 2 * PIECES / NT;                // of both, per thread
+  constexpr int OLD = HEAD + 8;                      // output rows in LDS, padded
+  constexpr int LDS = 2 * STAGE > COLS * OLD * 2 ? 2 * STAGE : COLS * OLD * 2;
+  static_assert(2 * PIECES % NT == 0, "pieces are shared out evenly");
+  __shared__ __attribute__((aligned(1024))) unsigned char lds[LDS];
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int col = lane & 31, half = lane >> 5;
+
+  const int kvh = blockIdx.x % p.num_kv_heads;
+  int b = blockIdx.x / p.num_kv_heads;
+  const int split = b % p.splits;
+  b /= p.splits;
+  // a sequence's last rows, which see most under the causal mask, first
+  const int ct = p.col_tiles - 1 - b % p.col_tiles, seq = b / p.col_tiles;
+  const int G = p.group;
+  const int start = p.starts ? p.starts[seq] : seq;
+  const int qlen = p.starts ? p.starts[seq + 1] - start : 1;
+  const int cols = min(qlen, p.num_rows - start) * G;
+  if (start < 0 || ct * COLS >= cols || cols < p.min_cols) return;
+  const int seq_len = p.seq_lens[seq];
+  const int c0 = ct * COLS, c1 = min(c0 + COLS, cols) - 1;
+  const int pos0 = seq_len - qlen + c0 / G, pos1 = seq_len - qlen + c1 / G;
+  const Span span = span_of(p, pos0, pos1);
+  const int begin = split == 0 ? 0 : split * p.split_tiles;
+  const int end = split == p.splits - 1 ? span.tiles : min(begin + p.split_tiles, span.tiles);
+  if (split > 0 && begin >= end) return;
+  const bool whole = span.tiles <= p.split_tiles;
+  const int wg_low = p.window ? pos0 - p.window + 1 : INT_MIN;    // below it, only sinks are seen
+
+  // ---- this lane's query column ---------------------------------------------------------------------------------------
+  const int wc0 = c0 + wave * 32, wc1 = min(wc0 + 32, cols) - 1;  // the wave's columns (none: wc0 > wc1)
+  const int c = min(wc0 + col, c1);
+  const int row = start + c / G, head = kvh * G + c % G;
+  const int pos = seq_len - qlen + c / G;
+  const int wpos0 = seq_len - qlen + min(wc0, c1) / G, wpos1 = seq_len - qlen + min(wc0 + 31, c1) / G;
+  u32x4 qf[KS];
+  float qscale = fabsf(p.scale) * WA_LOG2E;
+  {
+    const uint16_t* qp = p.q + (int64_t)row * p.q_stride + (int64_t)head * HEAD + 8 * half;
+#pragma unroll
+    for (int s = 0; s < KS; s++) qf[s] = *reinterpret_cast<const u32x4*>(qp + 16 * s);
+    if constexpr (EB == 1 && DT::id == MI355Q_BF16) {
+      float top = 0.f;
+#pragma unroll
+      for (int s = 0; s < KS; s++)
+#pragma unroll
+        for (int e = 0; e < 4; e++)
+          top = fmaxf(top, fmaxf(fabsf(BF16::to_f32((uint16_t)qf[s][e])), fabsf(BF16::to_f32((uint16_t)(qf[s][e] >> 16)))));
+      top = pair_max(top);
+      int ex = (int)(__float_as_uint(top) >> 23);
+      ex = ex == 255 ? 140 : max(ex, 20);
+      const float up = __uint_as_float((uint32_t)(127 + 140 - ex) << 23);
+      qscale *= __uint_as_float((uint32_t)(ex - 13) << 23);
+#pragma unroll
+      for (int s = 0; s < KS; s++)
+#pragma unroll
+        for (int e = 0; e < 4; e++)
+          qf[s][e] = pack2<FP16>(BF16::to_f32((uint16_t)qf[s][e]) * up, BF16::to_f32((uint16_t)(qf[s][e] >> 16)) * up);
+    }
+    if (p.scale < 0.f) {   // the factor of the exponent stays positive
+#pragma unroll
+      for (int s = 0; s < KS; s++) qf[s] ^= u32x4{0x80008000u, 0x80008000u, 0x80008000u, 0x80008000u};
+    }
+  }
+
+  const int32_t* table = p.tables + (int64_t)seq * p.table_width;
+  const int blocks16 = p.bs >> 4;
+  const unsigned char* kc = p.kc + (int64_t)kvh * p.head_stride;
+  const unsigned char* vc = p.vc + (int64_t)kvh * p.head_stride;
+
+  // ---- a tile on its way: codes in registers, what its four 16-token stretches are scaled by -----------------------------
+  u32x4 piece[PP];
+  float ks_next[4], vs_next[4];
+  int ok_next = 0;          // stretches that hold a token somebody sees
+  auto is_k = [&](int i) { return (PIECES % NT == 0) ? i * NT < PIECES : i * NT + wave * 64 < PIECES; };
+  auto request = [&](int tile) {
+    const int t0 = span.base(tile), lim = span.limit(tile);
+    int64_t at[4];
+    int off[4];
+    ok_next = 0;
+#pragma unroll
+    for (int j = 0; j < 4; j++) {
+      const int n = min(t0 + 16 * j, (lim - 1) & ~15) >> 4;
+      const int pg = wa_page(n, p.page_magic);
+      const int blk = sload(table + pg);
+      off[j] = (n - pg * blocks16) * 16;
+      const bool in = (unsigned)blk < (unsigned)p.num_blocks;
+      at[j] = in ? blk : 0;
+      ok_next |= in && t0 + 16 * j < lim ? 1 << j : 0;
+    }
+    if constexpr (KV != KV16) {
+#pragma unroll
+      for (int j = 0; j < 4; j++) {
+        const int64_t si = at[j] * p.scale_block_stride + kvh * p.scale_head_stride;
+        ks_next[j] = sload(p.ks + si);
+        vs_next[j] = sload(p.vs + si);
+      }
+    }
+    const unsigned char* kb = kc;
+#pragma unroll
+    for (int j = 0; j < 4; j++)
+      if ((lane >> 4) == j) kb = kc + at[j] * p.block_stride + (int64_t)off[j] * 16;
+    kb += (lane & 15) * 16;
+#pragma unroll
+    for (int i = 0; i < PP; i++) {
+      const int n0 = i * NT + wave * 64;      // the wave's first piece
+      if (is_k(i)) {
+        piece[i] = *reinterpret_cast<const u32x4*>(kb + (int64_t)(n0 >> 6) * p.bs * 16);
+      } else {
+        const int m0 = n0 - PIECES;
+        int st, d, h = 0;
+        if constexpr (EB == 1) {
+          st = m0 / HEAD;
+          d = m0 % HEAD + lane;
+        } else {
+          st = m0 / (2 * HEAD);
+          d = m0 % (2 * HEAD) / 2 + col;
+          h = half;
+        }
+        int64_t a = 0;
+        int o = 0;
+#pragma unroll
+        for (int j = 0; j < 4; j++)
+          if (st == j) a = at[j], o = off[j];
+        piece[i] = *reinterpret_cast<const u32x4*>(vc + a * p.block_stride + ((int64_t)d * p.bs + o + 8 * h) * EB);
+      }
+    }
+  };
+  // the requested tile into LDS buffer `buf`, as operands; returns the vref its V is relative to
+  float vref = 0.f;
+  auto deliver = [&](int tile, int buf) {
+    const int t0 = span.base(tile), lim = span.limit(tile);
+    unsigned char* st0 = lds + buf * STAGE;
+    float ratio[4];
+    if constexpr (KV != KV16) {
+      float top = 0.f;
+#pragma unroll
+      for (int j = 0; j < 4; j++) top = fmaxf(top, (ok_next >> j) & 1 ? vs_next[j] : 0.f);
+      if (top > vref) vref = 2.f * top;
+#pragma unroll
+      for (int j = 0; j < 4; j++) ratio[j] = vref > 0.f ? vs_next[j] * (WA_VSHIFT / vref) : vs_next[j];
+    }
+    // tokens that no column of the workgroup sees are zeros in V, whatever their places hold
+    const bool full = ok_next == 15 && t0 + 64 <= lim && (t0 >= wg_low || t0 + 64 <= p.sinks);
+#pragma unroll
+    for (int i = 0; i < PP; i++) {
+      const int n0 = i * NT + wave * 64;
+      if (is_k(i)) {
+        const int ch = n0 >> 6, r = lane & 31;
+        const int rho = (r & 0x13) | ((r & 4) << 1) | ((r & 8) >> 1);
+        if constexpr (EB == 1) {
+          unsigned char* to = st0 + ((half * KS + ch) * 64 + rho) * 16;
+          *reinterpret_cast<u32x4*>(to) = widen8<KV>(piece[i], 0);
+          *reinterpret_cast<u32x4*>(to + 512) = widen8<KV>(piece[i], 1);
+        } else {
+          *reinterpret_cast<u32x4*>(st0 + ((half * KS + (ch >> 1)) * 64 + (ch & 1) * 32 + rho) * 16) = piece[i];
+        }
+      } else {
+        const int m0 = n0 - PIECES;
+        const int st = EB == 1 ? m0 / HEAD : m0 / (2 * HEAD);
+        const int d = EB == 1 ? m0 % HEAD + lane : m0 % (2 * HEAD) / 2 + col;
+        unsigned char* to = st0 + KBYTES + (((d >> 5) * 4 + st) * 64 + (d & 31)) * 16;
+        uint32_t seen = 0xffffu;
+        if (!full) {
+          seen = 0;
+#pragma unroll
+          for (int k = 0; k < 16; k++) {
+            const int t = t0 + 16 * st + k;
+            seen |= (t < lim && (t >= wg_low || t < p.sinks)) ? 1u << k : 0u;
+          }
+          if (!((ok_next >> st) & 1)) seen = 0;
+        }
+        auto cut = [&](u32x4 v, uint32_t m) {
+          if (!full) {
+#pragma unroll
+            for (int e = 0; e < 4; e++) v[e] &= ((m >> (2 * e)) & 1 ? 0xffffu : 0u) | ((m >> (2 * e)) & 2 ? 0xffff0000u : 0u);
+          }
+          return v;
+        };
+        if constexpr (EB == 1) {
+          float rs = 0.f;
+#pragma unroll
+          for (int j = 0; j < 4; j++)
+            if (st == j) rs = ratio[j];
+          const _Float16 r16 = (_Float16)rs;
+          const wa_f16x2 rr = {r16, r16};
+#pragma unroll
+          for (int h = 0; h < 2; h++) {
+            u32x4 v = widen8<KV>(piece[i], h);
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+              const uint32_t w = v[e];   // (a bit cast of the vector element itself would take element 0)
+              v[e] = __builtin_bit_cast(uint32_t, __builtin_bit_cast(wa_f16x2, w) * rr);
+            }
+            *reinterpret_cast<u32x4*>(to + h * 512) = cut(v, seen >> (8 * h));
+          }
+        } else {
+          *reinterpret_cast<u32x4*>(to + half * 512) = cut(piece[i], seen >> (8 * half));
+        }
+      }
+    }
+  };
+  auto arrive = [&]() {
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+  };
+
+  f32x16 o[DTL];
+#pragma unroll
+  for (int d = 0; d < DTL; d++)
+#pragma unroll
+    for (int e = 0; e < 16; e++) o[d][e] = 0.f;
+  float m = -INFINITY, l = 0.f, oref = 0.f;
+
+  float ks[4] = {0.f, 0.f, 0.f, 0.f}, vref_now = 0.f;
+  int ok = 0;
+  if (begin < end) {
+    request(begin);
+    deliver(begin, 0);
+    vref_now = vref;
+    ok = ok_next;
+#pragma unroll
+    for (int j = 0; j < 4; j++) ks[j] = ks_next[j];
+    if (begin + 1 < end) request(begin + 1);
+  }
+  for (int tile = begin; tile < end; tile++) {
+    const int buf = (tile - begin) & 1;
+    arrive();               // the tile is in place for every wave, and the other buffer is free
+    const unsigned char* st0 = lds + buf * STAGE;
+    const int t0 = span.base(tile), lim = span.limit(tile);
+    const bool more = tile + 1 < end;
+    // does any of the wave's columns see any of it?
+    const bool idle = wc0 > wc1 || t0 > wpos1 || (p.window && t0 + 63 <= wpos0 - p.window && t0 >= p.sinks) || ok == 0;
+
+    f32x16 s[2];
+    if (!idle) {
+#pragma unroll
+      for (int rt = 0; rt < 2; rt++) {
+#pragma unroll
+        for (int e = 0; e < 16; e++) s[rt][e] = 0.f;
+#pragma unroll
+        for (int k = 0; k < KS; k++) {
+          const u32x4 a = *reinterpret_cast<const u32x4*>(st0 + ((rt * KS + k) * 64 + lane) * 16);
+          s[rt] = mfma32<MT>(a, qf[k], s[rt]);
+        }
+      }
+    }
+    const float vref_tile = vref_now;
+    const int ok_tile = ok;
+    float f[4];
+#pragma unroll
+    for (int j = 0; j < 4; j++) f[j] = KV == KV16 ? qscale : qscale * ks[j];
+    if (more) {
+      deliver(tile + 1, buf ^ 1);
+      vref_now = vref;
+      ok = ok_next;
+#pragma unroll
+      for (int j = 0; j < 4; j++) ks[j] = ks_next[j];
+      if (tile + 2 < end) request(tile + 2);
+    }
+    if (idle) continue;
+
+    // ---- running softmax ----------------------------------------------------------------------------------------------
+    const bool inner = ok_tile == 15 && t0 + 64 <= lim && t0 + 63 <= wpos0 && (!p.window || t0 > wpos1 - p.window);
+    uint32_t seen = ~0u;     // bit 16 rt + register
+    if (!inner) {
+      seen = 0;
+      const int hi = min(pos, lim - 1) - t0 - 8 * half, lo = p.window ? pos - p.window + 1 - t0 - 8 * half : INT_MIN, sk = p.sinks - t0 - 8 * half;
+#pragma unroll
+      for (int e = 0; e < 32; e++) {
+        const int at = 32 * (e >> 4) + 16 * ((e >> 3) & 1) + (e & 7);
+        const bool yes = at <= hi && (at >= lo || at < sk) && ((ok_tile >> (e >> 3)) & 1);
+        seen |= yes ? 1u << e : 0u;
+        s[e >> 4][e & 15] = yes ? s[e >> 4][e & 15] : -INFINITY;
+      }
+    }
+    float mx = -INFINITY;
+#pragma unroll
+    for (int j = 0; j < 4; j++) {
+      float a = s[j >> 1][8 * (j & 1)];
+#pragma unroll
+      for (int e = 1; e < 8; e++) a = fmaxf(a, s[j >> 1][8 * (j & 1) + e]);
+      mx = fmaxf(mx, a == -INFINITY ? a : a * f[j]);
+    }
+    mx = pair_max(mx);
+    if (__any(mx > m + WA_LAG) || (KV != KV16 && vref_tile != oref)) {
+      const float mn = mx > m + WA_LAG ? mx : m;
+      float a = m == -INFINITY ? 0.f : exp2_fast(m - mn);
+      l *= a;
+      if constexpr (KV != KV16) {
+        if (vref_tile != oref) a *= oref / vref_tile;
+        oref = vref_tile;
+      }
+#pragma unroll
+      for (int d = 0; d < DTL; d++) o[d] *= a;
+      m = mn;
+    }
+    const float ms = (m == -INFINITY ? 0.f : m) - WA_SHIFT;
+    u32x4 pf[4];
+#pragma unroll
+    for (int j = 0; j < 4; j++) {
+#pragma unroll
+      for (int e = 0; e < 4; e++) {
+        float w[2];
+#pragma unroll
+        for (int u = 0; u < 2; u++) {
+          const int r = 2 * e + u;
+          float x = __builtin_fmaf(s[j >> 1][8 * (j & 1) + r], f[j], -ms);
+          w[u] = exp2_fast(x);
+          if (!inner) w[u] = (seen >> (8 * j + r)) & 1 ? w[u] : 0.f;
+        }
+        pf[j][e] = pack2<MT>(w[0], w[1]);
+        l = add_pair<MT>(pf[j][e], l);
+      }
+    }
+
+    // ---- O^T += V^T P^T -------------------------------------------------------------------------------------------------
+    const unsigned char* vt = st0 + KBYTES;
+    bool bad = false;
+    if (!inner) {
+#pragma unroll
+      for (int d = 0; d < DTL; d++)
+#pragma unroll
+        for (int st = 0; st < 4; st++) bad |= not_finite<MT>(*reinterpret_cast<const u32x4*>(vt + ((d * 4 + st) * 64 + lane) * 16));
+    }
+    if (!__any(bad)) {
+#pragma unroll
+      for (int d = 0; d < DTL; d++)
+#pragma unroll
+        for (int st = 0; st < 4; st++) {
+          const u32x4 a = *reinterpret_cast<const u32x4*>(vt + ((d * 4 + st) * 64 + lane) * 16);
+          o[d] = mfma32<MT>(a, pf[st], o[d]);
+        }
+    } else {
+      // an infinity or NaN that some columns may see and others must not: one token at a time, added where it is seen
+#pragma unroll 1
+      for (int n = 0; n < 64; n++) {
+        const int h = (n >> 3) & 1, i = n & 7;
+        const bool here = half == h;
+        const uint32_t theirs = (uint32_t)__shfl((int)seen, h * 32 + col, 64);
+#pragma unroll
+        for (int st = 0; st < 4; st++) {
+          if (st != n >> 4) continue;
+          const bool counts = (theirs >> (8 * st + i)) & 1;
+          const u32x4 pb = only<MT>(pf[st], here, i);
+#pragma unroll
+          for (int d = 0; d < DTL; d++) {
+            const u32x4 a = only<MT>(*reinterpret_cast<const u32x4*>(vt + ((d * 4 + st) * 64 + lane) * 16), here, i);
+            const f32x16 r = mfma32<MT>(a, pb, o[d]);
+#pragma unroll
+            for (int e = 0; e < 16; e++) o[d][e] = counts ? r[e] : o[d][e];
+          }
+        }
+      }
+    }
+  }
+
+  // ---- out ----------------------------------------------------------------------------------------------------------------
+  l = pair_sum(l);
+  const float unit = KV == KV16 ? 1.f : oref / WA_VSHIFT;
+  if (whole) {
+    arrive();               // the last tile has been read by every wave: LDS takes the output rows
+    const float inv = m == -INFINITY ? 0.f : unit / l;
+    uint16_t* mine = reinterpret_cast<uint16_t*>(lds) + (wave * 32 + col) * OLD;
+#pragma unroll
+    for (int d = 0; d < DTL; d++)
+#pragma unroll
+      for (int q = 0; q < 4; q++) {
+        u32x2 w;
+        w[0] = m == -INFINITY ? 0u : pack2<DT>(o[d][4 * q] * inv, o[d][4 * q + 1] * inv);
+        w[1] = m == -INFINITY ? 0u : pack2<DT>(o[d][4 * q + 2] * inv, o[d][4 * q + 3] * inv);
+        *reinterpret_cast<u32x2*>(mine + 32 * d + 8 * q + 4 * half) = w;
+      }
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");   // a wave reads back only what it wrote
+    constexpr int LPR = HEAD / 8;                        // lanes per row, 16 bytes each
+#pragma unroll
+    for (int i = 0; i < 32 / (64 / LPR); i++) {
+      const int r = i * (64 / LPR) + lane / LPR, d = lane % LPR * 8;
+      const int cc = wc0 + r;
+      if (cc > wc1) continue;
+      const u32x4 w = *reinterpret_cast<const u32x4*>(reinterpret_cast<uint16_t*>(lds) + (wave * 32 + r) * OLD + d);
+      uint16_t* to = p.out + (int64_t)(start + cc / G) * p.out_stride + (int64_t)(kvh * G + cc % G) * HEAD + d;
+      if (p.out16) *reinterpret_cast<u32x4*>(to) = w;
+      else
+#pragma unroll
+        for (int e = 0; e < 4; e++) reinterpret_cast<uint32_t*>(to)[e] = w[e];
+    }
+  } else if (wc0 + col <= wc1) {
+    const int64_t at = ((int64_t)row * p.num_heads + head) * p.part_stride + split;
+    float* to = p.part_o + at * HEAD + 4 * half;
+#pragma unroll
+    for (int d = 0; d < DTL; d++)
+#pragma unroll
+      for (int q = 0; q < 4; q++)
+        *reinterpret_cast<f32x4*>(to + 32 * d + 8 * q) =
+            f32x4{o[d][4 * q] * unit, o[d][4 * q + 1] * unit, o[d][4 * q + 2] * unit, o[d][4 * q + 3] * unit};
+    if (half == 0) {
+      p.part_ml[2 * at] = m;
+      p.part_ml[2 * at + 1] = l;
+    }
+  }
+}
+
+// Joins the stretches of a long context: one wave per column (query row and head).  COLS: columns of a workgroup of the
+// launch before, whose span decides how many stretches there are.
 template <typename DT, int HEAD>
-__global__ __launch_bounds__(256) void window_merge_kernel(const WindowParams p) {
+__global__ __launch_bounds__(256) void window_merge_kernel(const WindowParams p, int COLS) {
   constexpr int PER = HEAD / 64;
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   int b = blockIdx.x;
-  const int per_seq = (p.col_tiles * 16 + 3) / 4;
+  const int per_seq = p.col_tiles * COLS / 4;
   const int c = (b % per_seq) * 4 + wave;
   b /= per_seq;
   const int kvh = b % p.num_kv_heads, seq = b / p.num_kv_heads;
   const int start = p.starts ? p.starts[seq] : seq;
   const int qlen = p.starts ? p.starts[seq + 1] - start : 1;
   const int cols = min(qlen, p.num_rows - start) * p.group;
-  if (start < 0 || c >= cols) return;
+  if (start < 0 || c >= cols || cols < p.min_cols || cols > p.max_cols) return;
   const int seq_len = p.seq_lens[seq];
-  const int c0 = c & ~15, c1 = min(c0 + 16, cols) - 1;
+  const int c0 = c / COLS * COLS, c1 = min(c0 + COLS, cols) - 1;
   const Span span = span_of(p, seq_len - qlen + c0 / p.group, seq_len - qlen + c1 / p.group);
   if (span.tiles <= p.split_tiles) return;    // written by its only workgroup
   const int n = min(p.splits, (span.tiles + p.split_tiles - 1) / p.split_tiles);
   const int row = start + c / p.group, head = kvh * p.group + c % p.group;
-  const int64_t at = ((int64_t)row * p.num_heads + head) * p.splits;
+  const int64_t at = ((int64_t)row * p.num_heads + head) * p.part_stride;
   const float* ml = p.part_ml + 2 * at;
   const float* po = p.part_o + at * HEAD + lane * PER;
   float top = -INFINITY;
@@ -517,26 +980,76 @@ __global__ __launch_bounds__(256) void window_merge_kernel(const WindowParams p)
 // ---------------------------------------------------------------------------------------------------------------------
 // how a call is cut: host side, from what the caller bounds
 // ---------------------------------------------------------------------------------------------------------------------
-struct WindowPlan { int col_tiles, splits, split_tiles; };
+struct WindowPart { int col_tiles, splits, split_tiles; };
+struct WindowPlan {
+  WindowPart rows, flash;       // col_tiles 0: not launched
+  int part_stride;
+};
 
-static WindowPlan window_plan(int num_seqs, int num_heads, int num_kv_heads, int max_query_len, int max_seq_len, int window, int sinks) {
-  WindowPlan w;
-  const int G = num_heads / num_kv_heads;
-  w.col_tiles = (int)(((int64_t)max_query_len * G + 15) / 16);
-  // tiles that 16 columns see: the window of their first row, their own rows, an unaligned start, the sinks
+// columns (rows x heads per kv head) up to which a sequence is served 16 at a time
+constexpr int WA_ROWS_COLS = 64;
+constexpr int WA_WAVES = 8, WA_FLASH_COLS = 32 * WA_WAVES;
+
+static WindowPart window_part(int64_t max_cols, int cols, int G, int num_seqs, int num_kv_heads, int max_seq_len, int window, int sinks,
+                              int groups_wanted, int least_tiles) {
+  WindowPart w;
+  w.col_tiles = (int)((max_cols + cols - 1) / cols);
+  // tiles that `cols` columns see: the window of their first row, their own rows, an unaligned start, the sinks
   int64_t tiles = ((int64_t)max_seq_len + 63) / 64;
-  if (window) tiles = std::min(tiles + 1, ((int64_t)std::min(window, max_seq_len) + 16 + 15 + 63) / 64 + ((int64_t)std::min(sinks, max_seq_len) + 63) / 64);
+  if (window)
+    tiles = std::min(tiles + 1, ((int64_t)std::min(window, max_seq_len) + (cols + G - 1) / G + 15 + 63) / 64 +
+                                    ((int64_t)std::min(sinks, max_seq_len) + 63) / 64);
   tiles = std::max<int64_t>(tiles, 1);
   const int64_t groups = (int64_t)num_seqs * num_kv_heads * w.col_tiles;
-  // enough workgroups for four on each of the 256 CUs, at least 4 tiles (one per wave) in each
-  const int64_t want = std::max<int64_t>(1, (1024 + groups - 1) / groups);
-  w.split_tiles = (int)std::max<int64_t>(4, (tiles + want - 1) / want);
+  const int64_t want = std::max<int64_t>(1, (groups_wanted + groups - 1) / groups);
+  w.split_tiles = (int)std::max<int64_t>(least_tiles, (tiles + want - 1) / want);
   w.splits = (int)((tiles + w.split_tiles - 1) / w.split_tiles);
   return w;
 }
 
+static WindowPlan window_plan(int num_seqs, int num_rows, int num_heads, int num_kv_heads, int max_query_len, int max_seq_len, int window, int sinks) {
+  WindowPlan w{};
+  const int G = num_heads / num_kv_heads;
+  const int64_t cols = (int64_t)max_query_len * G;
+  const bool prompts = cols > WA_ROWS_COLS;
+  // a batch whose sequences all have max_query_len rows needs one kind only
+  if (!prompts || (int64_t)num_seqs * max_query_len != num_rows)
+    // four workgroups for each of the 256 CUs, at least 4 tiles (one per wave) in each
+    w.rows = window_part(std::min<int64_t>(cols, WA_ROWS_COLS), 16, G, num_seqs, num_kv_heads, max_seq_len, window, sinks, 1024, 4);
+  if (prompts) w.flash = window_part(cols, WA_FLASH_COLS, G, num_seqs, num_kv_heads, max_seq_len, window, sinks, 256, 16);
+  w.part_stride = std::max(w.rows.splits, w.flash.splits);
+  return w;
+}
+
 static size_t window_workspace(const WindowPlan& w, int num_rows, int num_heads, int head_size) {
-  return w.splits == 1 ? 0 : (size_t)num_rows * num_heads * w.splits * (head_size + 2) * sizeof(float);
+  return w.part_stride <= 1 ? 0 : (size_t)num_rows * num_heads * w.part_stride * (head_size + 2) * sizeof(float);
+}
+
+template <typename DT, int KV, int HEAD>
+static int launch_window(WindowParams p, const WindowPlan& w, hipStream_t s) {
+  auto groups = [&](const WindowPart& a) { return (int64_t)p.num_seqs * p.num_kv_heads * a.col_tiles * a.splits; };
+  auto merges = [&](const WindowPart& a, int cols) { return (int64_t)p.num_seqs * p.num_kv_heads * a.col_tiles * (cols / 4); };
+  const int64_t most = (int64_t)1 << 31;
+  MI355Q_REQUIRE(groups(w.rows) < most && groups(w.flash) < most && merges(w.rows, 16) < most && merges(w.flash, WA_FLASH_COLS) < most,
+                 "paged_window_attention: too many workgroups");
+  for (int kind = 0; kind < 2; kind++) {
+    const WindowPart& a = kind ? w.flash : w.rows;
+    if (!a.col_tiles) continue;
+    p.col_tiles = a.col_tiles, p.splits = a.splits;
+    p.split_tiles = a.splits == 1 ? INT_MAX : a.split_tiles;
+    p.min_cols = kind ? WA_ROWS_COLS + 1 : 0;
+    p.max_cols = kind ? INT_MAX : WA_ROWS_COLS;
+    const dim3 grid((unsigned)groups(a));
+    if (kind) hipLaunchKernelGGL((window_flash_kernel<DT, KV, HEAD, WA_WAVES>), grid, dim3(64 * WA_WAVES), 0, s, p);
+    else hipLaunchKernelGGL((window_rows_kernel<DT, KV, HEAD>), grid, dim3(256), 0, s, p);
+    if (int e = check_launch("paged_window_attention")) return e;
+    if (a.splits > 1) {
+      const int cols = kind ? WA_FLASH_COLS : 16;
+      hipLaunchKernelGGL((window_merge_kernel<DT, HEAD>), dim3((unsigned)merges(a, cols)), dim3(256), 0, s, p, cols);
+      if (int e = check_launch("paged_window_attention")) return e;
+    }
+  }
+  return MI355Q_OK;
 }
 
 }  // namespace mi355q
@@ -546,7 +1059,8 @@ using namespace mi355q;
 extern "C" size_t mi355q_paged_window_attention_workspace_bytes(int num_seqs, int num_rows, int num_heads, int num_kv_heads, int head_size,
                                                                 int max_query_len, int max_seq_len, int window, int sinks) {
   if (num_seqs <= 0 || num_rows <= 0 || num_kv_heads <= 0 || num_heads <= 0 || max_query_len <= 0 || max_seq_len <= 0) return 0;
-  return window_workspace(window_plan(num_seqs, num_heads, num_kv_heads, max_query_len, max_seq_len, window, sinks), num_rows, num_heads, head_size);
+  return window_workspace(window_plan(num_seqs, num_rows, num_heads, num_kv_heads, max_query_len, max_seq_len, window, sinks), num_rows, num_heads,
+                          head_size);
 }
 
 extern "C" int mi355q_paged_window_attention(void* out, int64_t out_stride, const void* query, int64_t q_stride, const void* key_cache,
@@ -578,7 +1092,7 @@ extern "C" int mi355q_paged_window_attention(void* out, int64_t out_stride, cons
   MI355Q_REQUIRE((((uintptr_t)key_cache | (uintptr_t)value_cache | (uintptr_t)query) & 15) == 0 && q_stride % 8 == 0,
                  "paged_window_attention: caches and query rows must be 16-byte aligned");
   MI355Q_REQUIRE(((uintptr_t)out & 3) == 0 && out_stride % 2 == 0, "paged_window_attention: output rows must be 4-byte aligned");
-  const WindowPlan w = window_plan(num_seqs, num_heads, num_kv_heads, max_query_len, max_seq_len, window, sinks);
+  const WindowPlan w = window_plan(num_seqs, num_rows, num_heads, num_kv_heads, max_query_len, max_seq_len, window, sinks);
   const size_t need = window_workspace(w, num_rows, num_heads, head_size);
   if (need && (!workspace || workspace_bytes < need))
     return set_error(MI355Q_ENOSPACE, "paged_window_attention: workspace of %zu bytes, %zu needed", workspace ? workspace_bytes : (size_t)0, need);
@@ -591,7 +1105,7 @@ extern "C" int mi355q_paged_window_attention(void* out, int64_t out_stride, cons
   p.ks = k_scale, p.vs = v_scale;
   p.tables = block_tables, p.seq_lens = seq_lens, p.starts = query_start_loc;
   p.part_o = (float*)workspace;
-  p.part_ml = (float*)workspace + (size_t)num_rows * num_heads * w.splits * head_size;
+  p.part_ml = (float*)workspace + (size_t)num_rows * num_heads * w.part_stride * head_size;
   p.out_stride = out_stride, p.q_stride = q_stride;
   p.block_stride = kv_block_stride * eb, p.head_stride = kv_head_stride * eb;
   p.scale_block_stride = scale_block_stride, p.scale_head_stride = scale_head_stride;
@@ -602,32 +1116,13 @@ extern "C" int mi355q_paged_window_attention(void* out, int64_t out_stride, cons
   const int pieces = block_size / 16;
   p.page_magic = pieces == 1 ? 0 : (int)(((1ull << 32) + pieces - 1) / pieces);
   p.window = std::min(window, 1 << 30), p.sinks = sinks;
-  p.splits = w.splits, p.split_tiles = w.splits == 1 ? INT_MAX : w.split_tiles, p.col_tiles = w.col_tiles;
-  const int64_t groups = (int64_t)num_seqs * num_kv_heads * w.col_tiles * w.splits;
-  const int64_t merges = (int64_t)num_seqs * num_kv_heads * (w.col_tiles * 4);
-  MI355Q_REQUIRE(groups < (int64_t)1 << 31 && merges < (int64_t)1 << 31, "paged_window_attention: too many workgroups");
+  p.part_stride = w.part_stride;
+  p.out16 = ((uintptr_t)out & 15) == 0 && out_stride % 8 == 0;
   hipStream_t s = (hipStream_t)stream;
-#define ROWS(DT, KV, HD) hipLaunchKernelGGL((window_rows_kernel<DT, KV, HD>), dim3((unsigned)groups), dim3(256), 0, s, p)
-#define MERGE(DT, HD) hipLaunchKernelGGL((window_merge_kernel<DT, HD>), dim3((unsigned)merges), dim3(256), 0, s, p)
-#define BY_KV(DT, HD)                                                \
-  do {                                                               \
-    if (kv_type == MI355Q_KV_16) ROWS(DT, KV16, HD);                 \
-    else if (kv_type == MI355Q_KV_FP8) ROWS(DT, KVF8, HD);           \
-    else ROWS(DT, KVI8, HD);                                         \
-    if (w.splits > 1) {                                              \
-      if (int e = check_launch("window_rows_kernel")) return e;      \
-      MERGE(DT, HD);                                                 \
-    }                                                                \
-  } while (0)
-  if (dtype == MI355Q_BF16) {
-    if (head_size == 128) BY_KV(BF16, 128);
-    else BY_KV(BF16, 64);
-  } else {
-    if (head_size == 128) BY_KV(FP16, 128);
-    else BY_KV(FP16, 64);
-  }
+#define BY_KV(DT, HD)                                                                                                     \
+  (kv_type == MI355Q_KV_16 ? launch_window<DT, KV16, HD>(p, w, s)                                                        \
+                           : kv_type == MI355Q_KV_FP8 ? launch_window<DT, KVF8, HD>(p, w, s) : launch_window<DT, KVI8, HD>(p, w, s))
+  if (dtype == MI355Q_BF16) return head_size == 128 ? BY_KV(BF16, 128) : BY_KV(BF16, 64);
+  return head_size == 128 ? BY_KV(FP16, 128) : BY_KV(FP16, 64);
 #undef BY_KV
-#undef MERGE
-#undef ROWS
-  return check_launch("paged_window_attention");
 }
