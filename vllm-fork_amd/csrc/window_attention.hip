@@ -18,6 +18,7 @@
 #include <math.h>
 
 #include <algorithm>
+#include <type_traits>
 
 #include "common.h"
 
@@ -177,11 +178,11 @@ __global__ __launch_bounds__(256, 2) void window_rows_kernel(const WindowParams 
   const int ct = b % p.col_tiles, seq = b / p.col_tiles;
   const int G = p.group;
 
-  const int start = p.starts ? p.starts[seq] : seq;
-  const int qlen = p.starts ? p.starts[seq + 1] - start : 1;
+  const int start = p.starts ? sload(p.starts + seq) : seq;
+  const int qlen = p.starts ? sload(p.starts + seq + 1) - start : 1;
   const int cols = min(qlen, p.num_rows - start) * G;
   if (start < 0 || ct * 16 >= cols || cols > p.max_cols) return;
-  const int seq_len = p.seq_lens[seq];
+  const int seq_len = sload(p.seq_lens + seq);
   const int c0 = ct * 16, c1 = min(c0 + 16, cols) - 1;
   const int pos0 = seq_len - qlen + c0 / G, pos1 = seq_len - qlen + c1 / G;
   const Span span = span_of(p, pos0, pos1);
@@ -532,7 +533,16 @@ __global__ __launch_bounds__(64 * NW, 2) void window_flash_kernel(const WindowPa
   constexpr int OLD = HEAD + 8;                      // output rows in LDS, padded
   constexpr int LDS = 2 * STAGE > COLS * OLD * 2 ? 2 * STAGE : COLS * OLD * 2;
   static_assert(2 * PIECES % NT == 0, "pieces are shared out evenly");
+  constexpr int CHUNK = 64;
+  struct Chunk {
+    u32x4 at[4 * CHUNK];      // per stretch: block offset (64 bits), token offset in the block, tokens somebody sees
+    float ks[4 * CHUNK], vs[4 * CHUNK];
+    int ok[CHUNK];            // per tile: stretches whose page exists and that begin before the end
+    float vref;
+  };
   __shared__ __attribute__((aligned(1024))) unsigned char lds[LDS];
+  __shared__ __attribute__((aligned(16))) Chunk chunks[2];
+  __shared__ int bad_tile[2];   // a tile (from 1) with a V that is not finite and that some columns see in part
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int col = lane & 31, half = lane >> 5;
@@ -544,11 +554,11 @@ __global__ __launch_bounds__(64 * NW, 2) void window_flash_kernel(const WindowPa
   // a sequence's last rows, which see most under the causal mask, first
   const int ct = p.col_tiles - 1 - b % p.col_tiles, seq = b / p.col_tiles;
   const int G = p.group;
-  const int start = p.starts ? p.starts[seq] : seq;
-  const int qlen = p.starts ? p.starts[seq + 1] - start : 1;
+  const int start = p.starts ? sload(p.starts + seq) : seq;
+  const int qlen = p.starts ? sload(p.starts + seq + 1) - start : 1;
   const int cols = min(qlen, p.num_rows - start) * G;
   if (start < 0 || ct * COLS >= cols || cols < p.min_cols) return;
-  const int seq_len = p.seq_lens[seq];
+  const int seq_len = sload(p.seq_lens + seq);
   const int c0 = ct * COLS, c1 = min(c0 + COLS, cols) - 1;
   const int pos0 = seq_len - qlen + c0 / G, pos1 = seq_len - qlen + c1 / G;
   const Span span = span_of(p, pos0, pos1);
@@ -599,136 +609,158 @@ __global__ __launch_bounds__(64 * NW, 2) void window_flash_kernel(const WindowPa
   const unsigned char* kc = p.kc + (int64_t)kvh * p.head_stride;
   const unsigned char* vc = p.vc + (int64_t)kvh * p.head_stride;
 
-  // ---- a tile on its way: codes in registers, what its four 16-token stretches are scaled by -----------------------------
-  u32x4 piece[PP];
-  float ks_next[4], vs_next[4];
-  int ok_next = 0;          // stretches that hold a token somebody sees
-  auto is_k = [&](int i) { return (PIECES % NT == 0) ? i * NT < PIECES : i * NT + wave * 64 < PIECES; };
-  auto request = [&](int tile) {
-    const int t0 = span.base(tile), lim = span.limit(tile);
-    int64_t at[4];
-    int off[4];
-    ok_next = 0;
+  // the tiles that every column sees whole: past the sinks and the window's moving start, before the moving end (numbered from
+  // `begin`, like every tile below)
+  const int tiles = end - begin;
+  int in0, in1;
+  {
+    const int first = p.window ? span.sink_tiles + max(0, pos1 - p.window + 1 - span.low + 63) / 64 : span.sink_tiles;
+    const int to = min(pos0, span.end - 1) - 63 - span.low;
+    in0 = max(0, min(tiles, first - begin));
+    in1 = max(in0, min(tiles, span.sink_tiles + (to < 0 ? 0 : to / 64 + 1) - begin));
+  }
+
+  // ---- where the tiles lie -------------------------------------------------------------------------------------------------
+  // Looked up CHUNK tiles at a time by one wave, a 16-token stretch per lane, into LDS (two chunks, so that the next one is
+  // there before it is needed): the loop itself then has no page arithmetic, and V's scales have one reference per chunk.
+  auto fill = [&](int first) {
+    Chunk& ch = chunks[(first - begin) / CHUNK & 1];
+    float v[CHUNK / 16], top = 0.f;
 #pragma unroll
-    for (int j = 0; j < 4; j++) {
-      const int n = min(t0 + 16 * j, (lim - 1) & ~15) >> 4;
-      const int pg = wa_page(n, p.page_magic);
-      const int blk = sload(table + pg);
-      off[j] = (n - pg * blocks16) * 16;
+    for (int i = 0; i < CHUNK / 16; i++) {
+      const int n = 64 * i + lane, j = n & 3, tile = min(first + (n >> 2), end - 1);
+      const int t0 = span.base(tile), lim = span.limit(tile), t = t0 + 16 * j;
+      const int n16 = min(t, (lim - 1) & ~15) >> 4;           // past the end: the last stretch again, masked
+      const int pg = wa_page(n16, p.page_magic);
+      const int blk = table[pg];
       const bool in = (unsigned)blk < (unsigned)p.num_blocks;
-      at[j] = in ? blk : 0;
-      ok_next |= in && t0 + 16 * j < lim ? 1 << j : 0;
+      const int64_t at = in ? blk : 0;
+      // tokens that some column of the workgroup sees
+      auto below = [&](int k) { return k <= 0 ? 0u : k >= 16 ? 0xffffu : (1u << k) - 1; };
+      uint32_t seen = below(lim - t);
+      if (p.window) seen &= ~below(wg_low - t) | below(p.sinks - t);
+      if (!in) seen = 0;
+      const uint64_t ok = __ballot(in && t < lim);
+      v[i] = 0.f;
+      if constexpr (KV != KV16) {
+        const int64_t si = at * p.scale_block_stride + kvh * p.scale_head_stride;
+        ch.ks[n] = in ? p.ks[si] : 1.f;
+        v[i] = seen ? p.vs[si] : 0.f;
+        top = fmaxf(top, v[i]);
+      }
+      const int64_t byte = at * p.block_stride;
+      ch.at[n] = u32x4{(uint32_t)byte, (uint32_t)(byte >> 32), (uint32_t)((n16 - pg * blocks16) * 16), seen};
+      if (j == 0) ch.ok[n >> 2] = (int)(ok >> (lane & ~3)) & 15;
     }
     if constexpr (KV != KV16) {
+      top = wave_max(top);
+      if (first > begin) top = fmaxf(top, chunks[((first - begin) / CHUNK & 1) ^ 1].vref);   // never falls
+      const float inv = top > 0.f ? WA_VSHIFT / top : 0.f;
 #pragma unroll
-      for (int j = 0; j < 4; j++) {
-        const int64_t si = at[j] * p.scale_block_stride + kvh * p.scale_head_stride;
-        ks_next[j] = sload(p.ks + si);
-        vs_next[j] = sload(p.vs + si);
-      }
-    }
-    const unsigned char* kb = kc;
-#pragma unroll
-    for (int j = 0; j < 4; j++)
-      if ((lane >> 4) == j) kb = kc + at[j] * p.block_stride + (int64_t)off[j] * 16;
-    kb += (lane & 15) * 16;
-#pragma unroll
-    for (int i = 0; i < PP; i++) {
-      const int n0 = i * NT + wave * 64;      // the wave's first piece
-      if (is_k(i)) {
-        piece[i] = *reinterpret_cast<const u32x4*>(kb + (int64_t)(n0 >> 6) * p.bs * 16);
-      } else {
-        const int m0 = n0 - PIECES;
-        int st, d, h = 0;
-        if constexpr (EB == 1) {
-          st = m0 / HEAD;
-          d = m0 % HEAD + lane;
-        } else {
-          st = m0 / (2 * HEAD);
-          d = m0 % (2 * HEAD) / 2 + col;
-          h = half;
-        }
-        int64_t a = 0;
-        int o = 0;
-#pragma unroll
-        for (int j = 0; j < 4; j++)
-          if (st == j) a = at[j], o = off[j];
-        piece[i] = *reinterpret_cast<const u32x4*>(vc + a * p.block_stride + ((int64_t)d * p.bs + o + 8 * h) * EB);
-      }
+      for (int i = 0; i < CHUNK / 16; i++) ch.vs[64 * i + lane] = v[i] * inv + (v[i] - v[i]);   // (a NaN stays one where top is 0)
+      if (lane == 0) ch.vref = top;
     }
   };
-  // the requested tile into LDS buffer `buf`, as operands; returns the vref its V is relative to
-  float vref = 0.f;
-  auto deliver = [&](int tile, int buf) {
-    const int t0 = span.base(tile), lim = span.limit(tile);
-    unsigned char* st0 = lds + buf * STAGE;
-    float ratio[4];
-    if constexpr (KV != KV16) {
-      float top = 0.f;
+
+  // ---- a tile on its way -------------------------------------------------------------------------------------------------
+  // A wave fetches PP groups of 64 pieces, all of one 16-token stretch jw: the address is one scalar base and offsets that
+  // never change.  K group: 16 tokens x 4 chunks of 16 bytes; V group: 64 head dims (8-bit), or 32 x 2 halves.
+  u32x4 piece[PP];
+  constexpr int GROUPS = PIECES / 64, GPJ = GROUPS / 4, KPP = PP > 1 ? PP / 2 : 1;
+  const bool fetches_k = PP > 1 || wave < NW / 2;       // (PP 1: half the waves fetch K, half V)
+  const int g0 = PP > 1 ? wave * KPP : wave % (NW / 2); // the wave's first K group and first V group
+  const int jw = g0 / GPJ;
+  static_assert(PP == 1 || GPJ % KPP == 0, "a wave's groups lie in one stretch");
+  int koff[KPP], voff[KPP];
 #pragma unroll
-      for (int j = 0; j < 4; j++) top = fmaxf(top, (ok_next >> j) & 1 ? vs_next[j] : 0.f);
-      if (top > vref) vref = 2.f * top;
+  for (int i = 0; i < KPP; i++) {
+    const int q = (g0 + i) % GPJ;
+    koff[i] = ((q * 4 + (lane >> 4)) * p.bs + (lane & 15)) * 16;
+    voff[i] = (EB == 1 ? q * 64 + lane : q * 32 + col) * p.bs * EB + (EB == 2 ? 16 * half : 0);
+  }
+  auto chunk_of = [&](int n) -> Chunk& { return chunks[n / CHUNK & 1]; };   // n: tile - begin
+  auto request = [&](int n) {
+    const u32x4 e = chunk_of(n).at[n % CHUNK * 4 + jw];
+    const uint32_t lo = __builtin_amdgcn_readfirstlane(e[0]), hi = __builtin_amdgcn_readfirstlane(e[1]);
+    const uint32_t off = __builtin_amdgcn_readfirstlane(e[2]);
+    const int64_t at = (int64_t)((uint64_t)hi << 32 | lo);
+    const unsigned char* kb = kc + at + off * 16;
+    const unsigned char* vb = vc + at + off * EB;
+    if constexpr (PP > 1) {
 #pragma unroll
-      for (int j = 0; j < 4; j++) ratio[j] = vref > 0.f ? vs_next[j] * (WA_VSHIFT / vref) : vs_next[j];
+      for (int i = 0; i < KPP; i++) {
+        piece[i] = *reinterpret_cast<const u32x4*>(kb + (unsigned)koff[i]);
+        piece[KPP + i] = *reinterpret_cast<const u32x4*>(vb + (unsigned)voff[i]);
+      }
+    } else {
+      piece[0] = *reinterpret_cast<const u32x4*>((fetches_k ? kb : vb) + (unsigned)(fetches_k ? koff[0] : voff[0]));
     }
-    // tokens that no column of the workgroup sees are zeros in V, whatever their places hold
-    const bool full = ok_next == 15 && t0 + 64 <= lim && (t0 >= wg_low || t0 + 64 <= p.sinks);
+  };
+  // the requested tile into LDS, as operands
+  const int rho = ((lane & 3) | ((lane & 4) << 1) | ((lane & 8) >> 1)) + 16 * (jw & 1);   // K row of this lane's token
+  auto deliver = [&](int n) {
+    unsigned char* to = lds + (n & 1) * STAGE;
+    auto put_k = [&](int i, u32x4 w) {
+      const int ch = (g0 + i) % GPJ * 4 + (lane >> 4);      // 16-byte chunk of the head
+      if constexpr (EB == 1) {
+        unsigned char* at = to + (((jw >> 1) * KS + ch) * 64 + rho) * 16;
+        *reinterpret_cast<u32x4*>(at) = widen8<KV>(w, 0);
+        *reinterpret_cast<u32x4*>(at + 512) = widen8<KV>(w, 1);
+      } else {
+        *reinterpret_cast<u32x4*>(to + (((jw >> 1) * KS + (ch >> 1)) * 64 + (ch & 1) * 32 + rho) * 16) = w;
+      }
+    };
+    auto put_v = [&](int i, u32x4 w) {
+      const int d = (g0 + i) % GPJ * (EB == 1 ? 64 : 32) + (EB == 1 ? lane : col);
+      unsigned char* at = to + KBYTES + (((d >> 5) * 4 + jw) * 64 + (d & 31)) * 16;
+      const int e0 = n % CHUNK * 4 + jw;
+      // tokens that no column of the workgroup sees are zeros in V, whatever their places hold
+      const uint32_t seen = __builtin_amdgcn_readfirstlane(chunk_of(n).at[e0][3]);
+      u32x4 v[EB == 1 ? 2 : 1];
+      if constexpr (EB == 1) {
+        const _Float16 r16 = (_Float16)chunk_of(n).vs[e0];
+        const wa_f16x2 rr = {r16, r16};
 #pragma unroll
-    for (int i = 0; i < PP; i++) {
-      const int n0 = i * NT + wave * 64;
-      if (is_k(i)) {
-        const int ch = n0 >> 6, r = lane & 31;
-        const int rho = (r & 0x13) | ((r & 4) << 1) | ((r & 8) >> 1);
-        if constexpr (EB == 1) {
-          unsigned char* to = st0 + ((half * KS + ch) * 64 + rho) * 16;
-          *reinterpret_cast<u32x4*>(to) = widen8<KV>(piece[i], 0);
-          *reinterpret_cast<u32x4*>(to + 512) = widen8<KV>(piece[i], 1);
-        } else {
-          *reinterpret_cast<u32x4*>(st0 + ((half * KS + (ch >> 1)) * 64 + (ch & 1) * 32 + rho) * 16) = piece[i];
+        for (int h = 0; h < 2; h++) {
+          v[h] = widen8<KV>(w, h);
+#pragma unroll
+          for (int e = 0; e < 4; e++) {
+            const uint32_t x = v[h][e];   // (a bit cast of the vector element itself would take element 0)
+            v[h][e] = __builtin_bit_cast(uint32_t, __builtin_bit_cast(wa_f16x2, x) * rr);
+          }
         }
       } else {
-        const int m0 = n0 - PIECES;
-        const int st = EB == 1 ? m0 / HEAD : m0 / (2 * HEAD);
-        const int d = EB == 1 ? m0 % HEAD + lane : m0 % (2 * HEAD) / 2 + col;
-        unsigned char* to = st0 + KBYTES + (((d >> 5) * 4 + st) * 64 + (d & 31)) * 16;
-        uint32_t seen = 0xffffu;
-        if (!full) {
-          seen = 0;
+        v[0] = w;
+      }
+      if (seen != 0xffffu) {
 #pragma unroll
-          for (int k = 0; k < 16; k++) {
-            const int t = t0 + 16 * st + k;
-            seen |= (t < lim && (t >= wg_low || t < p.sinks)) ? 1u << k : 0u;
-          }
-          if (!((ok_next >> st) & 1)) seen = 0;
-        }
-        auto cut = [&](u32x4 v, uint32_t m) {
-          if (!full) {
+        for (int h = 0; h < (EB == 1 ? 2 : 1); h++) {
+          const uint32_t mask = EB == 1 ? seen >> (8 * h) : seen >> (8 * half);
 #pragma unroll
-            for (int e = 0; e < 4; e++) v[e] &= ((m >> (2 * e)) & 1 ? 0xffffu : 0u) | ((m >> (2 * e)) & 2 ? 0xffff0000u : 0u);
-          }
-          return v;
-        };
-        if constexpr (EB == 1) {
-          float rs = 0.f;
-#pragma unroll
-          for (int j = 0; j < 4; j++)
-            if (st == j) rs = ratio[j];
-          const _Float16 r16 = (_Float16)rs;
-          const wa_f16x2 rr = {r16, r16};
-#pragma unroll
-          for (int h = 0; h < 2; h++) {
-            u32x4 v = widen8<KV>(piece[i], h);
-#pragma unroll
-            for (int e = 0; e < 4; e++) {
-              const uint32_t w = v[e];   // (a bit cast of the vector element itself would take element 0)
-              v[e] = __builtin_bit_cast(uint32_t, __builtin_bit_cast(wa_f16x2, w) * rr);
-            }
-            *reinterpret_cast<u32x4*>(to + h * 512) = cut(v, seen >> (8 * h));
-          }
-        } else {
-          *reinterpret_cast<u32x4*>(to + half * 512) = cut(piece[i], seen >> (8 * half));
+          for (int e = 0; e < 4; e++) v[h][e] &= ((mask >> (2 * e)) & 1 ? 0xffffu : 0u) | ((mask >> (2 * e)) & 2 ? 0xffff0000u : 0u);
         }
       }
+      if (n < in0 || n >= in1) {
+        bool bad = not_finite<MT>(v[0]);
+        if constexpr (EB == 1) bad |= not_finite<MT>(v[1]);
+        if (__any(bad)) bad_tile[n & 1] = n + 1;
+      }
+      if constexpr (EB == 1) {
+        *reinterpret_cast<u32x4*>(at) = v[0];
+        *reinterpret_cast<u32x4*>(at + 512) = v[1];
+      } else {
+        *reinterpret_cast<u32x4*>(at + half * 512) = v[0];
+      }
+    };
+    if constexpr (PP > 1) {
+#pragma unroll
+      for (int i = 0; i < KPP; i++) {
+        put_k(i, piece[i]);
+        put_v(i, piece[KPP + i]);
+      }
+    } else {
+      if (fetches_k) put_k(0, piece[0]);
+      else put_v(0, piece[0]);
     }
   };
   auto arrive = [&]() {
@@ -744,25 +776,28 @@ __global__ __launch_bounds__(64 * NW, 2) void window_flash_kernel(const WindowPa
     for (int e = 0; e < 16; e++) o[d][e] = 0.f;
   float m = -INFINITY, l = 0.f, oref = 0.f;
 
-  float ks[4] = {0.f, 0.f, 0.f, 0.f}, vref_now = 0.f;
-  int ok = 0;
-  if (begin < end) {
-    request(begin);
-    deliver(begin, 0);
-    vref_now = vref;
-    ok = ok_next;
-#pragma unroll
-    for (int j = 0; j < 4; j++) ks[j] = ks_next[j];
-    if (begin + 1 < end) request(begin + 1);
+  if (tiles > 0) {
+    if (wave == 0) fill(begin);
+    if (threadIdx.x < 2) bad_tile[threadIdx.x] = 0;
+    arrive();
+    request(0);
+    deliver(0);
+    if (tiles > 1) request(1);
   }
-  for (int tile = begin; tile < end; tile++) {
-    const int buf = (tile - begin) & 1;
+
+  // One tile.  INNER: every column of the workgroup sees every token of it, if its pages exist.
+  auto step = [&](int n, auto inner) {
+    constexpr bool INNER = decltype(inner)::value;
     arrive();               // the tile is in place for every wave, and the other buffer is free
-    const unsigned char* st0 = lds + buf * STAGE;
-    const int t0 = span.base(tile), lim = span.limit(tile);
-    const bool more = tile + 1 < end;
+    // the next chunk, half a chunk ahead: its slot's last reader was tile n - CHUNK / 2
+    if (n % CHUNK == CHUNK / 2 && begin + n + CHUNK / 2 < end && wave == (n / CHUNK & (NW - 1))) fill(begin + n + CHUNK / 2);
+    const unsigned char* st0 = lds + (n & 1) * STAGE + lane * 16;
+    const Chunk& ch = chunk_of(n);
+    const int t0 = INNER ? 0 : span.base(begin + n), lim = INNER ? 0 : span.limit(begin + n);
+    const int ok_tile = __builtin_amdgcn_readfirstlane(ch.ok[n % CHUNK]);
+    bool idle = wc0 > wc1;
     // does any of the wave's columns see any of it?
-    const bool idle = wc0 > wc1 || t0 > wpos1 || (p.window && t0 + 63 <= wpos0 - p.window && t0 >= p.sinks) || ok == 0;
+    if constexpr (!INNER) idle = idle || t0 > wpos1 || (p.window && t0 + 63 <= wpos0 - p.window && t0 >= p.sinks) || ok_tile == 0;
 
     f32x16 s[2];
     if (!idle) {
@@ -771,39 +806,49 @@ __global__ __launch_bounds__(64 * NW, 2) void window_flash_kernel(const WindowPa
 #pragma unroll
         for (int e = 0; e < 16; e++) s[rt][e] = 0.f;
 #pragma unroll
-        for (int k = 0; k < KS; k++) {
-          const u32x4 a = *reinterpret_cast<const u32x4*>(st0 + ((rt * KS + k) * 64 + lane) * 16);
-          s[rt] = mfma32<MT>(a, qf[k], s[rt]);
-        }
+        for (int k = 0; k < KS; k++) s[rt] = mfma32<MT>(*reinterpret_cast<const u32x4*>(st0 + (rt * KS + k) * 1024), qf[k], s[rt]);
       }
     }
-    const float vref_tile = vref_now;
-    const int ok_tile = ok;
     float f[4];
+    if constexpr (KV == KV16) {
 #pragma unroll
-    for (int j = 0; j < 4; j++) f[j] = KV == KV16 ? qscale : qscale * ks[j];
-    if (more) {
-      deliver(tile + 1, buf ^ 1);
-      vref_now = vref;
-      ok = ok_next;
+      for (int j = 0; j < 4; j++) f[j] = qscale;
+    } else {
+      const f32x4 ks = *reinterpret_cast<const f32x4*>(&ch.ks[n % CHUNK * 4]);
 #pragma unroll
-      for (int j = 0; j < 4; j++) ks[j] = ks_next[j];
-      if (tile + 2 < end) request(tile + 2);
+      for (int j = 0; j < 4; j++) f[j] = qscale * ks[j];
     }
-    if (idle) continue;
+    if (n + 1 < tiles) {
+      deliver(n + 1);
+      if (n + 2 < tiles) request(n + 2);
+    }
+    if (idle) return;
 
     // ---- running softmax ----------------------------------------------------------------------------------------------
-    const bool inner = ok_tile == 15 && t0 + 64 <= lim && t0 + 63 <= wpos0 && (!p.window || t0 > wpos1 - p.window);
-    uint32_t seen = ~0u;     // bit 16 rt + register
-    if (!inner) {
-      seen = 0;
-      const int hi = min(pos, lim - 1) - t0 - 8 * half, lo = p.window ? pos - p.window + 1 - t0 - 8 * half : INT_MIN, sk = p.sinks - t0 - 8 * half;
+    if constexpr (!INNER) {
+      // logits scaled here, so that what is masked is -inf whatever its scale
 #pragma unroll
-      for (int e = 0; e < 32; e++) {
-        const int at = 32 * (e >> 4) + 16 * ((e >> 3) & 1) + (e & 7);
-        const bool yes = at <= hi && (at >= lo || at < sk) && ((ok_tile >> (e >> 3)) & 1);
-        seen |= yes ? 1u << e : 0u;
-        s[e >> 4][e & 15] = yes ? s[e >> 4][e & 15] : -INFINITY;
+      for (int e = 0; e < 32; e++) s[e >> 4][e & 15] *= f[e >> 3];
+      auto token = [](int e) { return 32 * (e >> 4) + 16 * ((e >> 3) & 1) + (e & 7); };   // less 8 half
+      const int from = t0 + 8 * half;
+      if (t0 + 63 > wpos0 || t0 + 64 > lim) {
+        const int hi = min(pos, lim - 1) - from;
+#pragma unroll
+        for (int e = 0; e < 32; e++) s[e >> 4][e & 15] = token(e) <= hi ? s[e >> 4][e & 15] : -INFINITY;
+      }
+      if (p.window && t0 <= wpos1 - p.window) {
+        const int lo = pos - p.window + 1 - from, sk = p.sinks - from;
+#pragma unroll
+        for (int e = 0; e < 32; e++) s[e >> 4][e & 15] = token(e) >= lo || token(e) < sk ? s[e >> 4][e & 15] : -INFINITY;
+      }
+    }
+    if (ok_tile != 15) {
+#pragma unroll
+      for (int j = 0; j < 4; j++) {
+        if ((ok_tile >> j) & 1) continue;
+        f[j] = 1.f;
+#pragma unroll
+        for (int e = 0; e < 8; e++) s[j >> 1][8 * (j & 1) + e] = -INFINITY;
       }
     }
     float mx = -INFINITY;
@@ -812,16 +857,16 @@ __global__ __launch_bounds__(64 * NW, 2) void window_flash_kernel(const WindowPa
       float a = s[j >> 1][8 * (j & 1)];
 #pragma unroll
       for (int e = 1; e < 8; e++) a = fmaxf(a, s[j >> 1][8 * (j & 1) + e]);
-      mx = fmaxf(mx, a == -INFINITY ? a : a * f[j]);
+      mx = fmaxf(mx, INNER ? a * f[j] : a);
     }
     mx = pair_max(mx);
-    if (__any(mx > m + WA_LAG) || (KV != KV16 && vref_tile != oref)) {
+    const float vref_tile = KV == KV16 ? 0.f : ch.vref;
+    if (__any(mx > m + WA_LAG) || (KV != KV16 && __any(vref_tile > oref))) {
       const float mn = mx > m + WA_LAG ? mx : m;
       float a = m == -INFINITY ? 0.f : exp2_fast(m - mn);
       l *= a;
       if constexpr (KV != KV16) {
-        if (vref_tile != oref) a *= oref / vref_tile;
-        oref = vref_tile;
+        if (vref_tile > oref) a *= oref / vref_tile, oref = vref_tile;
       }
 #pragma unroll
       for (int d = 0; d < DTL; d++) o[d] *= a;
@@ -832,60 +877,48 @@ __global__ __launch_bounds__(64 * NW, 2) void window_flash_kernel(const WindowPa
 #pragma unroll
     for (int j = 0; j < 4; j++) {
 #pragma unroll
-      for (int e = 0; e < 4; e++) {
-        float w[2];
-#pragma unroll
-        for (int u = 0; u < 2; u++) {
-          const int r = 2 * e + u;
-          float x = __builtin_fmaf(s[j >> 1][8 * (j & 1) + r], f[j], -ms);
-          w[u] = exp2_fast(x);
-          if (!inner) w[u] = (seen >> (8 * j + r)) & 1 ? w[u] : 0.f;
-        }
-        pf[j][e] = pack2<MT>(w[0], w[1]);
-        l = add_pair<MT>(pf[j][e], l);
+      for (int e = 0; e < 8; e++) {
+        const float x = s[j >> 1][8 * (j & 1) + e];
+        s[j >> 1][8 * (j & 1) + e] = exp2_fast(INNER ? __builtin_fmaf(x, f[j], -ms) : x - ms);
       }
     }
+#pragma unroll
+    for (int j = 0; j < 4; j++)
+#pragma unroll
+      for (int e = 0; e < 4; e++) {
+        pf[j][e] = pack2<MT>(s[j >> 1][8 * (j & 1) + 2 * e], s[j >> 1][8 * (j & 1) + 2 * e + 1]);
+        l = add_pair<MT>(pf[j][e], l);
+      }
 
     // ---- O^T += V^T P^T -------------------------------------------------------------------------------------------------
     const unsigned char* vt = st0 + KBYTES;
-    bool bad = false;
-    if (!inner) {
+    if (INNER || bad_tile[n & 1] != n + 1) {
 #pragma unroll
       for (int d = 0; d < DTL; d++)
 #pragma unroll
-        for (int st = 0; st < 4; st++) bad |= not_finite<MT>(*reinterpret_cast<const u32x4*>(vt + ((d * 4 + st) * 64 + lane) * 16));
-    }
-    if (!__any(bad)) {
-#pragma unroll
-      for (int d = 0; d < DTL; d++)
-#pragma unroll
-        for (int st = 0; st < 4; st++) {
-          const u32x4 a = *reinterpret_cast<const u32x4*>(vt + ((d * 4 + st) * 64 + lane) * 16);
-          o[d] = mfma32<MT>(a, pf[st], o[d]);
-        }
+        for (int st = 0; st < 4; st++) o[d] = mfma32<MT>(*reinterpret_cast<const u32x4*>(vt + (d * 4 + st) * 1024), pf[st], o[d]);
     } else {
       // an infinity or NaN that some columns may see and others must not: one token at a time, added where it is seen
 #pragma unroll 1
-      for (int n = 0; n < 64; n++) {
-        const int h = (n >> 3) & 1, i = n & 7;
-        const bool here = half == h;
-        const uint32_t theirs = (uint32_t)__shfl((int)seen, h * 32 + col, 64);
+      for (int k = 0; k < 64; k++) {
+        const int st = k >> 4, i = k & 7, t = t0 + k;
+        const bool here = half == ((k >> 3) & 1);
+        const bool counts = t < lim && t <= pos && (!p.window || t > pos - p.window || t < p.sinks) && ((ok_tile >> st) & 1);
+        const u32x4 pb = only<MT>(st == 0 ? pf[0] : st == 1 ? pf[1] : st == 2 ? pf[2] : pf[3], here, i);
 #pragma unroll
-        for (int st = 0; st < 4; st++) {
-          if (st != n >> 4) continue;
-          const bool counts = (theirs >> (8 * st + i)) & 1;
-          const u32x4 pb = only<MT>(pf[st], here, i);
+        for (int d = 0; d < DTL; d++) {
+          const u32x4 a = only<MT>(*reinterpret_cast<const u32x4*>(vt + (d * 4 + st) * 1024), here, i);
+          const f32x16 r = mfma32<MT>(a, pb, o[d]);
 #pragma unroll
-          for (int d = 0; d < DTL; d++) {
-            const u32x4 a = only<MT>(*reinterpret_cast<const u32x4*>(vt + ((d * 4 + st) * 64 + lane) * 16), here, i);
-            const f32x16 r = mfma32<MT>(a, pb, o[d]);
-#pragma unroll
-            for (int e = 0; e < 16; e++) o[d][e] = counts ? r[e] : o[d][e];
-          }
+          for (int e = 0; e < 16; e++) o[d][e] = counts ? r[e] : o[d][e];
         }
       }
     }
-  }
+  };
+  int n = 0;
+  for (; n < in0; n++) step(n, std::false_type());
+  for (; n < in1; n++) step(n, std::true_type());
+  for (; n < tiles; n++) step(n, std::false_type());
 
   // ---- out ----------------------------------------------------------------------------------------------------------------
   l = pair_sum(l);
@@ -945,11 +978,11 @@ __global__ __launch_bounds__(256) void window_merge_kernel(const WindowParams p,
   const int c = (b % per_seq) * 4 + wave;
   b /= per_seq;
   const int kvh = b % p.num_kv_heads, seq = b / p.num_kv_heads;
-  const int start = p.starts ? p.starts[seq] : seq;
-  const int qlen = p.starts ? p.starts[seq + 1] - start : 1;
+  const int start = p.starts ? sload(p.starts + seq) : seq;
+  const int qlen = p.starts ? sload(p.starts + seq + 1) - start : 1;
   const int cols = min(qlen, p.num_rows - start) * p.group;
   if (start < 0 || c >= cols || cols < p.min_cols || cols > p.max_cols) return;
-  const int seq_len = p.seq_lens[seq];
+  const int seq_len = sload(p.seq_lens + seq);
   const int c0 = c / COLS * COLS, c1 = min(c0 + COLS, cols) - 1;
   const Span span = span_of(p, seq_len - qlen + c0 / p.group, seq_len - qlen + c1 / p.group);
   if (span.tiles <= p.split_tiles) return;    // written by its only workgroup
