@@ -766,7 +766,8 @@ int mi355q_rope_and_cache_blocks(const int64_t* positions, const void* query, in
  * rocm_attn.py:271-300; ops/prefix_prefill.py SLIDING_WINDOW); visible first tokens and block scales have no counterpart there.
  */
 size_t mi355q_paged_window_attention_workspace_bytes(int num_seqs, int num_rows, int num_heads, int num_kv_heads,
-                                                     int head_size, int max_query_len, int max_seq_len, int window, int sinks);
+                                                     int head_size, int max_query_len, int max_seq_len, int window, int sinks,
+                                                     int kv_type);
 int mi355q_paged_window_attention(void* out, int64_t out_stride, const void* query, int64_t q_stride, const void* key_cache,
                                   const void* value_cache, int64_t kv_block_stride, int64_t kv_head_stride, int num_blocks,
                                   int num_rows, int num_seqs, int num_heads, int num_kv_heads, int head_size, float scale,

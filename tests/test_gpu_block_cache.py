@@ -456,7 +456,7 @@ def test_long_contexts_are_cut_and_joined(form, window, sinks):
     lens = [(4999, 1), (2047, 3), (64, 1)]
     b = Batch(lens, 4, 1, 128, 16, form, torch.float16, window=window, sinks=sinks, seed=4)
     if not window:
-        assert ops.paged_window_attention_workspace_bytes(3, b.rows + 1, 4, 1, 128, 3, 5000) > 0
+        assert ops.paged_window_attention_workspace_bytes(3, b.rows + 1, 4, 1, 128, 3, 5000, form) > 0
     b.check()
     # a bound on the lengths that is far off changes how the work is cut, not what comes out of it
     b.check(b.run(max_seq_len=64))
@@ -607,7 +607,7 @@ def test_strided_rows_tables_and_cache_heads():
 def test_streams_graphs_and_a_workspace_of_ones_own():
     b = Batch([(2999, 1), (700, 3)], 4, 1, 128, 16, "block_int8", torch.bfloat16, seed=14)
     want = cpu(b.run())
-    need = ops.paged_window_attention_workspace_bytes(2, b.rows + 1, 4, 1, 128, b.max_query, b.max_len)
+    need = ops.paged_window_attention_workspace_bytes(2, b.rows + 1, 4, 1, 128, b.max_query, b.max_len, b.form)
     ws = torch.empty(need, dtype=torch.uint8, device=DEV)
     assert torch.equal(cpu(b.run(workspace=ws)), want)
     with pytest.raises(RuntimeError, match="workspace"):

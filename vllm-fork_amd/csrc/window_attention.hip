@@ -56,6 +56,8 @@ struct WindowParams {
   int splits, split_tiles;      // the context in stretches of split_tiles 64-token tiles, at most `splits` of them
   int part_stride;              // partial sums are laid out for so many stretches
   int col_tiles;                // column tiles of the longest query that this launch serves
+  int longest_cols;             // columns of the longest query, at most WA_ROWS_COLS
+  int lds_cols;                 // rows kernel: columns of a 16-column tile that any sequence has
   int min_cols, max_cols;       // sequences with fewer or more columns (rows x heads per kv head) are another launch's
 };
 
@@ -148,25 +150,31 @@ __device__ inline u32x4 only(u32x4 v, bool here, int n) {
 }
 
 // ---------------------------------------------------------------------------------------------------------------------
-// Few columns (decode rows, drafts): one workgroup of 4 waves per (sequence, 16 columns, kv head, stretch of the context);
+// Few columns (decode rows, drafts): one workgroup of NW waves per (sequence, 16 NCT columns, kv head, stretch of the context);
 // the waves take the stretch's 64-token tiles in turn, each with a running softmax of its own, and meet once in LDS.
-// Bound by HBM: a wave keeps a tile of K or V on the way while it works on the other (K of the next tile is requested as
-// soon as this tile's logits stand, V as soon as its products do).
+// Bound by HBM: K of the next tile is requested as soon as this tile's logits stand, V as soon as its products do, so a wave
+// has half a tile to a whole one on the way at any time.  Pages and scales are looked up for 16 tiles at once, a 16-token
+// stretch per lane.
 //
 // Token order inside a tile: row i of 16-row MFMA tile T is token 16 (i / 4) + 4 T + i % 4, so the 16 logits that a lane of
 // group g = lane / 16 holds after S^T are tokens 16 g .. 16 g + 15: one block, one scale, and the B operand of O^T as
 // they stand; V comes in its own order, 16 tokens of a head dim per lane.
+//
+// Probabilities are 2^(x - m + 15) here (the largest fits fp16 once V's relative scale, at most 1/2, has been applied): what
+// a block whose scale is 10^-8 of the largest adds still has all its bits.
 // ---------------------------------------------------------------------------------------------------------------------
-template <typename DT, int KV, int HEAD>
-__global__ __launch_bounds__(256, 2) void window_rows_kernel(const WindowParams p) {
+constexpr float WA_ROWS_SHIFT = 15.0f;
+
+template <typename DT, int KV, int HEAD, int NCT, int NW>
+__global__ __launch_bounds__(64 * NW, 2) void window_rows_kernel(const WindowParams p) {
   typedef typename MathOf<DT, KV>::T MT;
   constexpr int EB = KV == KV16 ? 2 : 1;
   constexpr int DS = HEAD / 32, DT16 = HEAD / 16;
   constexpr int KP = EB == 1 ? DS / 2 : DS;      // 16-byte pieces of K per lane and row tile
   constexpr int VP = EB == 1 ? 1 : 2;            // of V per lane and 16 head dims
-  constexpr int LD = HEAD + 4;
-  __shared__ __attribute__((aligned(16))) float acc[4][16 * LD];
-  __shared__ float stat[4][2][16];
+  constexpr int LD = HEAD + 4, COLS = 16 * NCT;
+  extern __shared__ __attribute__((aligned(16))) float acc[];   // [NW][columns of a 16-column tile][LD]
+  __shared__ float stat[NW][2][COLS];
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int g = lane >> 4, col = lane & 15;
@@ -180,10 +188,10 @@ __global__ __launch_bounds__(256, 2) void window_rows_kernel(const WindowParams 
 
   const int start = p.starts ? sload(p.starts + seq) : seq;
   const int qlen = p.starts ? sload(p.starts + seq + 1) - start : 1;
-  const int cols = min(qlen, p.num_rows - start) * G;
-  if (start < 0 || ct * 16 >= cols || cols > p.max_cols) return;
+  const int all = min(qlen, p.num_rows - start) * G, cols = min(all, p.longest_cols);   // (no more than the caller announced)
+  if (start < 0 || ct * COLS >= cols || all > p.max_cols) return;
   const int seq_len = sload(p.seq_lens + seq);
-  const int c0 = ct * 16, c1 = min(c0 + 16, cols) - 1;
+  const int c0 = ct * COLS, c1 = min(c0 + COLS, cols) - 1;
   const int pos0 = seq_len - qlen + c0 / G, pos1 = seq_len - qlen + c1 / G;
   const Span span = span_of(p, pos0, pos1);
   // (a context longer than the caller's bound: the last stretch takes the rest)
@@ -192,285 +200,399 @@ __global__ __launch_bounds__(256, 2) void window_rows_kernel(const WindowParams 
   if (split > 0 && begin >= end) return;      // nothing here; the merge knows how many stretches there are
   const bool whole = span.tiles <= p.split_tiles;
 
-  const int c = min(c0 + col, c1);
-  const int row = start + c / G, head = kvh * G + c % G;
-  const int pos = seq_len - qlen + c / G;
-  const int low = p.window ? pos - p.window + 1 : INT_MIN;
-
-  // ---- this lane's query column -------------------------------------------------------------------------------------
-  u32x4 qf[DS];
-  float qscale = p.scale * WA_LOG2E;
-  {
+  // ---- this lane's query columns ------------------------------------------------------------------------------------
+  u32x4 qf[NCT][DS];
+  float qscale[NCT];
+  int pos[NCT];
+#pragma unroll
+  for (int n = 0; n < NCT; n++) {
+    const int c = min(c0 + 16 * n + col, c1);
+    const int row = start + c / G, head = kvh * G + c % G;
+    pos[n] = seq_len - qlen + c / G;
+    qscale[n] = fabsf(p.scale) * WA_LOG2E;
     const uint16_t* qp = p.q + (int64_t)row * p.q_stride + (int64_t)head * HEAD;
 #pragma unroll
     for (int ds = 0; ds < DS; ds++) {
       const int d0 = EB == 1 ? 16 * (4 * (ds >> 1) + g) + 8 * (ds & 1) : 32 * ds + 8 * g;
-      qf[ds] = *reinterpret_cast<const u32x4*>(qp + d0);
+      qf[n][ds] = *reinterpret_cast<const u32x4*>(qp + d0);
     }
+  }
+
+  // ---- pages and scales of the wave's next 16 tiles, a stretch per lane -------------------------------------------------
+  const int32_t* table = p.tables + (int64_t)seq * p.table_width;
+  const int pieces = p.bs >> 4;
+  const unsigned char* kc = p.kc + (int64_t)kvh * p.head_stride;
+  const unsigned char* vc = p.vc + (int64_t)kvh * p.head_stride;
+  const int wg_low = p.window ? pos0 - p.window + 1 : INT_MIN;
+  int64_t at_k = 0, at_v = 0;
+  float at_ks = 1.f, at_vs = 0.f;
+  uint64_t at_ok = 0;
+  auto look_up = [&](int first) {        // first: a tile of this wave
+    const int tile = min(first + NW * (lane >> 2), end - 1), j = lane & 3;
+    const int t = span.base(tile) + 16 * j, lim = span.limit(tile);
+    const int n16 = min(t, (lim - 1) & ~15) >> 4;         // past the end: the last stretch again, masked
+    const int pg = wa_page(n16, p.page_magic);
+    const int blk = table[pg];
+    const bool in = (unsigned)blk < (unsigned)p.num_blocks;
+    const int64_t at = in ? blk : 0;
+    const int off = (n16 - pg * pieces) * 16;
+    at_k = at * p.block_stride + off * 16;
+    at_v = at * p.block_stride + off * EB;
+    // a stretch counts where some column sees some of it
+    const bool ok = in && t < lim && (t + 16 > wg_low || t < p.sinks);
+    at_ok = __ballot(ok);
+    if constexpr (KV != KV16) {
+      const int64_t si = at * p.scale_block_stride + kvh * p.scale_head_stride;
+      at_ks = ok ? p.ks[si] : 1.f;
+      at_vs = ok ? p.vs[si] : 0.f;
+    }
+  };
+  auto from = [](int64_t v, int l) {
+    return (int64_t)(((uint64_t)(uint32_t)__shfl((int)(v >> 32), l, 64) << 32) | (uint32_t)__shfl((int)v, l, 64));
+  };
+
+  const int klane = (g * p.bs + (col & 3)) * 16, vlane = col * p.bs * EB, kstep = 64 * p.bs, vstep = 16 * p.bs * EB;
+  u32x4 kf[4][KP], vf[DT16][VP];
+  auto load_k = [&](int i) {             // tile i of the 16
+    const unsigned char* kp = kc + from(at_k, 4 * i + (col >> 2)) + klane;
+#pragma unroll
+    for (int s = 0; s < KP; s++) {
+#pragma unroll
+      for (int T = 0; T < 4; T++) kf[T][s] = *reinterpret_cast<const u32x4*>(kp + T * 64);
+      kp += kstep;
+    }
+  };
+  auto load_v = [&](int i) {
+    const unsigned char* vp = vc + from(at_v, 4 * i + g) + vlane;
+#pragma unroll
+    for (int d = 0; d < DT16; d++) {
+#pragma unroll
+      for (int s = 0; s < VP; s++) vf[d][s] = *reinterpret_cast<const u32x4*>(vp + s * 16);
+      vp += vstep;
+    }
+  };
+
+  int tile = begin + wave, at = 0;       // `at`: the tile's place among the 16 looked up
+  if (tile < end) {
+    look_up(tile);
+    load_k(0);
+    load_v(0);
+  }
+  // (the queries were requested first and are turned to fp16 while the tiles are on their way)
+#pragma unroll
+  for (int n = 0; n < NCT; n++) {
     if constexpr (EB == 1 && DT::id == MI355Q_BF16) {
       float top = 0.f;
 #pragma unroll
       for (int ds = 0; ds < DS; ds++)
 #pragma unroll
         for (int e = 0; e < 4; e++)
-          top = fmaxf(top, fmaxf(fabsf(BF16::to_f32((uint16_t)qf[ds][e])), fabsf(BF16::to_f32((uint16_t)(qf[ds][e] >> 16)))));
+          top = fmaxf(top, fmaxf(fabsf(BF16::to_f32((uint16_t)qf[n][ds][e])), fabsf(BF16::to_f32((uint16_t)(qf[n][ds][e] >> 16)))));
       top = group_max(top);
       int ex = (int)(__float_as_uint(top) >> 23);            // biased exponent; 255: not finite, 0: zero or subnormal
       ex = ex == 255 ? 140 : max(ex, 20);
       const float up = __uint_as_float((uint32_t)(127 + 140 - ex) << 23);   // 2^(13 - exponent)
-      qscale *= __uint_as_float((uint32_t)(ex - 13) << 23);
+      qscale[n] *= __uint_as_float((uint32_t)(ex - 13) << 23);
 #pragma unroll
       for (int ds = 0; ds < DS; ds++)
 #pragma unroll
         for (int e = 0; e < 4; e++)
-          qf[ds][e] = pack2<FP16>(BF16::to_f32((uint16_t)qf[ds][e]) * up, BF16::to_f32((uint16_t)(qf[ds][e] >> 16)) * up);
+          qf[n][ds][e] = pack2<FP16>(BF16::to_f32((uint16_t)qf[n][ds][e]) * up, BF16::to_f32((uint16_t)(qf[n][ds][e] >> 16)) * up);
+    }
+    if (p.scale < 0.f) {   // the factor of the exponent stays positive
+#pragma unroll
+      for (int ds = 0; ds < DS; ds++) qf[n][ds] ^= u32x4{0x80008000u, 0x80008000u, 0x80008000u, 0x80008000u};
     }
   }
 
-  const int32_t* table = p.tables + (int64_t)seq * p.table_width;
-  const int pieces = p.bs >> 4;
-  const unsigned char* kc = p.kc + (int64_t)kvh * p.head_stride;
-  const unsigned char* vc = p.vc + (int64_t)kvh * p.head_stride;
-  const int64_t klane = ((int64_t)g * p.bs + (col & 3)) * 16;
-  const int64_t vlane = (int64_t)col * p.bs * EB;
-
-  // one tile's four 16-token stretches: where their block lies, what scales it, whether anything of it is seen
-  auto place_of = [&](int tile, const unsigned char*& kp, const unsigned char*& vp, float& ks, float& vs, bool& ok) {
-    const int t0 = span.base(tile), lim = span.limit(tile);
-    int blk[4], off[4];
+  f32x4 o[NCT][DT16];
+  float m[NCT], l[NCT], vref = 0.f;
 #pragma unroll
-    for (int j = 0; j < 4; j++) {
-      const int n = min(t0 + 16 * j, (lim - 1) & ~15) >> 4;   // past the end: the last stretch again, masked
-      const int pg = wa_page(n, p.page_magic);
-      blk[j] = sload(table + pg);
-      off[j] = (n - pg * pieces) * 16;
-    }
-    kp = kc, vp = vc, ks = 0.f, vs = 0.f, ok = false;
+  for (int n = 0; n < NCT; n++) {
+    m[n] = -INFINITY;
+    l[n] = 0.f;
 #pragma unroll
-    for (int j = 0; j < 4; j++) {
-      const bool in = (unsigned)blk[j] < (unsigned)p.num_blocks;
-      const int64_t at = in ? blk[j] : 0;
-      const unsigned char* kj = kc + at * p.block_stride + (int64_t)off[j] * 16;
-      const unsigned char* vj = vc + at * p.block_stride + off[j] * EB;
-      if ((col >> 2) == j) kp = kj;
-      if constexpr (KV != KV16) {
-        const int64_t si = at * p.scale_block_stride + kvh * p.scale_head_stride;
-        const float a = sload(p.ks + si), b = sload(p.vs + si);
-        ks = g == j ? a : ks;
-        vs = g == j ? b : vs;
-      }
-      if (g == j) {
-        vp = vj;
-        ok = in && t0 + 16 * j < lim;
-      }
-    }
-  };
-
-  u32x4 kf[4][KP], vf[DT16][VP];
-  auto load_k = [&](const unsigned char* kp) {
-#pragma unroll
-    for (int T = 0; T < 4; T++)
-#pragma unroll
-      for (int s = 0; s < KP; s++)
-        kf[T][s] = *reinterpret_cast<const u32x4*>(kp + klane + T * 64 + (int64_t)s * 64 * p.bs);
-  };
-  auto load_v = [&](const unsigned char* vp) {
-#pragma unroll
-    for (int d = 0; d < DT16; d++)
-#pragma unroll
-      for (int s = 0; s < VP; s++)
-        vf[d][s] = *reinterpret_cast<const u32x4*>(vp + vlane + (int64_t)d * 16 * p.bs * EB + s * 16);
-  };
-
-  f32x4 o[DT16];
-#pragma unroll
-  for (int d = 0; d < DT16; d++) o[d] = f32x4{0.f, 0.f, 0.f, 0.f};
-  float m = -INFINITY, l = 0.f, vref = 0.f;
-
-  int tile = begin + wave;
-  const unsigned char *kp, *vp;
-  float ks, vs;
-  bool ok;
-  if (tile < end) {
-    place_of(tile, kp, vp, ks, vs, ok);
-    load_k(kp);
-    load_v(vp);
+    for (int d = 0; d < DT16; d++) o[n][d] = f32x4{0.f, 0.f, 0.f, 0.f};
   }
-  for (; tile < end; tile += 4) {
-    const int t0 = span.base(tile), lim = span.limit(tile);
-    const float ks_now = ks, vs_now = vs;
-    const bool ok_now = ok, more = tile + 4 < end;
-    if (more) place_of(tile + 4, kp, vp, ks, vs, ok);
 
-    f32x4 s[4];
+  auto fragment = [&](int d, int h) {
+    if constexpr (EB == 1) return widen8<KV>(vf[d][0], h);
+    else return vf[d][h];
+  };
+  auto logits = [&](f32x4 (&s)[NCT][4]) {
 #pragma unroll
     for (int T = 0; T < 4; T++) {
-      s[T] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int n = 0; n < NCT; n++) s[n][T] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
       for (int ds = 0; ds < DS; ds++) {
         u32x4 a;
         if constexpr (EB == 1) a = widen8<KV>(kf[T][ds >> 1], ds & 1);
         else a = kf[T][ds];
-        s[T] = mfma16<MT>(a, qf[ds], s[T]);
+#pragma unroll
+        for (int n = 0; n < NCT; n++) s[n][T] = mfma16<MT>(a, qf[n][ds], s[n][T]);
       }
     }
-    if (more) load_k(kp);
+  };
+  // bits of the 16 tokens from tg on that column n sees
+  auto sees = [&](int n, int tg, int lim, bool ok) {
+    auto below = [](int k) { return k <= 0 ? 0u : k >= 16 ? 0xffffu : (1u << k) - 1; };
+    uint32_t bits = ok ? below(min(pos[n] + 1, lim) - tg) : 0u;
+    if (p.window) bits &= ~below(pos[n] - p.window + 1 - tg) | below(p.sinks - tg);
+    return bits;
+  };
+  // V's tokens that no column sees become zeros, whatever bytes their places hold; whether what is left has an infinity or NaN
+  auto clear_v = [&](int tg, int lim, bool ok) {
+    auto below = [](int k) { return k <= 0 ? 0u : k >= 16 ? 0xffffu : (1u << k) - 1; };
+    uint32_t any = ok ? below(min(pos1 + 1, lim) - tg) : 0u;
+    if (p.window) any &= ~below(wg_low - tg) | below(p.sinks - tg);
+    u32x4 keep[VP];
+#pragma unroll
+    for (int s = 0; s < VP; s++)
+#pragma unroll
+      for (int e = 0; e < 4; e++) {
+        if constexpr (EB == 1) {
+          const uint32_t k = any >> (4 * e);
+          keep[s][e] = ((k & 1) | ((k & 2) << 7) | ((k & 4) << 14) | ((k & 8) << 21)) * 0xffu;
+        } else {
+          const uint32_t k = any >> (8 * s + 2 * e);
+          keep[s][e] = (k & 1 ? 0xffffu : 0u) | (k & 2 ? 0xffff0000u : 0u);
+        }
+      }
+    bool bad = false;
+#pragma unroll
+    for (int d = 0; d < DT16; d++)
+#pragma unroll
+      for (int s = 0; s < VP; s++) {
+        vf[d][s] &= keep[s];
+        asm volatile("" : "+v"(vf[d][s]));      // in place: no second copy of the tile in registers
+        if constexpr (EB == 2) {
+          bad |= not_finite<MT>(vf[d][s]);
+        } else {
+#pragma unroll
+          for (int e = 0; e < 4; e++) bad |= (((vf[d][s][e] & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u) != 0;   // e4m3: 0x7f, 0xff
+        }
+      }
+    return bad;
+  };
+
+  // One tile.  INNER: every column sees every token of it, if its pages exist.
+  bool left_out = false;               // a tile whose V holds an infinity or NaN that only some columns may see
+  auto step = [&](auto inner) {
+    constexpr bool INNER = decltype(inner)::value;
+    const int t0 = span.base(tile), lim = span.limit(tile), tg = t0 + 16 * g;
+    const uint32_t ok_tile = (uint32_t)(at_ok >> (4 * at)) & 15;
+    const bool ok = (ok_tile >> g) & 1;
+    float ks = 1.f, vs = 1.f;
+    if constexpr (KV != KV16) {
+      ks = __shfl(at_ks, 4 * at + g, 64);
+      vs = __shfl(at_vs, 4 * at + g, 64);
+    }
+    f32x4 s[NCT][4];
+    logits(s);
+    const bool more = tile + NW < end;
+    if (more) {
+      if (++at == 16) {
+        look_up(tile + NW);
+        at = 0;
+      }
+      if constexpr (INNER) load_k(at);   // (the masks of a partial tile need the registers)
+    }
 
     // ---- running softmax -------------------------------------------------------------------------------------------
-    const int tg = t0 + 16 * g;
-    const float f = KV == KV16 ? qscale : qscale * ks_now;
-    // every column sees every token of the tile?
-    const bool inner = __all(ok_now) && t0 + 64 <= lim && t0 + 63 <= pos0 && (!p.window || t0 > pos1 - p.window);
-    uint32_t seen = 0xffffu;
-    if (!inner) {
-      seen = 0;
-#pragma unroll
-      for (int i = 0; i < 16; i++) {
-        const int t = tg + i;
-        if (ok_now && t < lim && t <= pos && (t >= low || t < p.sinks)) seen |= 1u << i;
-      }
-    }
-    float x[16], mx = -INFINITY;
-#pragma unroll
-    for (int i = 0; i < 16; i++) {
-      x[i] = s[i >> 2][i & 3] * f;
-      if (!inner) x[i] = (seen >> i) & 1 ? x[i] : -INFINITY;
-      mx = fmaxf(mx, x[i]);
-    }
-    mx = group_max(mx);
     float vtop = 0.f;
-    if constexpr (KV != KV16) vtop = group_max(ok_now ? vs_now : 0.f);
-    if (__any(mx > m + WA_LAG || vtop > vref)) {
-      const float mn = fmaxf(m, mx);
-      float a = m == -INFINITY ? 0.f : exp2_fast(m - mn);
-      l *= a;
-      if (vtop > vref) {        // headroom of 2: the next slightly larger scale needs no rescaling
-        a *= vref / (2.f * vtop);
-        vref = 2.f * vtop;
+    if constexpr (KV != KV16) vtop = group_max(vs);
+    float back = 1.f;                  // what a new reference for V's scales does to the sums
+    if (KV != KV16 && __any(vtop > vref)) {
+      back = vref / (2.f * vtop);      // headroom of 2: the next slightly larger scale changes nothing
+      vref = 2.f * vtop;
+    }
+    const float r = KV == KV16 ? 1.f : vref > 0.f ? vs / vref : vs;
+    u32x4 pf[NCT][2];
+#pragma unroll
+    for (int n = 0; n < NCT; n++) {
+      const float f = KV == KV16 ? qscale[n] : qscale[n] * ks;
+      uint32_t seen = 0xffffu;
+      float x[16], mx = -INFINITY;
+#pragma unroll
+      for (int i = 0; i < 16; i++) x[i] = s[n][i >> 2][i & 3];
+      if constexpr (INNER) {
+        if (ok_tile != 15 && !ok) {
+#pragma unroll
+          for (int i = 0; i < 16; i++) x[i] = -INFINITY;
+        }
+#pragma unroll
+        for (int i = 0; i < 16; i++) mx = fmaxf(mx, x[i]);
+        mx *= f;
+      } else {
+        seen = sees(n, tg, lim, ok);
+#pragma unroll
+        for (int i = 0; i < 16; i++) {
+          x[i] = (seen >> i) & 1 ? x[i] * f : -INFINITY;
+          mx = fmaxf(mx, x[i]);
+        }
       }
+      mx = group_max(mx);
+      if (__any(mx > m[n] || back != 1.f)) {
+        const float mn = fmaxf(m[n], mx);
+        const float a = m[n] == -INFINITY ? 0.f : exp2_fast(m[n] - mn);
+        l[n] *= a;
 #pragma unroll
-      for (int d = 0; d < DT16; d++) o[d] *= a;
-      m = mn;
-    }
-    const float ms = (m == -INFINITY ? 0.f : m) - WA_SHIFT;
-    float w[16];
-#pragma unroll
-    for (int i = 0; i < 16; i++) {
-      w[i] = exp2_fast(x[i] - ms);
-      l += w[i];
-    }
-    if constexpr (KV != KV16) {
-      const float r = vref > 0.f ? vs_now / vref : (vs_now == 0.f ? 0.f : vs_now);
+        for (int d = 0; d < DT16; d++) o[n][d] *= a * back;
+        m[n] = mn;
+      }
+      const float ms = (m[n] == -INFINITY ? 0.f : m[n]) - WA_ROWS_SHIFT;
 #pragma unroll
       for (int i = 0; i < 16; i++) {
-        w[i] *= r;
-        if (!inner) w[i] = (seen >> i) & 1 ? w[i] : 0.f;   // whatever the scale of a block that is not seen
+        x[i] = exp2_fast(INNER ? __builtin_fmaf(x[i], f, -ms) : x[i] - ms);
+        l[n] += x[i];
+      }
+#pragma unroll
+      for (int i = 0; i < 8; i++) {
+        uint32_t w = KV == KV16 ? pack2<MT>(x[2 * i], x[2 * i + 1]) : pack2<MT>(x[2 * i] * r, x[2 * i + 1] * r);
+        // (a NaN scale reaches only the columns that see its tokens)
+        if (!INNER && KV != KV16) w &= ((seen >> (2 * i)) & 1 ? 0xffffu : 0u) | ((seen >> (2 * i)) & 2 ? 0xffff0000u : 0u);
+        pf[n][i >> 2][i & 3] = w;
       }
     }
-    u32x4 pf[2];
-#pragma unroll
-    for (int i = 0; i < 8; i++) pf[i >> 2][i & 3] = pack2<MT>(w[2 * i], w[2 * i + 1]);
 
     // ---- O^T += V^T P^T ----------------------------------------------------------------------------------------------
-    auto fragment = [&](int d, int h) {
-      if constexpr (EB == 1) return widen8<KV>(vf[d][0], h);
-      else return vf[d][h];
-    };
-    if (inner || KV == KVI8) {
-#pragma unroll
-      for (int d = 0; d < DT16; d++)
-#pragma unroll
-        for (int h = 0; h < 2; h++) o[d] = mfma16<MT>(fragment(d, h), pf[h], o[d]);
-    } else {
-      // tokens that no column sees count for nothing, whatever bytes their places hold
-      uint32_t any = 0;
-#pragma unroll
-      for (int i = 0; i < 16; i++) {
-        const int t = tg + i;
-        const bool some = ok_now && t < lim && t <= pos1 && (!p.window || t > pos0 - p.window || t < p.sinks);
-        any |= some ? 1u << i : 0u;
-      }
-      bool bad = false;
-      auto seen_fragment = [&](int d, int h) {
-        u32x4 v = fragment(d, h);
-#pragma unroll
-        for (int e = 0; e < 4; e++) {
-          const uint32_t two = any >> (8 * h + 2 * e);
-          v[e] &= (two & 1 ? 0xffffu : 0u) | (two & 2 ? 0xffff0000u : 0u);
-        }
-        return v;
-      };
+    bool bad = false;
+    if constexpr (!INNER && KV != KVI8) {
+      bad = __any(clear_v(tg, lim, ok));
+      left_out |= bad;
+    }
+    if (INNER || KV == KVI8 || !bad) {
 #pragma unroll
       for (int d = 0; d < DT16; d++)
 #pragma unroll
         for (int h = 0; h < 2; h++) {
-          const u32x4 v = seen_fragment(d, h);
-          bad |= not_finite<MT>(v);
+          const u32x4 v = fragment(d, h);
+#pragma unroll
+          for (int n = 0; n < NCT; n++) o[n][d] = mfma16<MT>(v, pf[n][h], o[n][d]);
         }
-      if (!__any(bad)) {
+    }
+    if (more) {
+      if constexpr (!INNER) load_k(at);
+      load_v(at);
+    }
+    tile += NW;
+  };
+  // the tiles that every column sees whole: past the sinks and the window's moving start, before the moving end
+  {
+    const int first = p.window ? span.sink_tiles + max(0, pos1 - p.window + 1 - span.low + 63) / 64 : span.sink_tiles;
+    const int to = min(pos0, span.end - 1) - 63 - span.low;
+    const int in0 = min(end, first), in1 = min(end, span.sink_tiles + (to < 0 ? 0 : to / 64 + 1));
+    while (tile < in0) step(std::false_type());
+    while (tile < in1) step(std::true_type());
+    while (tile < end) step(std::false_type());
+
+    // tiles left out: once more, one token at a time, added to the columns that see it
+    if (KV != KVI8 && left_out) {
+      for (tile = begin + wave; tile < end; tile += NW) {
+        if (tile >= in0 && tile < in1) continue;
+        look_up(tile);
+        load_k(0);
+        load_v(0);
+        const int lim = span.limit(tile), tg = span.base(tile) + 16 * g;
+        const bool ok = (at_ok >> g) & 1;
+        if (!__any(clear_v(tg, lim, ok))) continue;
+        f32x4 s[NCT][4];
+        logits(s);
+        const float ks = KV == KV16 ? 1.f : __shfl(at_ks, g, 64), vs = KV == KV16 ? 1.f : __shfl(at_vs, g, 64);
+        const float r = KV == KV16 ? 1.f : vref > 0.f ? vs / vref : vs;
+        uint32_t seen[NCT];
+        u32x4 pf[NCT][2];
 #pragma unroll
-        for (int d = 0; d < DT16; d++)
+        for (int n = 0; n < NCT; n++) {
+          seen[n] = sees(n, tg, lim, ok);
+          const float f = qscale[n] * ks, ms = (m[n] == -INFINITY ? 0.f : m[n]) - WA_ROWS_SHIFT;
 #pragma unroll
-          for (int h = 0; h < 2; h++) o[d] = mfma16<MT>(seen_fragment(d, h), pf[h], o[d]);
-      } else {
-        // an infinity or NaN that some columns may see and others must not: one token at a time, added where it is seen
+          for (int i = 0; i < 8; i++)
+            pf[n][i >> 2][i & 3] = pack2<MT>(exp2_fast(s[n][i >> 1][2 * (i & 1)] * f - ms) * r, exp2_fast(s[n][i >> 1][2 * (i & 1) + 1] * f - ms) * r);
+        }
 #pragma unroll 1
-        for (int n = 0; n < 64; n++) {
-          const int gn = n >> 4, i = n & 15;
-          const bool here = g == gn;
-          const bool counts = (__shfl((int)seen, gn * 16 + col, 64) >> i) & 1;
+        for (int k = 0; k < 64; k++) {
+          const int i = k & 15;
+          const bool here = g == k >> 4;
+          uint32_t zero;
+          asm volatile("v_mov_b32 %0, 0" : "=v"(zero));   // keeps widened operands out of registers across the loop
 #pragma unroll
-          for (int d = 0; d < DT16; d++) {
-            f32x4 r = o[d];
+          for (int n = 0; n < NCT; n++) {
+            const bool counts = (__shfl((int)seen[n], (k & 48) + col, 64) >> i) & 1;
 #pragma unroll
-            for (int h = 0; h < 2; h++) r = mfma16<MT>(only<MT>(seen_fragment(d, h), here, i - 8 * h), only<MT>(pf[h], here, i - 8 * h), r);
-            if (counts) o[d] = r;
+            for (int d = 0; d < DT16; d++) {
+              f32x4 x = o[n][d];
+#pragma unroll
+              for (int h = 0; h < 2; h++) {
+                u32x4 v;
+                if constexpr (EB == 1) v = widen8<KV>(vf[d][0] ^ u32x4{zero, zero, zero, zero}, h);
+                else v = vf[d][h] ^ u32x4{zero, zero, zero, zero};
+                x = mfma16<MT>(only<MT>(v, here, i - 8 * h), only<MT>(pf[n][h], here, i - 8 * h), x);
+              }
+              if (counts) o[n][d] = x;
+            }
           }
         }
       }
     }
-    if (more) load_v(vp);
   }
 
-  // ---- the four waves meet -------------------------------------------------------------------------------------------
-  l = group_sum(l);
-  if (g == 0) {
-    stat[wave][0][col] = m;
-    stat[wave][1][col] = l;
-  }
-  __syncthreads();
-  const float mall = fmaxf(fmaxf(stat[0][0][col], stat[1][0][col]), fmaxf(stat[2][0][col], stat[3][0][col]));
-  {
-    float a = m == -INFINITY ? 0.f : exp2_fast(m - mall);
-    if constexpr (KV != KV16) a *= vref;
+  // ---- the waves meet --------------------------------------------------------------------------------------------------
 #pragma unroll
-    for (int d = 0; d < DT16; d++) *reinterpret_cast<f32x4*>(&acc[wave][col * LD + 16 * d + 4 * g]) = o[d] * a;
+  for (int n = 0; n < NCT; n++) {
+    l[n] = group_sum(l[n]);
+    if (g == 0) {
+      stat[wave][0][16 * n + col] = m[n];
+      stat[wave][1][16 * n + col] = l[n];
+    }
   }
   __syncthreads();
   constexpr int PER = HEAD / 16;
-  const int cc = threadIdx.x >> 4, d0 = (threadIdx.x & 15) * PER;
-  if (c0 + cc > c1) return;
-  float top = -INFINITY, sum = 0.f;
+  const int width = p.lds_cols;          // columns of a 16-column tile that exist in some workgroup
 #pragma unroll
-  for (int w = 0; w < 4; w++) top = fmaxf(top, stat[w][0][cc]);
+  for (int n = 0; n < NCT; n++) {
+    if (c0 + 16 * n > c1) break;
+    if (n > 0) __syncthreads();
+    float mall = stat[0][0][16 * n + col];
 #pragma unroll
-  for (int w = 0; w < 4; w++) sum += stat[w][0][cc] == -INFINITY ? 0.f : stat[w][1][cc] * exp2_fast(stat[w][0][cc] - top);
-  float v[PER];
+    for (int w = 1; w < NW; w++) mall = fmaxf(mall, stat[w][0][16 * n + col]);
+    float a = m[n] == -INFINITY ? 0.f : exp2_fast(m[n] - mall);
+    if constexpr (KV != KV16) a *= vref;
+    if (col < width) {
 #pragma unroll
-  for (int i = 0; i < PER; i++) v[i] = (acc[0][cc * LD + d0 + i] + acc[1][cc * LD + d0 + i]) + (acc[2][cc * LD + d0 + i] + acc[3][cc * LD + d0 + i]);
-  const int orow = start + (c0 + cc) / G, ohead = kvh * G + (c0 + cc) % G;
-  if (whole) {
-    const float inv = top == -INFINITY ? 0.f : 1.f / sum;
-    uint32_t* out = reinterpret_cast<uint32_t*>(p.out + (int64_t)orow * p.out_stride + (int64_t)ohead * HEAD + d0);
+      for (int d = 0; d < DT16; d++) *reinterpret_cast<f32x4*>(&acc[(wave * width + col) * LD + 16 * d + 4 * g]) = o[n][d] * a;
+    }
+    __syncthreads();
+    const int cc = threadIdx.x >> 4, d0 = (threadIdx.x & 15) * PER, c = c0 + 16 * n + cc;
+    if (cc >= 16 || c > c1) continue;
+    float top = -INFINITY, sum = 0.f;
 #pragma unroll
-    for (int i = 0; i < PER / 2; i++) out[i] = top == -INFINITY ? 0u : pack2<DT>(v[2 * i] * inv, v[2 * i + 1] * inv);
-  } else {
-    const int64_t at = ((int64_t)orow * p.num_heads + ohead) * p.part_stride + split;
+    for (int w = 0; w < NW; w++) top = fmaxf(top, stat[w][0][16 * n + cc]);
+    f32x4 v[PER / 4];
 #pragma unroll
-    for (int i = 0; i < PER; i += 4) *reinterpret_cast<f32x4*>(p.part_o + at * HEAD + d0 + i) = f32x4{v[i], v[i + 1], v[i + 2], v[i + 3]};
-    if (d0 == 0) {
-      p.part_ml[2 * at] = top;
-      p.part_ml[2 * at + 1] = sum;
+    for (int i = 0; i < PER / 4; i++) v[i] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int w = 0; w < NW; w++) {
+      const float mw = stat[w][0][16 * n + cc];
+      sum += mw == -INFINITY ? 0.f : stat[w][1][16 * n + cc] * exp2_fast(mw - top);
+#pragma unroll
+      for (int i = 0; i < PER / 4; i++) v[i] += *reinterpret_cast<const f32x4*>(&acc[(w * width + cc) * LD + d0 + 4 * i]);
+    }
+    const int orow = start + c / G, ohead = kvh * G + c % G;
+    if (whole) {
+      const float inv = top == -INFINITY ? 0.f : 1.f / sum;
+      uint32_t* out = reinterpret_cast<uint32_t*>(p.out + (int64_t)orow * p.out_stride + (int64_t)ohead * HEAD + d0);
+#pragma unroll
+      for (int i = 0; i < PER / 2; i++) out[i] = top == -INFINITY ? 0u : pack2<DT>(v[i >> 1][2 * (i & 1)] * inv, v[i >> 1][2 * (i & 1) + 1] * inv);
+    } else {
+      const int64_t to = ((int64_t)orow * p.num_heads + ohead) * p.part_stride + split;
+#pragma unroll
+      for (int i = 0; i < PER / 4; i++) *reinterpret_cast<f32x4*>(p.part_o + to * HEAD + d0 + 4 * i) = v[i];
+      if (d0 == 0) {
+        p.part_ml[2 * to] = top;
+        p.part_ml[2 * to + 1] = sum;
+      }
     }
   }
 }
@@ -1013,43 +1135,53 @@ __global__ __launch_bounds__(256) void window_merge_kernel(const WindowParams p,
 // ---------------------------------------------------------------------------------------------------------------------
 // how a call is cut: host side, from what the caller bounds
 // ---------------------------------------------------------------------------------------------------------------------
-struct WindowPart { int col_tiles, splits, split_tiles; };
+struct WindowPart { int cols, waves, col_tiles, splits, split_tiles; };
 struct WindowPlan {
   WindowPart rows, flash;       // col_tiles 0: not launched
   int part_stride;
 };
 
-// columns (rows x heads per kv head) up to which a sequence is served 16 at a time
+// columns (rows x heads per kv head) up to which a sequence is served 16 or 32 at a time
 constexpr int WA_ROWS_COLS = 64;
 constexpr int WA_WAVES = 8, WA_FLASH_COLS = 32 * WA_WAVES;
 
-static WindowPart window_part(int64_t max_cols, int cols, int G, int num_seqs, int num_kv_heads, int max_seq_len, int window, int sinks,
-                              int groups_wanted, int least_tiles) {
-  WindowPart w;
-  w.col_tiles = (int)((max_cols + cols - 1) / cols);
-  // tiles that `cols` columns see: the window of their first row, their own rows, an unaligned start, the sinks
+// 64-token tiles that `cols` columns see at most: the window of their first row, their own rows, an unaligned start, the sinks
+static int64_t window_tiles(int cols, int G, int max_seq_len, int window, int sinks) {
   int64_t tiles = ((int64_t)max_seq_len + 63) / 64;
   if (window)
     tiles = std::min(tiles + 1, ((int64_t)std::min(window, max_seq_len) + (cols + G - 1) / G + 15 + 63) / 64 +
                                     ((int64_t)std::min(sinks, max_seq_len) + 63) / 64);
-  tiles = std::max<int64_t>(tiles, 1);
-  const int64_t groups = (int64_t)num_seqs * num_kv_heads * w.col_tiles;
-  const int64_t want = std::max<int64_t>(1, (groups_wanted + groups - 1) / groups);
+  return std::max<int64_t>(tiles, 1);
+}
+static void window_cut(WindowPart& w, int64_t tiles, int64_t want, int least_tiles) {
   w.split_tiles = (int)std::max<int64_t>(least_tiles, (tiles + want - 1) / want);
   w.splits = (int)((tiles + w.split_tiles - 1) / w.split_tiles);
-  return w;
 }
 
-static WindowPlan window_plan(int num_seqs, int num_rows, int num_heads, int num_kv_heads, int max_query_len, int max_seq_len, int window, int sinks) {
+static WindowPlan window_plan(int num_seqs, int num_rows, int num_heads, int num_kv_heads, int kv_type, int max_query_len, int max_seq_len,
+                              int window, int sinks) {
   WindowPlan w{};
   const int G = num_heads / num_kv_heads;
   const int64_t cols = (int64_t)max_query_len * G;
   const bool prompts = cols > WA_ROWS_COLS;
   // a batch whose sequences all have max_query_len rows needs one kind only
-  if (!prompts || (int64_t)num_seqs * max_query_len != num_rows)
-    // four workgroups for each of the 256 CUs, at least 4 tiles (one per wave) in each
-    w.rows = window_part(std::min<int64_t>(cols, WA_ROWS_COLS), 16, G, num_seqs, num_kv_heads, max_seq_len, window, sinks, 1024, 4);
-  if (prompts) w.flash = window_part(cols, WA_FLASH_COLS, G, num_seqs, num_kv_heads, max_seq_len, window, sinks, 256, 16);
+  if (!prompts || (int64_t)num_seqs * max_query_len != num_rows) {
+    const int64_t mine = std::min<int64_t>(cols, WA_ROWS_COLS);
+    // 32 columns to a workgroup read a draft's K and V once instead of twice; a 16-bit tile leaves no registers for it
+    w.rows.cols = mine > 16 && kv_type != MI355Q_KV_16 ? 32 : 16;
+    w.rows.col_tiles = (int)((mine + w.rows.cols - 1) / w.rows.cols);
+    const int64_t tiles = window_tiles(w.rows.cols, G, max_seq_len, window, sinks);
+    const int64_t groups = (int64_t)num_seqs * num_kv_heads * w.rows.col_tiles;
+    w.rows.waves = groups <= 256 || w.rows.cols == 32 ? 8 : 4;
+    window_cut(w.rows, tiles, groups <= 256 ? 256 / groups : (2048 + groups - 1) / groups, 4 * w.rows.waves);
+  }
+  if (prompts) {
+    w.flash.cols = WA_FLASH_COLS;
+    w.flash.waves = WA_WAVES;
+    w.flash.col_tiles = (int)((cols + WA_FLASH_COLS - 1) / WA_FLASH_COLS);
+    const int64_t groups = (int64_t)num_seqs * num_kv_heads * w.flash.col_tiles;
+    window_cut(w.flash, window_tiles(WA_FLASH_COLS, G, max_seq_len, window, sinks), std::max<int64_t>(1, (256 + groups - 1) / groups), 16);
+  }
   w.part_stride = std::max(w.rows.splits, w.flash.splits);
   return w;
 }
@@ -1061,9 +1193,9 @@ static size_t window_workspace(const WindowPlan& w, int num_rows, int num_heads,
 template <typename DT, int KV, int HEAD>
 static int launch_window(WindowParams p, const WindowPlan& w, hipStream_t s) {
   auto groups = [&](const WindowPart& a) { return (int64_t)p.num_seqs * p.num_kv_heads * a.col_tiles * a.splits; };
-  auto merges = [&](const WindowPart& a, int cols) { return (int64_t)p.num_seqs * p.num_kv_heads * a.col_tiles * (cols / 4); };
+  auto merges = [&](const WindowPart& a) { return (int64_t)p.num_seqs * p.num_kv_heads * a.col_tiles * (a.cols / 4); };
   const int64_t most = (int64_t)1 << 31;
-  MI355Q_REQUIRE(groups(w.rows) < most && groups(w.flash) < most && merges(w.rows, 16) < most && merges(w.flash, WA_FLASH_COLS) < most,
+  MI355Q_REQUIRE(groups(w.rows) < most && groups(w.flash) < most && merges(w.rows) < most && merges(w.flash) < most,
                  "paged_window_attention: too many workgroups");
   for (int kind = 0; kind < 2; kind++) {
     const WindowPart& a = kind ? w.flash : w.rows;
@@ -1072,13 +1204,21 @@ static int launch_window(WindowParams p, const WindowPlan& w, hipStream_t s) {
     p.split_tiles = a.splits == 1 ? INT_MAX : a.split_tiles;
     p.min_cols = kind ? WA_ROWS_COLS + 1 : 0;
     p.max_cols = kind ? INT_MAX : WA_ROWS_COLS;
-    const dim3 grid((unsigned)groups(a));
-    if (kind) hipLaunchKernelGGL((window_flash_kernel<DT, KV, HEAD, WA_WAVES>), grid, dim3(64 * WA_WAVES), 0, s, p);
-    else hipLaunchKernelGGL((window_rows_kernel<DT, KV, HEAD>), grid, dim3(256), 0, s, p);
+    p.lds_cols = std::min(16, p.longest_cols);
+    const dim3 grid((unsigned)groups(a)), wg(64 * a.waves);
+    const size_t lds = (size_t)a.waves * p.lds_cols * (HEAD + 4) * sizeof(float);
+    if (kind) {
+      hipLaunchKernelGGL((window_flash_kernel<DT, KV, HEAD, WA_WAVES>), grid, wg, 0, s, p);
+    } else if (a.cols == 32) {
+      if constexpr (KV != KV16) hipLaunchKernelGGL((window_rows_kernel<DT, KV, HEAD, 2, 8>), grid, wg, lds, s, p);
+    } else if (a.waves == 8) {
+      hipLaunchKernelGGL((window_rows_kernel<DT, KV, HEAD, 1, 8>), grid, wg, lds, s, p);
+    } else {
+      hipLaunchKernelGGL((window_rows_kernel<DT, KV, HEAD, 1, 4>), grid, wg, lds, s, p);
+    }
     if (int e = check_launch("paged_window_attention")) return e;
     if (a.splits > 1) {
-      const int cols = kind ? WA_FLASH_COLS : 16;
-      hipLaunchKernelGGL((window_merge_kernel<DT, HEAD>), dim3((unsigned)merges(a, cols)), dim3(256), 0, s, p, cols);
+      hipLaunchKernelGGL((window_merge_kernel<DT, HEAD>), dim3((unsigned)merges(a)), dim3(256), 0, s, p, a.cols);
       if (int e = check_launch("paged_window_attention")) return e;
     }
   }
@@ -1090,9 +1230,9 @@ static int launch_window(WindowParams p, const WindowPlan& w, hipStream_t s) {
 using namespace mi355q;
 
 extern "C" size_t mi355q_paged_window_attention_workspace_bytes(int num_seqs, int num_rows, int num_heads, int num_kv_heads, int head_size,
-                                                                int max_query_len, int max_seq_len, int window, int sinks) {
+                                                                int max_query_len, int max_seq_len, int window, int sinks, int kv_type) {
   if (num_seqs <= 0 || num_rows <= 0 || num_kv_heads <= 0 || num_heads <= 0 || max_query_len <= 0 || max_seq_len <= 0) return 0;
-  return window_workspace(window_plan(num_seqs, num_rows, num_heads, num_kv_heads, max_query_len, max_seq_len, window, sinks), num_rows, num_heads,
+  return window_workspace(window_plan(num_seqs, num_rows, num_heads, num_kv_heads, kv_type, max_query_len, max_seq_len, window, sinks), num_rows, num_heads,
                           head_size);
 }
 
@@ -1125,7 +1265,7 @@ extern "C" int mi355q_paged_window_attention(void* out, int64_t out_stride, cons
   MI355Q_REQUIRE((((uintptr_t)key_cache | (uintptr_t)value_cache | (uintptr_t)query) & 15) == 0 && q_stride % 8 == 0,
                  "paged_window_attention: caches and query rows must be 16-byte aligned");
   MI355Q_REQUIRE(((uintptr_t)out & 3) == 0 && out_stride % 2 == 0, "paged_window_attention: output rows must be 4-byte aligned");
-  const WindowPlan w = window_plan(num_seqs, num_rows, num_heads, num_kv_heads, max_query_len, max_seq_len, window, sinks);
+  const WindowPlan w = window_plan(num_seqs, num_rows, num_heads, num_kv_heads, kv_type, max_query_len, max_seq_len, window, sinks);
   const size_t need = window_workspace(w, num_rows, num_heads, head_size);
   if (need && (!workspace || workspace_bytes < need))
     return set_error(MI355Q_ENOSPACE, "paged_window_attention: workspace of %zu bytes, %zu needed", workspace ? workspace_bytes : (size_t)0, need);
@@ -1150,6 +1290,7 @@ extern "C" int mi355q_paged_window_attention(void* out, int64_t out_stride, cons
   p.page_magic = pieces == 1 ? 0 : (int)(((1ull << 32) + pieces - 1) / pieces);
   p.window = std::min(window, 1 << 30), p.sinks = sinks;
   p.part_stride = w.part_stride;
+  p.longest_cols = (int)std::min<int64_t>((int64_t)max_query_len * p.group, WA_ROWS_COLS);
   p.out16 = ((uintptr_t)out & 15) == 0 && out_stride % 8 == 0;
   hipStream_t s = (hipStream_t)stream;
 #define BY_KV(DT, HD)                                                                                                     \

@@ -140,7 +140,7 @@ _SIGS = {
     "mi355q_rope_and_cache_blocks": (c_int, [c_vp, c_vp, c_i64, c_vp, c_i64, c_vp, c_i64, c_vp, c_i64, c_int, c_int, c_int,
                                              c_vp, c_int, c_int, c_int, c_int, c_vp, c_vp, c_int, c_int, c_i64, c_vp, c_vp,
                                              c_i64, c_i64, c_vp, c_int, c_int, c_int, c_vp]),
-    "mi355q_paged_window_attention_workspace_bytes": (c_sz, [c_int] * 9),
+    "mi355q_paged_window_attention_workspace_bytes": (c_sz, [c_int] * 10),
     "mi355q_paged_window_attention": (c_int, [c_vp, c_i64, c_vp, c_i64, c_vp, c_vp, c_i64, c_i64, c_int, c_int, c_int, c_int,
                                               c_int, c_int, c_f32, c_vp, c_int, c_vp, c_vp, c_int, c_int, c_int, c_int, c_int,
                                               c_int, c_int, c_vp, c_vp, c_i64, c_i64, c_vp, c_sz, c_vp]),

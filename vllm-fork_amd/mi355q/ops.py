@@ -1368,11 +1368,18 @@ def _append_blocks(what, positions, q2, o2, key, value, head_size, cos_sin, is_n
             slot_mapping.data_ptr(), T, _dt(key), _BLOCK_CODES[kv_cache_dtype])
 
 
+def _kv_type(kv_cache_dtype: str) -> int:
+    if kv_cache_dtype in _BLOCK_CODES:
+        return _BLOCK_CODES[kv_cache_dtype]
+    return _lib.KV_FP8 if _is_fp8(kv_cache_dtype) else _lib.KV_16
+
+
 def paged_window_attention_workspace_bytes(num_seqs: int, num_rows: int, num_heads: int, num_kv_heads: int, head_size: int,
-                                           max_query_len: int, max_seq_len: int, sliding_window: int = 0, sink_tokens: int = 0) -> int:
+                                           max_query_len: int, max_seq_len: int, kv_cache_dtype: str, sliding_window: int = 0,
+                                           sink_tokens: int = 0) -> int:
     """Scratch that `paged_window_attention` takes for a batch of these bounds (0 for many)."""
     return _lib.lib().mi355q_paged_window_attention_workspace_bytes(num_seqs, num_rows, num_heads, num_kv_heads, head_size, max_query_len,
-                                                                    max_seq_len, sliding_window, sink_tokens)
+                                                                    max_seq_len, sliding_window, sink_tokens, _kv_type(kv_cache_dtype))
 
 
 def paged_window_attention(out: torch.Tensor, query: torch.Tensor, key_cache: torch.Tensor, value_cache: torch.Tensor, num_kv_heads: int,
@@ -1405,14 +1412,10 @@ def paged_window_attention(out: torch.Tensor, query: torch.Tensor, key_cache: to
         raise RuntimeError(f"{what}: query_start_loc must be contiguous int32 [{S + 1}]")
     if sliding_window < 0 or sink_tokens < 0:
         raise RuntimeError(f"{what}: sliding_window and sink_tokens must not be negative")
-    if kv_cache_dtype in _BLOCK_CODES:
-        kv, element = _BLOCK_CODES[kv_cache_dtype], 1
-    elif _is_fp8(kv_cache_dtype):
-        kv, element = _lib.KV_FP8, 1
-    else:
-        kv, element = _lib.KV_16, 2
-        if key_cache.dtype != query.dtype or value_cache.dtype != query.dtype:
-            raise RuntimeError(f"{what}: a 16-bit cache must have the query's dtype")
+    kv = _kv_type(kv_cache_dtype)
+    element = 2 if kv == _lib.KV_16 else 1
+    if element == 2 and (key_cache.dtype != query.dtype or value_cache.dtype != query.dtype):
+        raise RuntimeError(f"{what}: a 16-bit cache must have the query's dtype")
     kvh, bs = _paged_cache(what, key_cache, value_cache, D, element)
     if kvh != num_kv_heads:
         raise RuntimeError(f"{what}: {num_kv_heads} kv heads over a cache of {kvh}")
@@ -1429,7 +1432,7 @@ def paged_window_attention(out: torch.Tensor, query: torch.Tensor, key_cache: to
     if rows == 0 or S == 0:
         return
     L = _lib.lib()
-    need = L.mi355q_paged_window_attention_workspace_bytes(S, rows, H, kvh, D, max_query_len, max_seq_len, sliding_window, sink_tokens)
+    need = L.mi355q_paged_window_attention_workspace_bytes(S, rows, H, kvh, D, max_query_len, max_seq_len, sliding_window, sink_tokens, kv)
     if need and workspace is None:
         workspace = torch.empty(need, dtype=torch.uint8, device=query.device)
     _launch(query.device, L.mi355q_paged_window_attention, out.data_ptr(), out.stride(0), query.data_ptr(), query.stride(0),
