@@ -1260,42 +1260,56 @@ def is_block_scaled(kv_cache_dtype: str) -> bool:
     return kv_cache_dtype in _BLOCK_CODES
 
 
-def _one_device(what: str, first: torch.Tensor, *ts) -> None:
-    for t in (first, *ts):
-        if t is not None and (not t.is_cuda or t.device != first.device):
-            raise RuntimeError(f"{what}: every tensor must be on one GPU (MI355X); no CPU fallback exists")
+def _one_device(what: str, *ts) -> int:
+    """Index of the GPU that every tensor lives on."""
+    index = ts[0].get_device()
+    for t in ts:
+        if t is not None and t.get_device() != index:
+            index = -1
+    if index < 0:
+        raise RuntimeError(f"{what}: every tensor must be on one GPU (MI355X); no CPU fallback exists")
+    return index
 
 
-def _launch(device: torch.device, fn, *args) -> None:
-    """fn(*args, stream) on the device the tensors live on, on torch's current stream there."""
-    if device.index == torch.cuda.current_device():
-        check(fn(*args, _stream()))
+_raw_stream = torch._C._cuda_getCurrentRawStream   # torch.cuda.current_stream(index).cuda_stream without the objects
+
+
+def _launch(index: int, fn, *args) -> None:
+    """fn(*args, stream) on GPU `index`, on torch's current stream there."""
+    if index == torch.cuda.current_device():
+        check(fn(*args, _raw_stream(index)))
     else:
-        with torch.cuda.device(device):
-            check(fn(*args, _stream()))
+        with torch.cuda.device(index):
+            check(fn(*args, _raw_stream(index)))
+
+
+def _rows(t: torch.Tensor, T: int) -> torch.Tensor:
+    return t if t.dim() == 2 else t.view(T, -1)
 
 
 def _paged_cache(what: str, key_cache: torch.Tensor, value_cache: torch.Tensor, head_size: int, element: int):
-    """(kv heads, block size) of K [blocks, kv_heads, head / x, block, x] and V [blocks, kv_heads, head, block]."""
+    """(blocks, kv heads, block size, strides) of K [blocks, kv_heads, head / x, block, x] and V [blocks, kv_heads, head, block]."""
     x = 16 // element
-    if value_cache.dim() != 4 or key_cache.dim() != 5:
+    ks, vs, kt, vt = key_cache.shape, value_cache.shape, key_cache.stride(), value_cache.stride()
+    if len(vs) != 4 or len(ks) != 5:
         raise RuntimeError(f"{what}: key_cache must be [blocks, kv_heads, head / {x}, block, {x}], value_cache [blocks, kv_heads, head, block]")
-    n, kvh, d, bs = value_cache.shape
-    if d != head_size or key_cache.shape != (n, kvh, head_size // x, bs, x) or n == 0:
-        raise RuntimeError(f"{what}: cache shapes {tuple(key_cache.shape)} / {tuple(value_cache.shape)} for heads of {head_size}")
+    n, kvh, d, bs = vs
+    if d != head_size or ks != (n, kvh, d // x, bs, x) or n == 0:
+        raise RuntimeError(f"{what}: cache shapes {tuple(ks)} / {tuple(vs)} for heads of {head_size}")
     if key_cache.element_size() != element or value_cache.element_size() != element:
         raise RuntimeError(f"{what}: cache elements must have {element} bytes")
-    if key_cache.stride()[2:] != (bs * x, x, 1) or value_cache.stride()[2:] != (bs, 1) or key_cache.stride()[:2] != value_cache.stride()[:2]:
+    if kt[2:] != (bs * x, x, 1) or vt[2:] != (bs, 1) or kt[:2] != vt[:2]:
         raise RuntimeError(f"{what}: the pages of a head must be contiguous, and both caches laid out alike")
-    return kvh, bs
+    return n, kvh, bs, kt
 
 
-def _block_scales(what: str, k_scales: torch.Tensor, v_scales: torch.Tensor, blocks: int, kvh: int) -> None:
-    for s in (k_scales, v_scales):
-        if s.dtype != torch.float32 or s.shape != (blocks, kvh):
-            raise RuntimeError(f"{what}: scales must be fp32 [{blocks}, {kvh}]")
-    if k_scales.stride() != v_scales.stride():
+def _block_scales(what: str, k_scales: torch.Tensor, v_scales: torch.Tensor, blocks: int, kvh: int):
+    if k_scales.dtype != torch.float32 or v_scales.dtype != torch.float32 or k_scales.shape != (blocks, kvh) or v_scales.shape != (blocks, kvh):
+        raise RuntimeError(f"{what}: scales must be fp32 [{blocks}, {kvh}]")
+    strides = k_scales.stride()
+    if strides != v_scales.stride():
         raise RuntimeError(f"{what}: k_scales and v_scales must have the same strides")
+    return strides
 
 
 def rope_and_cache_blocks(positions: torch.Tensor, query: torch.Tensor, key: torch.Tensor, value: torch.Tensor, head_size: int,
@@ -1309,22 +1323,27 @@ def rope_and_cache_blocks(positions: torch.Tensor, query: torch.Tensor, key: tor
     slot_mapping int64 [T]: negative slots and slots past the cache are skipped; the tokens of one block follow one
     another (skipped ones may stand between them).  Not idempotent on `query` when in place, and tokens must be appended in their order."""
     what = "rope_and_cache_blocks"
-    _one_device(what, key, positions, query, value, cos_sin_cache, key_cache, value_cache, k_scales, v_scales, slot_mapping, query_out)
+    index = _one_device(what, key, positions, query, value, cos_sin_cache, key_cache, value_cache, k_scales, v_scales, slot_mapping, query_out)
     T = slot_mapping.numel()
     if positions.dtype != torch.int64 or slot_mapping.dtype != torch.int64 or positions.numel() != T:
         raise RuntimeError(f"{what}: positions and slot_mapping must be int64 [T]")
     if not positions.is_contiguous() or not slot_mapping.is_contiguous():
         raise RuntimeError(f"{what}: positions and slot_mapping must be contiguous")
-    q2 = query.view(T, -1)
-    o2 = q2 if query_out is None else query_out.view(T, -1)
-    if cos_sin_cache.dim() != 2 or not cos_sin_cache.is_contiguous() or cos_sin_cache.shape[1] > head_size or cos_sin_cache.shape[1] % 2:
+    if T == 0:
+        return
+    q2 = _rows(query, T)
+    o2 = q2 if query_out is None else _rows(query_out, T)
+    table = cos_sin_cache.shape
+    if len(table) != 2 or not cos_sin_cache.is_contiguous() or table[1] > head_size or table[1] % 2:
         raise RuntimeError(f"{what}: cos_sin_cache must be contiguous [positions, rot_dim] with an even rot_dim of at most {head_size}")
-    if q2.shape != o2.shape or q2.shape[1] % head_size or o2.dtype != key.dtype or q2.dtype != key.dtype:
+    width, qs, os_ = q2.shape[1], q2.stride(), o2.stride()
+    if q2.shape != (T, width) or o2.shape != (T, width) or width % head_size or o2.dtype != key.dtype or q2.dtype != key.dtype:
         raise RuntimeError(f"{what}: query and query_out must be [T, heads * {head_size}] of the key's dtype")
-    if T and (q2.stride(1) != 1 or o2.stride(1) != 1):
+    if qs[1] != 1 or os_[1] != 1:
         raise RuntimeError(f"{what}: query rows must be contiguous")
-    _append_blocks(what, positions, q2, o2, key, value, head_size, cos_sin_cache, is_neox, key_cache, value_cache, k_scales, v_scales,
-                   slot_mapping, kv_cache_dtype)
+    _append_blocks(what, index, (positions.data_ptr(), q2.data_ptr(), qs[0], o2.data_ptr(), os_[0]), key, value, head_size, width // head_size,
+                   (cos_sin_cache.data_ptr(), table[1], table[0], _dt(cos_sin_cache, True), int(is_neox)), key_cache, value_cache, k_scales,
+                   v_scales, slot_mapping, T, kv_cache_dtype)
 
 
 def reshape_and_cache_blocks(key: torch.Tensor, value: torch.Tensor, key_cache: torch.Tensor, value_cache: torch.Tensor,
@@ -1332,7 +1351,7 @@ def reshape_and_cache_blocks(key: torch.Tensor, value: torch.Tensor, key_cache: 
     """The append of `rope_and_cache_blocks` without a rotation: the block-scaled form of `reshape_and_cache`.
     key / value [T, kv_heads, head]; T may exceed slot_mapping's length (graph padding)."""
     what = "reshape_and_cache_blocks"
-    _one_device(what, key, value, key_cache, value_cache, k_scales, v_scales, slot_mapping)
+    index = _one_device(what, key, value, key_cache, value_cache, k_scales, v_scales, slot_mapping)
     if slot_mapping.dtype != torch.int64 or not slot_mapping.is_contiguous():
         raise RuntimeError(f"{what}: slot_mapping must be contiguous int64 [T]")
     T, head_size = slot_mapping.numel(), value_cache.shape[2] if value_cache.dim() == 4 else 0
@@ -1340,32 +1359,27 @@ def reshape_and_cache_blocks(key: torch.Tensor, value: torch.Tensor, key_cache: 
         raise RuntimeError(f"{what}: key and value must be [T, kv_heads, head] with a row for each slot")
     if key.stride()[1:] != (key.shape[2], 1) or value.dim() != 3 or value.stride()[1:] != (value.shape[2], 1):
         raise RuntimeError(f"{what}: key / value rows must be contiguous")
-    _append_blocks(what, None, None, None, key[:T].flatten(1), value[:T].flatten(1), head_size, None, False, key_cache, value_cache, k_scales,
-                   v_scales, slot_mapping, kv_cache_dtype)
+    if T:
+        _append_blocks(what, index, (None, None, 0, None, 0), key[:T].flatten(1), value[:T].flatten(1), head_size, 0, (None, 0, 0, BF16, 0),
+                       key_cache, value_cache, k_scales, v_scales, slot_mapping, T, kv_cache_dtype)
 
 
-def _append_blocks(what, positions, q2, o2, key, value, head_size, cos_sin, is_neox, key_cache, value_cache, k_scales, v_scales,
-                   slot_mapping, kv_cache_dtype) -> None:
-    if kv_cache_dtype not in _BLOCK_CODES:
+def _append_blocks(what, index, query, key, value, head_size, heads, table, key_cache, value_cache, k_scales, v_scales, slot_mapping, T,
+                   kv_cache_dtype) -> None:
+    code = _BLOCK_CODES.get(kv_cache_dtype)
+    if code is None:
         raise RuntimeError(f"{what}: unsupported kv_cache_dtype {kv_cache_dtype!r} (block_int8 or block_fp8)")
-    T = slot_mapping.numel()
-    kvh, bs = _paged_cache(what, key_cache, value_cache, head_size, 1)
-    if key_cache.stride(1) != head_size * bs:
+    blocks, kvh, bs, strides = _paged_cache(what, key_cache, value_cache, head_size, 1)
+    if strides[1] != head_size * bs:
         raise RuntimeError(f"{what}: the heads of a block must be contiguous")
-    blocks = key_cache.shape[0]
-    _block_scales(what, k_scales, v_scales, blocks, kvh)
-    k2, v2 = key.view(T, -1), value.view(T, -1)
-    if T == 0:
-        return
-    if k2.shape[1] != kvh * head_size or v2.shape != k2.shape or k2.stride(1) != 1 or v2.stride(1) != 1 or v2.dtype != key.dtype:
+    scale_strides = _block_scales(what, k_scales, v_scales, blocks, kvh)
+    k2, v2 = _rows(key, T), _rows(value, T)
+    ks, vs = k2.stride(), v2.stride()
+    if k2.shape != (T, kvh * head_size) or v2.shape != k2.shape or ks[1] != 1 or vs[1] != 1 or v2.dtype != key.dtype:
         raise RuntimeError(f"{what}: key and value must be [T, {kvh} * {head_size}] with contiguous rows")
-    _launch(key.device, _lib.lib().mi355q_rope_and_cache_blocks,
-            _ptr(positions), _ptr(q2), 0 if q2 is None else q2.stride(0), _ptr(o2), 0 if o2 is None else o2.stride(0), k2.data_ptr(),
-            k2.stride(0), v2.data_ptr(), v2.stride(0), head_size, 0 if q2 is None else q2.shape[1] // head_size, kvh, _ptr(cos_sin),
-            0 if cos_sin is None else cos_sin.shape[1], 0 if cos_sin is None else cos_sin.shape[0],
-            BF16 if cos_sin is None else _dt(cos_sin, True), int(is_neox), key_cache.data_ptr(), value_cache.data_ptr(), blocks, bs,
-            key_cache.stride(0), k_scales.data_ptr(), v_scales.data_ptr(), k_scales.stride(0), k_scales.stride(1),
-            slot_mapping.data_ptr(), T, _dt(key), _BLOCK_CODES[kv_cache_dtype])
+    _launch(index, _lib.lib().mi355q_rope_and_cache_blocks, *query, k2.data_ptr(), ks[0], v2.data_ptr(), vs[0], head_size, heads, kvh, *table,
+            key_cache.data_ptr(), value_cache.data_ptr(), blocks, bs, strides[0], k_scales.data_ptr(), v_scales.data_ptr(), *scale_strides,
+            slot_mapping.data_ptr(), T, _dt(key), code)
 
 
 def _kv_type(kv_cache_dtype: str) -> int:
@@ -1396,15 +1410,17 @@ def paged_window_attention(out: torch.Tensor, query: torch.Tensor, key_cache: to
     only decides how the work is cut.  Pages that no row sees are never looked at.  workspace: uint8 scratch of
     `paged_window_attention_workspace_bytes`, not shared with calls that may overlap; by default taken from the allocator."""
     what = "paged_window_attention"
-    _one_device(what, query, out, key_cache, value_cache, block_tables, seq_lens, query_start_loc, workspace)
-    if query.dim() != 3 or out.shape != query.shape or out.dtype != query.dtype:
+    index = _one_device(what, query, out, key_cache, value_cache, block_tables, seq_lens, query_start_loc, workspace)
+    shape, qs, os_ = query.shape, query.stride(), out.stride()
+    if len(shape) != 3 or out.shape != shape or out.dtype != query.dtype:
         raise RuntimeError(f"{what}: out and query must be [rows, heads, head] of one dtype")
-    rows, H, D = query.shape
-    if rows and (query.stride()[1:] != (D, 1) or out.stride()[1:] != (D, 1)):
+    rows, H, D = shape
+    if rows and (qs[1:] != (D, 1) or os_[1:] != (D, 1)):
         raise RuntimeError(f"{what}: the heads of a row must be contiguous")
-    if block_tables.dtype != torch.int32 or seq_lens.dtype != torch.int32 or block_tables.dim() != 2 or not block_tables.is_contiguous():
+    tables = block_tables.shape
+    if block_tables.dtype != torch.int32 or seq_lens.dtype != torch.int32 or len(tables) != 2 or not block_tables.is_contiguous():
         raise RuntimeError(f"{what}: block_tables must be contiguous int32 [S, pages], seq_lens int32 [S]")
-    S = block_tables.shape[0]
+    S = tables[0]
     if seq_lens.shape != (S,) or not seq_lens.is_contiguous():
         raise RuntimeError(f"{what}: seq_lens must be contiguous int32 [{S}]")
     if query_start_loc is not None and (query_start_loc.dtype != torch.int32 or query_start_loc.shape != (S + 1,)
@@ -1416,31 +1432,35 @@ def paged_window_attention(out: torch.Tensor, query: torch.Tensor, key_cache: to
     element = 2 if kv == _lib.KV_16 else 1
     if element == 2 and (key_cache.dtype != query.dtype or value_cache.dtype != query.dtype):
         raise RuntimeError(f"{what}: a 16-bit cache must have the query's dtype")
-    kvh, bs = _paged_cache(what, key_cache, value_cache, D, element)
+    blocks, kvh, bs, strides = _paged_cache(what, key_cache, value_cache, D, element)
     if kvh != num_kv_heads:
         raise RuntimeError(f"{what}: {num_kv_heads} kv heads over a cache of {kvh}")
-    strides = (0, 0)
+    scales = (None, None, 0, 0)
     if element == 1:
         if k_scale is None or v_scale is None:
             raise RuntimeError(f"{what}: an 8-bit cache needs k_scale and v_scale")
-        _one_device(what, query, k_scale, v_scale)
+        if k_scale.get_device() != index or v_scale.get_device() != index:
+            raise RuntimeError(f"{what}: k_scale and v_scale must be on the cache's GPU")
         if kv_cache_dtype in _BLOCK_CODES:
-            _block_scales(what, k_scale, v_scale, key_cache.shape[0], kvh)
-            strides = k_scale.stride()
+            scales = (k_scale.data_ptr(), v_scale.data_ptr(), *_block_scales(what, k_scale, v_scale, blocks, kvh))
         elif k_scale.numel() != 1 or v_scale.numel() != 1 or k_scale.dtype != torch.float32 or v_scale.dtype != torch.float32:
             raise RuntimeError(f"{what}: k_scale and v_scale of an fp8 cache are single fp32 values")
+        else:
+            scales = (k_scale.data_ptr(), v_scale.data_ptr(), 0, 0)
     if rows == 0 or S == 0:
         return
     L = _lib.lib()
     need = L.mi355q_paged_window_attention_workspace_bytes(S, rows, H, kvh, D, max_query_len, max_seq_len, sliding_window, sink_tokens, kv)
-    if need and workspace is None:
-        workspace = torch.empty(need, dtype=torch.uint8, device=query.device)
-    _launch(query.device, L.mi355q_paged_window_attention, out.data_ptr(), out.stride(0), query.data_ptr(), query.stride(0),
-            key_cache.data_ptr(), value_cache.data_ptr(), key_cache.stride(0), key_cache.stride(1), key_cache.shape[0], rows, S, H, kvh, D,
-            scale, block_tables.data_ptr(), block_tables.shape[1], seq_lens.data_ptr(), _ptr(query_start_loc), max_query_len, bs,
-            max_seq_len, sliding_window, sink_tokens, _dt(query), kv, _ptr(k_scale) if element == 1 else None,
-            _ptr(v_scale) if element == 1 else None, strides[0], strides[1], _ptr(workspace),
-            0 if workspace is None else workspace.numel() * workspace.element_size())
+    room = 0
+    if need:
+        if workspace is None:
+            workspace, room = torch.empty(need, dtype=torch.uint8, device=query.device), need
+        else:
+            room = workspace.numel() * workspace.element_size()
+    _launch(index, L.mi355q_paged_window_attention, out.data_ptr(), os_[0], query.data_ptr(), qs[0], key_cache.data_ptr(),
+            value_cache.data_ptr(), strides[0], strides[1], blocks, rows, S, H, kvh, D, scale, block_tables.data_ptr(), tables[1],
+            seq_lens.data_ptr(), _ptr(query_start_loc), max_query_len, bs, max_seq_len, sliding_window, sink_tokens, _dt(query), kv, *scales,
+            workspace.data_ptr() if room else None, room)
 
 
 # ---------------------------------------------------------------------------
