@@ -117,6 +117,10 @@ __device__ inline u32x4 widen8(u32x4 w, int h) {
   return u32x4{a[0], a[1], b[0], b[1]};
 }
 
+
+typedef __attribute__((ext_vector_type(2))) _Float16 cvt_f16x2;
+template <typename MT> __device__ inline uint32_t wpack(float lo, float hi) { return pack2<MT>(lo, hi); }
+template <> __device__ inline uint32_t wpack<FP16>(float lo, float hi) { return __builtin_bit_cast(uint32_t, __builtin_convertvector(f32x2{lo, hi}, cvt_f16x2)); }
 // max over the four lanes that share a column
 __device__ inline float group_max(float v) {
   auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
@@ -645,7 +649,7 @@ __device__ inline float add_pair<FP16>(uint32_t w, float c) {
 constexpr float WA_VSHIFT = 128.0f;
 
 template <typename DT, int KV, int HEAD, int NW>
-__global__ __launch_bounds__(64 * NW, 2) void window_flash_kernel(const WindowParams p) {
+__global__ __launch_bounds__(64 * NW, HEAD == 64 ? 4 : 2) void window_flash_kernel(const WindowParams p) {
   typedef typename MathOf<DT, KV>::T MT;
   constexpr int EB = KV == KV16 ? 2 : 1, NT = 64 * NW, COLS = 32 * NW;
   constexpr int KS = HEAD / 16, DTL = HEAD / 32;
@@ -930,6 +934,13 @@ __global__ __launch_bounds__(64 * NW, 2) void window_flash_kernel(const WindowPa
 #pragma unroll
         for (int k = 0; k < KS; k++) s[rt] = mfma32<MT>(*reinterpret_cast<const u32x4*>(st0 + (rt * KS + k) * 1024), qf[k], s[rt]);
       }
+      __builtin_amdgcn_sched_group_barrier(0x100, 6, 0);
+#pragma unroll
+      for (int k = 0; k < 2 * KS - 6; k++) {
+        __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+        __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+      }
+      __builtin_amdgcn_sched_group_barrier(0x008, 6, 0);
     }
     float f[4];
     if constexpr (KV == KV16) {
@@ -1008,7 +1019,7 @@ __global__ __launch_bounds__(64 * NW, 2) void window_flash_kernel(const WindowPa
     for (int j = 0; j < 4; j++)
 #pragma unroll
       for (int e = 0; e < 4; e++) {
-        pf[j][e] = pack2<MT>(s[j >> 1][8 * (j & 1) + 2 * e], s[j >> 1][8 * (j & 1) + 2 * e + 1]);
+        pf[j][e] = wpack<MT>(s[j >> 1][8 * (j & 1) + 2 * e], s[j >> 1][8 * (j & 1) + 2 * e + 1]);
         l = add_pair<MT>(pf[j][e], l);
       }
 
@@ -1019,6 +1030,13 @@ __global__ __launch_bounds__(64 * NW, 2) void window_flash_kernel(const WindowPa
       for (int d = 0; d < DTL; d++)
 #pragma unroll
         for (int st = 0; st < 4; st++) o[d] = mfma32<MT>(*reinterpret_cast<const u32x4*>(vt + (d * 4 + st) * 1024), pf[st], o[d]);
+      __builtin_amdgcn_sched_group_barrier(0x100, 4, 1);
+#pragma unroll
+      for (int k = 0; k < 4 * DTL - 4; k++) {
+        __builtin_amdgcn_sched_group_barrier(0x008, 1, 1);
+        __builtin_amdgcn_sched_group_barrier(0x100, 1, 1);
+      }
+      __builtin_amdgcn_sched_group_barrier(0x008, 4, 1);
     } else {
       // an infinity or NaN that some columns may see and others must not: one token at a time, added where it is seen
 #pragma unroll 1
@@ -1173,7 +1191,7 @@ static WindowPlan window_plan(int num_seqs, int num_rows, int num_heads, int num
     const int64_t tiles = window_tiles(w.rows.cols, G, max_seq_len, window, sinks);
     const int64_t groups = (int64_t)num_seqs * num_kv_heads * w.rows.col_tiles;
     w.rows.waves = groups <= 256 || w.rows.cols == 32 ? 8 : 4;
-    window_cut(w.rows, tiles, groups <= 256 ? 256 / groups : (2048 + groups - 1) / groups, 4 * w.rows.waves);
+    window_cut(w.rows, tiles, groups <= 256 ? 256 / groups : (2048 + groups - 1) / groups, (tiles <= 4 * w.rows.waves ? 4 : 2) * w.rows.waves);
   }
   if (prompts) {
     w.flash.cols = WA_FLASH_COLS;
