@@ -122,10 +122,14 @@ __device__ inline void load_table(float* out, const void* c, int64_t i, int dtyp
 // cos and sin of 16 elements from d0 on (halves), or of the 8 pairs they form
 struct Angles { float c[16], s[16]; };
 
-__device__ inline void load_angles(Angles& a, const AppendParams& p, int64_t pos, int d0) {
-  pos = pos < 0 ? 0 : pos >= p.max_pos ? p.max_pos - 1 : pos;   // a position outside the table stays inside memory
+// row of the table for token t; a position outside of it is brought to its ends
+__device__ inline int position(const AppendParams& p, int t) {
+  const int64_t pos = p.positions[t];
+  return pos < 0 ? 0 : pos >= p.max_pos ? p.max_pos - 1 : (int)pos;
+}
+__device__ inline void load_angles(Angles& a, const AppendParams& p, int pos, int d0) {
   const int e = p.rot / 2;
-  const int64_t row = pos * p.rot;
+  const int64_t row = (int64_t)pos * p.rot;
   if (p.rot_mode == ROT_HALVES) {
     const int j = d0 < e ? d0 : d0 - e;
     load_table<16>(a.c, p.cos_sin, row + j, p.cos_dtype);
@@ -158,9 +162,9 @@ __device__ inline Row16 rotate16(const Row16& x, const Row16& y, const Angles& a
 
 // ROT_ANY: elements d0 .. d0 + 15 of the head at x
 template <typename DT>
-__device__ inline Row16 rotate16_any(const uint16_t* x, int d0, const AppendParams& p, int64_t pos) {
-  pos = pos < 0 ? 0 : pos >= p.max_pos ? p.max_pos - 1 : pos;
+__device__ inline Row16 rotate16_any(const uint16_t* x, int d0, const AppendParams& p, int pos) {
   const int e = p.rot / 2;
+  const int64_t row = (int64_t)pos * p.rot;
   Row16 r;
 #pragma unroll
   for (int i = 0; i < 16; i += 2) {
@@ -173,14 +177,28 @@ __device__ inline Row16 rotate16_any(const uint16_t* x, int d0, const AppendPara
         const int at = p.is_neox ? (d < e ? d : d - e) : d >> 1;
         const bool first = p.is_neox ? d < e : !(d & 1);
         const int other = p.is_neox ? (first ? d + e : d - e) : d ^ 1;
-        const float c = table_at(p.cos_sin, pos * p.rot + at, p.cos_dtype);
-        const float s = table_at(p.cos_sin, pos * p.rot + e + at, p.cos_dtype);
+        const float c = table_at(p.cos_sin, row + at, p.cos_dtype);
+        const float s = table_at(p.cos_sin, row + e + at, p.cos_dtype);
         z[j] = z[j] * c + DT::to_f32(x[other]) * (first ? -s : s);
       }
     }
     put2<DT>(r, i, z[0], z[1]);
+    __builtin_amdgcn_sched_barrier(0);   // a pair at a time: the rare form must not set the kernel's registers
   }
   return r;
+}
+
+// 8 pairs (x, y) held as packed 16-bit values turned by their angles
+template <typename DT>
+__device__ inline void rotate8(u32x4& x, u32x4& y, const u32x4 c, const u32x4 s) {
+  auto lo = [](uint32_t w) { return DT::to_f32((uint16_t)w); };
+  auto hi = [](uint32_t w) { return DT::to_f32((uint16_t)(w >> 16)); };
+#pragma unroll
+  for (int e = 0; e < 4; e++) {
+    const float x0 = lo(x[e]), x1 = hi(x[e]), y0 = lo(y[e]), y1 = hi(y[e]), c0 = lo(c[e]), c1 = hi(c[e]), s0 = lo(s[e]), s1 = hi(s[e]);
+    x[e] = pack2<DT>(x0 * c0 - y0 * s0, x1 * c1 - y1 * s1);
+    y[e] = pack2<DT>(y0 * c0 + x0 * s0, y1 * c1 + x1 * s1);
+  }
 }
 
 // largest magnitude of 16 elements as the low 15 bits of the 16-bit type: ordered like the values, infinities and NaN on top
@@ -210,25 +228,45 @@ __device__ inline float scale_of(uint32_t bits, float qmax) {
   return bits >= inf ? __builtin_nanf("") : DT::to_f32((uint16_t)bits) * (1.0f / qmax);
 }
 
+// four quotients as codes.  int8: 1.5 * 2^23 + x holds x, rounded to the nearest integer (ties to even), in its low bits
 template <bool INT8>
 __device__ inline uint32_t encode4(float a, float b, float c, float d) {
   if constexpr (INT8) {
-    auto code = [](float v) { return (uint32_t)(int)rintf(v) & 0xffu; };
-    return code(a) | (code(b) << 8) | (code(c) << 16) | (code(d) << 24);
+    auto bits = [](float v) { return __float_as_uint(v + 12582912.0f); };
+    const uint32_t lo = __builtin_amdgcn_perm(bits(b), bits(a), 0x0c0c0400u), hi = __builtin_amdgcn_perm(bits(d), bits(c), 0x04000c0cu);
+    return lo | hi;
   } else {
     auto cut = [](float v) { return __builtin_fminf(__builtin_fmaxf(v, -448.0f), 448.0f); };
     const int r = __builtin_amdgcn_cvt_pk_fp8_f32(cut(a), cut(b), 0, false);
     return (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(cut(c), cut(d), r, true);
   }
 }
+
+// Division by a block's scale: with the reciprocal y of s, q = x y and q + (x - q s) y (both fused) is the correctly rounded
+// quotient (Markstein 1990; for the one mantissa of all ones it may be a neighbour), three instructions instead of a
+// dozen.  x and s are brought to the middle of the range first, by a power of two: 1 / s is finite, nothing underflows.
+struct Divisor {
+  float s, y, up;
+  __device__ inline explicit Divisor(float scale) {
+    up = scale < 0x1p-60f ? 0x1p90f : scale > 0x1p60f ? 0x1p-64f : 1.f;
+    s = scale * up;
+    y = scale > 0.f ? 1.f / s : 0.f;   // (0: every value is 0; NaN: a value was not finite; the codes are 0 in both)
+  }
+  __device__ inline float quotient(float x) const {
+    x *= up;
+    const float q = x * y;
+    return __builtin_fmaf(__builtin_fmaf(-q, s, x), y, q);
+  }
+};
 template <typename DT, bool INT8>
-__device__ inline u32x4 encode16(const Row16& x, float scale) {
+__device__ inline u32x4 encode16(const Row16& x, const Divisor& d) {
   u32x4 r = {0, 0, 0, 0};
-  if (!(scale > 0.f)) return r;   // an empty block (every value 0), or one whose scale is NaN
+  if (d.y != 0.f) {
 #pragma unroll
-  for (int i = 0; i < 4; i++)
-    r[i] = encode4<INT8>(elem<DT>(x, 4 * i) / scale, elem<DT>(x, 4 * i + 1) / scale, elem<DT>(x, 4 * i + 2) / scale,
-                         elem<DT>(x, 4 * i + 3) / scale);
+    for (int i = 0; i < 4; i++)
+      r[i] = encode4<INT8>(d.quotient(elem<DT>(x, 4 * i)), d.quotient(elem<DT>(x, 4 * i + 1)), d.quotient(elem<DT>(x, 4 * i + 2)),
+                           d.quotient(elem<DT>(x, 4 * i + 3)));
+  }
   return r;
 }
 template <bool INT8>
@@ -259,13 +297,19 @@ __device__ inline u32x4 byte_mask(uint32_t m) {
 }
 
 // One wave appends tokens t + i of one kv head for the bits i of `here`, all in block `blk`; lane i holds token t + i's
-// offset there.  A token takes HEAD / 16 lanes of 16 elements, 64 / (HEAD / 16) tokens a pass; the first two passes stay in
-// registers between the search for the largest magnitude and the encoding (a 16-token block of 128-wide heads is two),
-// later ones are read again.  K codes go out as the cache's own 16-byte pieces; V codes are turned in LDS, so that the
-// cache takes 16 tokens of a head dim at once.
-template <typename DT, bool INT8, int HEAD>
-__device__ inline void append_run(const AppendParams& p, int t, uint64_t here, int blk, int offset, int h, unsigned char* stage, int lane) {
-  constexpr int LPT = HEAD / 16, TPP = 64 / LPT, HELD = 2;
+// offset there and its row of the angles' table.  A token takes HEAD / 16 lanes of 16 elements, 64 / (HEAD / 16) tokens a pass;
+// the first two passes stay in registers between the search for the largest magnitude and the encoding (a 16-token block
+// of 128-wide heads is two), later ones are read again.  K codes go out as the cache's own 16-byte pieces; V codes are
+// turned in LDS, so that the cache takes 16 tokens of a head dim at once.  What the block held (needed where the scale
+// grows, and around the new tokens of V) is requested together with the new rows: a decode step is three round trips.
+// FORM_WHOLE: NeoX pairing over the whole head, 16-bit angles of the model's type, aligned rows; FORM_NONE: no rotation, aligned
+// rows -- nearly every call, in kernels that the general form's code (60 KB) does not weigh on: 47 -> 35 us for 8192 prompt
+// tokens of 32 + 8 heads, 8.1 -> 6.7 us for one token.  Under FORM_WHOLE a lane holds 8 elements of K and their 8 partners.
+enum { FORM_ANY = 0, FORM_WHOLE = 1, FORM_NONE = 2 };
+template <typename DT, bool INT8, int HEAD, int FORM>
+__device__ __forceinline__ void append_run(const AppendParams& p, int t, uint64_t here, int blk, int offset, int pos, int h,
+                                           unsigned char* stage, int lane) {
+  constexpr int LPT = HEAD / 16, TPP = 64 / LPT, HELD = 2, OLD = 2;
   constexpr float QMAX = INT8 ? 127.0f : 448.0f;
   const int chunk = lane % LPT, sub = lane / LPT, d0 = chunk * 16;
   const bool turns = (p.rot_mode == ROT_HALVES || p.rot_mode == ROT_PAIRS) && d0 < p.rot;
@@ -290,58 +334,101 @@ __device__ inline void append_run(const AppendParams& p, int t, uint64_t here, i
     }
     first = __builtin_ctzll(taken);
   }
+  const uint64_t stand = ~__ballot(dead);
+
+  const int passes = (n + TPP - 1) / TPP, per_row = p.bs >> 4;
+  float* const ks = p.ks + blk * p.scale_block_stride + h * p.scale_head_stride;
+  float* const vs = p.vs + blk * p.scale_block_stride + h * p.scale_head_stride;
+  unsigned char* const kb = p.kc + blk * p.block_stride + (int64_t)h * HEAD * p.bs;
+  unsigned char* const vb = p.vc + blk * p.block_stride + (int64_t)h * HEAD * p.bs;
 
   auto load = [&](int i, Row16& k, Row16& v) {
-    const int64_t row = t + min(i, n - 1);
+    const int j = min(i, n - 1);
+    const int64_t row = t + j;
     const uint16_t* kr = p.k + row * p.k_stride + (int64_t)h * HEAD;
-    v = load16(p.v + row * p.v_stride + (int64_t)h * HEAD + d0, p.aligned);
-    if (p.rot_mode == ROT_ANY) {
-      k = rotate16_any<DT>(kr, d0, p, p.positions[row]);
+    const int at = __shfl(pos, j, 64);
+    v = load16(p.v + row * p.v_stride + (int64_t)h * HEAD + d0, FORM != FORM_ANY || p.aligned);
+    if constexpr (FORM == FORM_NONE) {
+      k = load16(kr + d0, true);
+    } else if constexpr (FORM == FORM_WHOLE) {
+      const uint16_t* angle = reinterpret_cast<const uint16_t*>(p.cos_sin) + (int64_t)at * HEAD + 8 * chunk;
+      k.a = *reinterpret_cast<const u32x4*>(kr + 8 * chunk);
+      k.b = *reinterpret_cast<const u32x4*>(kr + HEAD / 2 + 8 * chunk);
+      rotate8<DT>(k.a, k.b, *reinterpret_cast<const u32x4*>(angle), *reinterpret_cast<const u32x4*>(angle + HEAD / 2));
+    } else if (p.rot_mode == ROT_ANY) {
+      k = rotate16_any<DT>(kr, d0, p, at);
     } else {
       k = load16(kr + d0, p.aligned);
       if (turns) {
         Angles a;
-        load_angles(a, p, p.positions[row], d0);
+        load_angles(a, p, at, d0);
         const Row16 other = halves ? load16(kr + d0 + partner, p.aligned) : k;
         k = rotate16<DT>(k, other, a, halves, first_half);
       }
     }
   };
-  const int passes = (n + TPP - 1) / TPP;
-  float* const ks = p.ks + blk * p.scale_block_stride + h * p.scale_head_stride;
-  float* const vs = p.vs + blk * p.scale_block_stride + h * p.scale_head_stride;
-  const float ks_old = first > 0 ? *ks : 0.f, vs_old = first > 0 ? *vs : 0.f;
+  auto stands = [&](int i) { return i < 64 && ((stand >> i) & 1); };
+
+  // what the block holds, the first OLD pieces of a lane; the scales it is held under
+  u32x4 k_old[OLD], v_old[OLD];
+  float ks_old = 0.f, vs_old = 0.f;
+  auto kept = [&](int i) { return i < LPT * p.bs && i % p.bs < first; };                        // a K piece of an earlier token
+  auto touched = [&](int i, uint32_t& fresh, int& before) {                                      // a V piece with new or earlier tokens
+    const int g = i % per_row;
+    fresh = (uint32_t)(taken >> (16 * g)) & 0xffffu;
+    before = min(max(first - 16 * g, 0), 16);
+    return i < HEAD * per_row;
+  };
+  if (first > 0) {
+    ks_old = *ks;
+    vs_old = *vs;
+#pragma unroll
+    for (int j = 0; j < OLD; j++)
+      if (kept(lane + 64 * j)) k_old[j] = reinterpret_cast<const u32x4*>(kb)[lane + 64 * j];
+  }
+#pragma unroll
+  for (int j = 0; j < OLD; j++) {
+    uint32_t fresh;
+    int before;
+    if (touched(lane + 64 * j, fresh, before) && fresh != 0xffffu && (fresh || before)) v_old[j] = reinterpret_cast<const u32x4*>(vb)[lane + 64 * j];
+  }
+
   Row16 k[HELD], v[HELD];
   uint32_t ktop = 0, vtop = 0;
-#pragma unroll
-  for (int s = 0; s < HELD; s++)
-    if (s < passes) load(s * TPP + sub, k[s], v[s]);
-  auto stands = [&](int i) { return __shfl((int)dead, min(i, 63), 64) == 0 && i < n; };
-#pragma unroll
-  for (int s = 0; s < HELD; s++)
-    if (s < passes && stands(s * TPP + sub)) {
-      ktop = max(ktop, top_bits(k[s]));
-      vtop = max(vtop, top_bits(v[s]));
-    }
-  for (int s = HELD; s < passes; s++) {
-    Row16 a, b;
-    load(s * TPP + sub, a, b);
-    if (stands(s * TPP + sub)) {
+  auto consider = [&](int i, const Row16& a, const Row16& b) {
+    if (stands(i)) {
       ktop = max(ktop, top_bits(a));
       vtop = max(vtop, top_bits(b));
     }
+  };
+#pragma unroll
+  for (int s = 0; s < HELD; s++)
+    if (s < passes) load(s * TPP + sub, k[s], v[s]);
+#pragma unroll
+  for (int s = 0; s < HELD; s++)
+    if (s < passes) consider(s * TPP + sub, k[s], v[s]);
+  for (int s = HELD; s < passes; s++) {
+    Row16 a, b;
+    load(s * TPP + sub, a, b);
+    consider(s * TPP + sub, a, b);
   }
   const float kn = scale_of<DT>(wave_umax(ktop), QMAX), vn = scale_of<DT>(wave_umax(vtop), QMAX);
   const float ks_new = kn > ks_old || kn != kn ? kn : ks_old, vs_new = vn > vs_old || vn != vn ? vn : vs_old;
   const bool kgrow = ks_new > ks_old, vgrow = vs_new > vs_old;
+  const Divisor kdiv(ks_new), vdiv(vs_new);
 
-  unsigned char* const kb = p.kc + blk * p.block_stride + (int64_t)h * HEAD * p.bs;
-  unsigned char* const vb = p.vc + blk * p.block_stride + (int64_t)h * HEAD * p.bs;
   auto put = [&](int i, const Row16& a, const Row16& b) {
     const int o = __shfl(offset, min(i, 63), 64);
     if (!stands(i)) return;
-    *reinterpret_cast<u32x4*>(kb + (chunk * p.bs + o) * 16) = encode16<DT, INT8>(a, ks_new);
-    const u32x4 c = encode16<DT, INT8>(b, vs_new);
+    const u32x4 kk = encode16<DT, INT8>(a, kdiv);
+    if constexpr (FORM == FORM_WHOLE) {
+      unsigned char* to = kb + ((chunk >> 1) * p.bs + o) * 16 + 8 * (chunk & 1);
+      *reinterpret_cast<u32x2*>(to) = u32x2{kk[0], kk[1]};
+      *reinterpret_cast<u32x2*>(to + LPT / 2 * p.bs * 16) = u32x2{kk[2], kk[3]};
+    } else {
+      *reinterpret_cast<u32x4*>(kb + (chunk * p.bs + o) * 16) = kk;
+    }
+    const u32x4 c = encode16<DT, INT8>(b, vdiv);
 #pragma unroll
     for (int j = 0; j < 16; j++) stage[(d0 + j) * p.bs + o] = (unsigned char)(c[j >> 2] >> (8 * (j & 3)));
   };
@@ -357,33 +444,35 @@ __device__ inline void append_run(const AppendParams& p, int t, uint64_t here, i
   // earlier tokens of the block under a larger scale
   if (kgrow && first > 0) {
     const float ratio = ks_old / ks_new;
-    for (int i = lane; i < LPT * p.bs; i += 64) {
-      if (i % p.bs >= first) continue;
+#pragma unroll
+    for (int j = 0; j < OLD; j++)
+      if (kept(lane + 64 * j)) reinterpret_cast<u32x4*>(kb)[lane + 64 * j] = rescale16<INT8>(k_old[j], ratio);
+    for (int i = lane + 64 * OLD; i < LPT * p.bs; i += 64) {
       u32x4* at = reinterpret_cast<u32x4*>(kb) + i;
-      *at = rescale16<INT8>(*at, ratio);
+      if (kept(i)) *at = rescale16<INT8>(*at, ratio);
     }
   }
   const float ratio = vgrow && first > 0 ? vs_old / vs_new : 1.f;
   asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");   // the wave's LDS writes are in place for its other lanes
-  const int per_row = p.bs >> 4;
-  for (int i = lane; i < HEAD * per_row; i += 64) {
-    const int g = i % per_row;
-    const uint32_t fresh = (uint32_t)(taken >> (16 * g)) & 0xffffu;
-    const int before = min(max(first - 16 * g, 0), 16);
-    const bool again = vgrow && before > 0;
-    if (!fresh && !again) continue;
-    u32x4* at = reinterpret_cast<u32x4*>(vb) + i;
+  auto merge = [&](int i, u32x4 old, uint32_t fresh, int before) {
     const u32x4 staged = reinterpret_cast<const u32x4*>(stage)[i];
     u32x4 r = staged;
     if (fresh != 0xffffu) {
-      const u32x4 old = *at;
+      const bool again = vgrow && before > 0;
       const u32x4 keep = again ? byte_mask((1u << before) - 1) : u32x4{0, 0, 0, 0}, mine = byte_mask(fresh);
       const u32x4 less = again ? rescale16<INT8>(old, ratio) : old;
 #pragma unroll
       for (int j = 0; j < 4; j++) r[j] = (staged[j] & mine[j]) | (less[j] & keep[j] & ~mine[j]) | (old[j] & ~keep[j] & ~mine[j]);
     }
-    *at = r;
-  }
+    reinterpret_cast<u32x4*>(vb)[i] = r;
+  };
+  uint32_t fresh;
+  int before;
+#pragma unroll
+  for (int j = 0; j < OLD; j++)
+    if (touched(lane + 64 * j, fresh, before) && (fresh || (vgrow && before > 0))) merge(lane + 64 * j, v_old[j], fresh, before);
+  for (int i = lane + 64 * OLD; touched(i, fresh, before); i += 64)
+    if (fresh || (vgrow && before > 0)) merge(i, fresh != 0xffffu ? reinterpret_cast<const u32x4*>(vb)[i] : u32x4{0, 0, 0, 0}, fresh, before);
   if (lane == 0) {
     *ks = ks_new;
     *vs = vs_new;
@@ -391,41 +480,89 @@ __device__ inline void append_run(const AppendParams& p, int t, uint64_t here, i
   asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
 }
 
-template <typename DT, bool INT8, int HEAD>
-__global__ __launch_bounds__(256) void rope_and_cache_blocks_kernel(const AppendParams p) {
+// The query of one token by one wave, 64 / (HEAD / 16) heads a pass: the general form, 16 elements of a head per lane.
+template <typename DT, int HEAD>
+__device__ inline void rotate_query(const AppendParams& p, int t, int lane) {
   constexpr int LPT = HEAD / 16, TPP = 64 / LPT;
+  const int chunk = lane % LPT, sub = lane / LPT, d0 = chunk * 16;
+  const bool turns = (p.rot_mode == ROT_HALVES || p.rot_mode == ROT_PAIRS) && d0 < p.rot;
+  const bool halves = p.rot_mode == ROT_HALVES, first_half = d0 < p.rot / 2;
+  const int partner = turns && halves ? (first_half ? p.rot / 2 : -(p.rot / 2)) : 0;
+  const uint16_t* q = p.q + (int64_t)t * p.q_stride;
+  uint16_t* out = p.q_out + (int64_t)t * p.q_out_stride;
+  const int pos = p.rot_mode == ROT_NONE ? 0 : position(p, t);
+  Angles a;
+  if (turns) load_angles(a, p, pos, d0);
+  for (int h0 = 0; h0 < p.num_heads; h0 += TPP) {
+    const int h = min(h0 + sub, p.num_heads - 1);
+    const uint16_t* x = q + (int64_t)h * HEAD;
+    Row16 r;
+    if (p.rot_mode == ROT_ANY) {
+      r = rotate16_any<DT>(x, d0, p, pos);
+    } else {
+      r = load16(x + d0, p.aligned);
+      if (turns) {
+        const Row16 other = halves ? load16(x + d0 + partner, p.aligned) : r;
+        r = rotate16<DT>(r, other, a, halves, first_half);
+      }
+    }
+    // (in place, a lane's partner has been read by now: the store needs what the same instructions loaded)
+    if (h0 + sub < p.num_heads) store16(out + (int64_t)h * HEAD + d0, r, p.aligned);
+  }
+}
+
+template <int HEAD>
+__device__ inline void copy_query(const AppendParams& p, int t, int lane) {
+  const u32x4* q = reinterpret_cast<const u32x4*>(p.q + (int64_t)t * p.q_stride);
+  u32x4* out = reinterpret_cast<u32x4*>(p.q_out + (int64_t)t * p.q_out_stride);
+  for (int i = lane; i < p.num_heads * (HEAD / 8); i += 64) out[i] = q[i];
+}
+
+// The same for FORM_WHOLE: nothing is read twice, and four passes (32 heads of 128) are requested before the first is turned: the
+// loop is bound by HBM, not by its round trips.
+template <typename DT, int HEAD>
+__device__ inline void rotate_query_whole(const AppendParams& p, int t, int lane) {
+  constexpr int LPT = HEAD / 16, TPP = 64 / LPT, DEEP = 4, E = HEAD / 2;
+  const int i0 = lane % LPT * 8, sub = lane / LPT;
+  const uint16_t* q = p.q + (int64_t)t * p.q_stride + i0;
+  uint16_t* out = p.q_out + (int64_t)t * p.q_out_stride + i0;
+  const uint16_t* angle = reinterpret_cast<const uint16_t*>(p.cos_sin) + (int64_t)position(p, t) * HEAD + i0;
+  u32x4 x[DEEP], y[DEEP], c, s;
+  for (int h0 = 0; h0 < p.num_heads; h0 += DEEP * TPP) {
+#pragma unroll
+    for (int j = 0; j < DEEP; j++) {
+      const int64_t at = (int64_t)min(h0 + j * TPP + sub, p.num_heads - 1) * HEAD;
+      x[j] = *reinterpret_cast<const u32x4*>(q + at);
+      y[j] = *reinterpret_cast<const u32x4*>(q + at + E);
+    }
+    if (h0 == 0) {
+      c = *reinterpret_cast<const u32x4*>(angle);
+      s = *reinterpret_cast<const u32x4*>(angle + E);
+    }
+#pragma unroll
+    for (int j = 0; j < DEEP; j++) {
+      const int h = h0 + j * TPP + sub;
+      rotate8<DT>(x[j], y[j], c, s);
+      if (h < p.num_heads) {
+        *reinterpret_cast<u32x4*>(out + (int64_t)h * HEAD) = x[j];
+        *reinterpret_cast<u32x4*>(out + (int64_t)h * HEAD + E) = y[j];
+      }
+    }
+  }
+}
+
+template <typename DT, bool INT8, int HEAD, int FORM>
+__global__ __launch_bounds__(256, FORM == FORM_ANY ? 2 : 3) void rope_and_cache_blocks_kernel(const AppendParams p) {
   extern __shared__ __attribute__((aligned(16))) unsigned char stage[];   // [4 waves][HEAD][block size]
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
 
   if ((int)blockIdx.x >= p.kv_groups) {
-    // ---- the query: one wave per token, TPP heads a pass -------------------------------------------------------------
     const int t = ((int)blockIdx.x - p.kv_groups) * 4 + wave;
-    if (t >= p.num_tokens) return;
-    const int chunk = lane % LPT, sub = lane / LPT, d0 = chunk * 16;
-    const bool turns = (p.rot_mode == ROT_HALVES || p.rot_mode == ROT_PAIRS) && d0 < p.rot;
-    const bool halves = p.rot_mode == ROT_HALVES, first_half = d0 < p.rot / 2;
-    const int partner = turns && halves ? (first_half ? p.rot / 2 : -(p.rot / 2)) : 0;
-    const uint16_t* q = p.q + (int64_t)t * p.q_stride;
-    uint16_t* out = p.q_out + (int64_t)t * p.q_out_stride;
-    const int64_t pos = p.rot_mode == ROT_NONE ? 0 : p.positions[t];
-    Angles a;
-    if (turns) load_angles(a, p, pos, d0);
-    for (int h0 = 0; h0 < p.num_heads; h0 += TPP) {
-      const int h = min(h0 + sub, p.num_heads - 1);
-      const uint16_t* x = q + (int64_t)h * HEAD;
-      Row16 r;
-      if (p.rot_mode == ROT_ANY) {
-        r = rotate16_any<DT>(x, d0, p, pos);
-      } else {
-        r = load16(x + d0, p.aligned);
-        if (turns) {
-          const Row16 other = halves ? load16(x + d0 + partner, p.aligned) : r;
-          r = rotate16<DT>(r, other, a, halves, first_half);
-        }
-      }
-      // (in place, a lane's partner has been read by now: the store needs what the same instructions loaded)
-      if (h0 + sub < p.num_heads) store16(out + (int64_t)h * HEAD + d0, r, p.aligned);
+    if (t < p.num_tokens) {
+      if constexpr (FORM == FORM_WHOLE) rotate_query_whole<DT, HEAD>(p, t, lane);
+      else if constexpr (FORM == FORM_NONE) copy_query<HEAD>(p, t, lane);
+      else rotate_query<DT, HEAD>(p, t, lane);
     }
     return;
   }
@@ -476,24 +613,36 @@ __global__ __launch_bounds__(256) void rope_and_cache_blocks_kernel(const Append
     }
     return -1;
   };
+  // Lane i looks at token t0 - 1 + i: whether a run begins at one of the wave's positions, and (all but always) the whole of it.
   int slot;
-  const int blk = lane < p.tokens_per_wave ? block_at(t0 + lane, slot) : -1;
-  const int blk_before = lane < p.tokens_per_wave ? block_at(t0 + lane - 1, slot) : -1;
-  uint64_t heads = __ballot(blk >= 0 && blk != blk_before);
+  const int tl = t0 - 1 + lane, blk = block_at(tl, slot);
+  const bool rotates = FORM == FORM_WHOLE || (FORM == FORM_ANY && p.rot_mode != ROT_NONE);
+  const int pos = rotates && tl >= 0 && tl < p.num_tokens ? position(p, tl) : 0;
+  const int before = __shfl_up(blk, 1, 64);
+  uint64_t heads = __ballot(lane > 0 && lane <= p.tokens_per_wave && blk >= 0 && blk != before);
   while (heads) {
     const int i = __builtin_ctzll(heads);
     heads &= heads - 1;
     const int b = __builtin_amdgcn_readlane(blk, i);
-    int t = t0 + i;
-    if (t > 0 && __builtin_amdgcn_readlane(blk_before, i) < 0 && block_before(t) == b) continue;   // a run goes on behind a gap
-    // a run of more than 64 positions is appended in stretches, one after the other
+    int t = t0 - 1 + i;
+    if (t > 0 && __builtin_amdgcn_readlane(before, i) < 0 && block_before(t) == b) continue;   // a run goes on behind a gap
+    // the run, a token per lane; one that does not end in sight is looked up again, 64 positions (at most) a stretch
+    const uint64_t others = __ballot(lane > i && blk >= 0 && blk != b);
+    bool in_sight = others || t0 + 63 >= p.num_tokens;
     for (;;) {
-      int s;
-      const int bt = block_at(t + lane, s);
-      const uint64_t others = __ballot(bt >= 0 && bt != b);
-      const uint64_t here = __ballot(bt == b) & (others ? (1ull << __builtin_ctzll(others)) - 1 : ~0ull);
-      append_run<DT, INT8, HEAD>(p, t, here, b, s - b * p.bs, h, stage + wave * HEAD * p.bs, lane);
-      if (others || t + 64 >= p.num_tokens) break;
+      int s, ps, bt;
+      if (in_sight) {
+        const int from = min(lane + i, 63);
+        s = __shfl(slot, from, 64), ps = __shfl(pos, from, 64), bt = __shfl(blk, from, 64);
+        if (lane + i > 63) bt = -1;
+      } else {
+        bt = block_at(t + lane, s);
+        ps = rotates && t + lane < p.num_tokens ? position(p, t + lane) : 0;
+      }
+      const uint64_t end = __ballot(bt >= 0 && bt != b);
+      const uint64_t here = __ballot(bt == b) & (end ? (1ull << __builtin_ctzll(end)) - 1 : ~0ull);
+      append_run<DT, INT8, HEAD, FORM>(p, t, here, b, s - b * p.bs, ps, h, stage + wave * HEAD * p.bs, lane);
+      if (in_sight || end || t + 64 >= p.num_tokens) break;
       int bn;
       t = next_token(t + 64, bn);
       if (bn != b) break;
@@ -566,11 +715,19 @@ extern "C" int mi355q_rope_and_cache_blocks(const int64_t* positions, const void
   hipStream_t s = (hipStream_t)stream;
   const dim3 grid(p.kv_groups + q_groups), wg(256);
   const bool i8 = code_type == MI355Q_KV_INT8;
-#define LAUNCH(DT, I8, HD) hipLaunchKernelGGL((rope_and_cache_blocks_kernel<DT, I8, HD>), grid, wg, lds, s, p)
-#define BY_HEAD(DT, I8)                       \
-  do {                                        \
-    if (head_size == 128) LAUNCH(DT, I8, 128); \
-    else LAUNCH(DT, I8, 64);                  \
+  const bool whole = p.rot_mode == ROT_HALVES && rot_dim == head_size && p.aligned && cos_dtype == dtype;
+  const bool none = p.rot_mode == ROT_NONE && p.aligned;
+#define LAUNCH(DT, I8, HD, FM) hipLaunchKernelGGL((rope_and_cache_blocks_kernel<DT, I8, HD, FM>), grid, wg, lds, s, p)
+#define BY_FORM(DT, I8, HD)                      \
+  do {                                           \
+    if (whole) LAUNCH(DT, I8, HD, FORM_WHOLE);   \
+    else if (none) LAUNCH(DT, I8, HD, FORM_NONE); \
+    else LAUNCH(DT, I8, HD, FORM_ANY);           \
+  } while (0)
+#define BY_HEAD(DT, I8)                          \
+  do {                                           \
+    if (head_size == 128) BY_FORM(DT, I8, 128);  \
+    else BY_FORM(DT, I8, 64);                    \
   } while (0)
   if (dtype == MI355Q_BF16) {
     if (i8) BY_HEAD(BF16, true);
@@ -580,6 +737,7 @@ extern "C" int mi355q_rope_and_cache_blocks(const int64_t* positions, const void
     else BY_HEAD(FP16, false);
   }
 #undef BY_HEAD
+#undef BY_FORM
 #undef LAUNCH
   return check_launch("rope_and_cache_blocks_kernel");
 }

@@ -119,8 +119,8 @@ __device__ inline u32x4 widen8(u32x4 w, int h) {
 
 
 typedef __attribute__((ext_vector_type(2))) _Float16 cvt_f16x2;
-template <typename MT> __device__ inline uint32_t wpack(float lo, float hi) { return pack2<MT>(lo, hi); }
-template <> __device__ inline uint32_t wpack<FP16>(float lo, float hi) { return __builtin_bit_cast(uint32_t, __builtin_convertvector(f32x2{lo, hi}, cvt_f16x2)); }
+template <typename MT> __device__ inline uint32_t pack_p(float lo, float hi) { return pack2<MT>(lo, hi); }
+template <> __device__ inline uint32_t pack_p<FP16>(float lo, float hi) { return __builtin_bit_cast(uint32_t, __builtin_convertvector(f32x2{lo, hi}, cvt_f16x2)); }
 // max over the four lanes that share a column
 __device__ inline float group_max(float v) {
   auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
@@ -1019,7 +1019,7 @@ __global__ __launch_bounds__(64 * NW, HEAD == 64 ? 4 : 2) void window_flash_kern
     for (int j = 0; j < 4; j++)
 #pragma unroll
       for (int e = 0; e < 4; e++) {
-        pf[j][e] = wpack<MT>(s[j >> 1][8 * (j & 1) + 2 * e], s[j >> 1][8 * (j & 1) + 2 * e + 1]);
+        pf[j][e] = pack_p<MT>(s[j >> 1][8 * (j & 1) + 2 * e], s[j >> 1][8 * (j & 1) + 2 * e + 1]);
         l = add_pair<MT>(pf[j][e], l);
       }
 
@@ -1156,6 +1156,7 @@ __global__ __launch_bounds__(256) void window_merge_kernel(const WindowParams p,
 struct WindowPart { int cols, waves, col_tiles, splits, split_tiles; };
 struct WindowPlan {
   WindowPart rows, flash;       // col_tiles 0: not launched
+  bool all_flash;               // sequences of few rows too
   int part_stride;
 };
 
@@ -1182,8 +1183,12 @@ static WindowPlan window_plan(int num_seqs, int num_rows, int num_heads, int num
   const int G = num_heads / num_kv_heads;
   const int64_t cols = (int64_t)max_query_len * G;
   const bool prompts = cols > WA_ROWS_COLS;
-  // a batch whose sequences all have max_query_len rows needs one kind only
-  if (!prompts || (int64_t)num_seqs * max_query_len != num_rows) {
+  const int64_t flash_tiles = window_tiles(WA_FLASH_COLS, G, max_seq_len, window, sinks);
+  // Decode rows between prompts go to the rows kernel, unless no context is longer than 32 tiles: a workgroup of the prompt
+  // kernel then walks it while the prompts' own run, which costs less than a launch (57 -> 47 us for five sequences under a
+  // window of 512), or the bounds say that every sequence has max_query_len rows.
+  w.all_flash = prompts && (flash_tiles <= 32 || (int64_t)num_seqs * max_query_len == num_rows);
+  if (!w.all_flash) {
     const int64_t mine = std::min<int64_t>(cols, WA_ROWS_COLS);
     // 32 columns to a workgroup read a draft's K and V once instead of twice; a 16-bit tile leaves no registers for it
     w.rows.cols = mine > 16 && kv_type != MI355Q_KV_16 ? 32 : 16;
@@ -1198,7 +1203,7 @@ static WindowPlan window_plan(int num_seqs, int num_rows, int num_heads, int num
     w.flash.waves = WA_WAVES;
     w.flash.col_tiles = (int)((cols + WA_FLASH_COLS - 1) / WA_FLASH_COLS);
     const int64_t groups = (int64_t)num_seqs * num_kv_heads * w.flash.col_tiles;
-    window_cut(w.flash, window_tiles(WA_FLASH_COLS, G, max_seq_len, window, sinks), std::max<int64_t>(1, (256 + groups - 1) / groups), 16);
+    window_cut(w.flash, flash_tiles, std::max<int64_t>(1, (256 + groups - 1) / groups), 16);
   }
   w.part_stride = std::max(w.rows.splits, w.flash.splits);
   return w;
@@ -1220,7 +1225,7 @@ static int launch_window(WindowParams p, const WindowPlan& w, hipStream_t s) {
     if (!a.col_tiles) continue;
     p.col_tiles = a.col_tiles, p.splits = a.splits;
     p.split_tiles = a.splits == 1 ? INT_MAX : a.split_tiles;
-    p.min_cols = kind ? WA_ROWS_COLS + 1 : 0;
+    p.min_cols = kind && !w.all_flash ? WA_ROWS_COLS + 1 : 0;
     p.max_cols = kind ? INT_MAX : WA_ROWS_COLS;
     p.lds_cols = std::min(16, p.longest_cols);
     const dim3 grid((unsigned)groups(a)), wg(64 * a.waves);
