@@ -41,7 +41,7 @@ def parse():
     ap.add_argument("--model", default=None, help="llama3-8b | llama3-70b | mixtral-8x7b | tiny | small ... (default: by --gpus)")
     ap.add_argument("--skip-configs", action="store_true", help="skip the other benchmark configurations (AWQ + fp8 KV, Mixtral)")
     ap.add_argument("--quant", default="gptq", choices=["gptq", "awq", "none"])
-    ap.add_argument("--kv-dtype", default="auto", choices=["auto", "fp8"])
+    ap.add_argument("--kv-dtype", default="auto", choices=["auto", "fp8", "block_int8", "block_fp8"])
     ap.add_argument("--no-graph", action="store_true")
     ap.add_argument("--roofline-only", action="store_true", help="run only the dominant-kernel timing pass")
     ap.add_argument("--skip-cpu", action="store_true")
@@ -424,7 +424,7 @@ def main():
     last_ids = runner.tokens.cpu().tolist()
 
     ctx_mid = in_len + args.warmup + args.steps // 2
-    kv_bytes = 1 if args.kv_dtype == "fp8" else 2
+    kv_bytes = 2 if args.kv_dtype == "auto" else 1
     if args.quant == "none":
         from mi355q.model import linear_shapes
         step_bytes = sum(K * N * 2 for K, N in linear_shapes(cfg, world).values()) * cfg.layers + \
@@ -438,7 +438,7 @@ def main():
         "ms_per_step": step_s * 1e3, "higher_is_better": True, "scaling": "strong" if n_gpus > 1 else "weak",
         "vs_baseline": None, "dtype": "int4 weights x bf16 activations, fp32 accumulate", "data": "synthetic",
         "config": {"workload": "%s %s-int4 g128 decode, TP=%d, batch %d, prompt %d, %s KV, %s" % (
-            model, args.quant, world, B, in_len, "fp8-e4m3" if args.kv_dtype == "fp8" else "bf16",
+            model, args.quant, world, B, in_len, {"auto": "bf16", "fp8": "fp8-e4m3"}.get(args.kv_dtype, args.kv_dtype),
             "hipGraph" if graph else "eager"), "parallelism": "tp%d" % world, "batch": B, "input_len": in_len},
         "ttft_ms_p50": ttft,
         "graph": bool(graph),          # false: capture (of the RCCL all-reduce at N > 1) failed or was disabled; eager steps timed

@@ -1,0 +1,127 @@
+"""Refusals and sizing of the block-scaled cache and of windowed attention: host checks only, no kernel is launched."""
+import ctypes
+
+import pytest
+import torch
+
+from mi355q import _lib, ops
+from mi355q.plugin.attention import Attention, Mi355AttentionBackend, Mi355AttentionImpl
+
+_BUFFER = ctypes.create_string_buffer(4096)
+PTR = (ctypes.addressof(_BUFFER) + 63) & ~63   # never read: every call below is refused
+
+APPEND = dict(positions=PTR, query=PTR, query_stride=512, query_out=PTR, query_out_stride=512, key=PTR, key_stride=512, value=PTR,
+              value_stride=512, head_size=128, num_heads=4, num_kv_heads=2, cos_sin=PTR, rot_dim=128, max_position=64, cos_dtype=_lib.BF16,
+              is_neox=1, key_cache=PTR, value_cache=PTR, num_blocks=8, block_size=16, block_stride=2 * 128 * 16, k_scales=PTR,
+              v_scales=PTR, scale_block_stride=2, scale_head_stride=1, slots=PTR, num_tokens=3, dtype=_lib.BF16, code_type=_lib.KV_INT8,
+              stream=None)
+ATTEND = dict(out=PTR, out_stride=512, query=PTR, q_stride=512, key_cache=PTR, value_cache=PTR, kv_block_stride=2 * 128 * 16,
+              kv_head_stride=128 * 16, num_blocks=8, num_rows=3, num_seqs=2, num_heads=4, num_kv_heads=2, head_size=128, scale=0.1,
+              tables=PTR, width=4, seq_lens=PTR, starts=PTR, max_query_len=2, block_size=16, max_seq_len=64, window=0, sinks=0,
+              dtype=_lib.BF16, kv_type=_lib.KV_INT8, k_scale=PTR, v_scale=PTR, scale_block_stride=2, scale_head_stride=1, workspace=None,
+              workspace_bytes=0, stream=None)
+
+
+def refused(fn, args, message, status=_lib.EINVAL, **over):
+    assert set(over) <= set(args)
+    assert fn(*{**args, **over}.values()) == status
+    assert message in _lib.lib().mi355q_last_error().decode()
+
+
+@pytest.mark.parametrize("over,message", [
+    (dict(dtype=_lib.FP32), "dtype"), (dict(code_type=_lib.KV_16), "codes"), (dict(head_size=96), "head_size"),
+    (dict(num_kv_heads=0), "bad sizes"), (dict(num_tokens=-1), "bad sizes"), (dict(key=None), "null"), (dict(k_scales=None), "null"),
+    (dict(slots=None), "null"), (dict(query_out=None), "null"), (dict(block_size=24), "block size"), (dict(block_size=80), "block size"),
+    (dict(num_blocks=1 << 28), "blocks"), (dict(num_blocks=0), "blocks"), (dict(block_stride=128), "block stride"),
+    (dict(block_stride=2 * 128 * 16 + 8), "block stride"), (dict(key_cache=PTR + 8), "aligned"), (dict(rot_dim=130), "rot_dim"),
+    (dict(rot_dim=3), "rot_dim"), (dict(positions=None), "positions"), (dict(max_position=0), "positions"), (dict(cos_dtype=7), "cos/sin"),
+])
+def test_append_refusals(over, message):
+    refused(_lib.lib().mi355q_rope_and_cache_blocks, APPEND, message, **over)
+
+
+def test_nothing_to_append_is_no_error():
+    assert _lib.lib().mi355q_rope_and_cache_blocks(*{**APPEND, "num_tokens": 0}.values()) == _lib.OK
+
+
+@pytest.mark.parametrize("over,message", [
+    (dict(dtype=_lib.FP32), "dtype"), (dict(kv_type=3), "cache type"), (dict(num_rows=-1), "bad sizes"), (dict(tables=None), "null"),
+    (dict(k_scale=None), "k_scale"), (dict(head_size=80), "head_size"), (dict(num_heads=5), "query heads"),
+    (dict(num_heads=34), "query heads"), (dict(block_size=8), "block size"), (dict(block_size=272), "block size"),
+    (dict(num_blocks=0), "block table"), (dict(width=0), "block table"), (dict(width=1 << 27), "block table"),
+    (dict(max_query_len=0), "length"), (dict(max_seq_len=0), "length"), (dict(window=-1), "length"), (dict(sinks=-1), "length"),
+    (dict(starts=None, num_seqs=4), "rows"), (dict(kv_head_stride=64), "strides"), (dict(kv_block_stride=2 * 128 * 16 + 8), "strides"),
+    (dict(query=PTR + 2), "aligned"), (dict(q_stride=516), "aligned"), (dict(out=PTR + 2), "aligned"), (dict(out_stride=513), "aligned"),
+])
+def test_attention_refusals(over, message):
+    refused(_lib.lib().mi355q_paged_window_attention, ATTEND, message, **over)
+
+
+def test_workspace_is_asked_for_and_checked():
+    L = _lib.lib()
+    size = L.mi355q_paged_window_attention_workspace_bytes
+    assert size(32, 32, 32, 8, 128, 1, 4096, 0, 0, _lib.KV_INT8) == 0            # a full batch: nothing to join
+    need = size(1, 1, 32, 8, 128, 1, 1 << 17, 0, 0, _lib.KV_INT8)
+    assert need > 0 and need % (32 * (128 + 2) * 4) == 0
+    assert size(1, 1, 32, 8, 128, 1, 1 << 17, 512, 4, _lib.KV_INT8) == 0         # a window bounds the work
+    assert size(0, 1, 32, 8, 128, 1, 100, 0, 0, 0) == 0
+    long = dict(num_seqs=1, num_rows=1, max_query_len=1, max_seq_len=1 << 17, width=1 << 13)
+    refused(L.mi355q_paged_window_attention, ATTEND, "workspace", _lib.ENOSPACE, **long)
+    refused(L.mi355q_paged_window_attention, ATTEND, "workspace", _lib.ENOSPACE, **long, workspace=PTR, workspace_bytes=16)
+    refused(L.mi355q_paged_window_attention, ATTEND, "16-byte", **long, workspace=PTR + 4, workspace_bytes=1 << 30)
+
+
+def test_nothing_to_attend_is_no_error():
+    f = _lib.lib().mi355q_paged_window_attention
+    assert f(*{**ATTEND, "num_rows": 0}.values()) == _lib.OK and f(*{**ATTEND, "num_seqs": 0}.values()) == _lib.OK
+
+
+def test_ops_refuse_host_tensors():
+    t, i = torch.zeros(2, 128, dtype=torch.bfloat16), torch.zeros(2, dtype=torch.int64)
+    kc, vc, s = torch.zeros(4, 1, 8, 16, 16, dtype=torch.uint8), torch.zeros(4, 1, 128, 16, dtype=torch.uint8), torch.zeros(4, 1)
+    with pytest.raises(RuntimeError, match="no CPU fallback"):
+        ops.rope_and_cache_blocks(i, t, t, t, 128, t, True, kc, vc, s, s, i, "block_int8")
+    with pytest.raises(RuntimeError, match="no CPU fallback"):
+        ops.reshape_and_cache_blocks(t[:, None], t[:, None], kc, vc, s, s, i, "block_fp8")
+    with pytest.raises(RuntimeError, match="no CPU fallback"):
+        ops.paged_window_attention(t[:, None], t[:, None], kc, vc, 1, 0.1, i.int()[:, None], i.int(), None, 1, 1, "block_int8", s, s)
+
+
+def test_attention_layer_arguments():
+    assert Mi355AttentionBackend.supports_sliding_window() and not Mi355AttentionBackend.supports_sink()
+    assert Mi355AttentionBackend.get_kv_scales_shape(10, 8) == (2, 10, 8)
+    impl = Mi355AttentionImpl(8, 128, 0.1, 2, None, 512, "auto", sink_tokens=4)
+    assert impl.windowed and not impl.block_scaled and (impl.sliding_window, impl.sink_tokens) == (512, 4)
+    assert not impl.decode_fused_supported() and impl.fused_rope_kvcache_supported()
+    for form in ("block_int8", "block_fp8"):
+        impl = Mi355AttentionImpl(8, 64, 0.1, 2, kv_cache_dtype=form)
+        assert impl.windowed and impl.block_scaled and impl.sliding_window == 0 and not impl.decode_fused_supported()
+        with pytest.raises(NotImplementedError):
+            impl.forward_decode_fused(None, None, None, None, None, None, None)
+    assert not Mi355AttentionImpl(8, 128, 0.1, 2).windowed
+    with pytest.raises(NotImplementedError, match="sink logits"):
+        Mi355AttentionImpl(8, 128, 0.1, 2, sinks=torch.zeros(8))
+    with pytest.raises(NotImplementedError, match="soft-capping"):
+        Mi355AttentionImpl(8, 128, 0.1, 2, logits_soft_cap=30.0)
+    with pytest.raises(NotImplementedError, match="ALiBi"):
+        Mi355AttentionImpl(8, 128, 0.1, 2, [0.1] * 8, 512)
+    with pytest.raises(NotImplementedError, match="ALiBi"):
+        Mi355AttentionImpl(8, 128, 0.1, 2, [0.1] * 8, None, "block_int8")
+    for bad in (dict(sliding_window=0), dict(sliding_window=-3), dict(sink_tokens=-1)):
+        with pytest.raises(ValueError):
+            Mi355AttentionImpl(8, 128, 0.1, 2, **bad)
+    layer = Attention(8, 128, 0.1, 2, cache_dtype="block_fp8", sliding_window=64)
+    layer.process_weights_after_loading()
+    assert layer.impl.block_scaled and not hasattr(layer, "k_scale") and layer.kv_scales is None
+
+
+def test_registered_operators_have_schemas_and_fakes():
+    from mi355q.plugin.torch_ops import register_torch_ops
+    register_torch_ops()
+    for name, written in (("rope_and_cache_blocks", 5), ("reshape_and_cache_blocks", 4), ("paged_window_attention", 1)):
+        schema = getattr(torch.ops.mi355q, name).default._schema
+        assert sum(a.alias_info is not None and a.alias_info.is_write for a in schema.arguments) == written
+    m = dict(device="meta")
+    t = torch.empty(2, 4, 64, dtype=torch.bfloat16, **m)
+    torch.ops.mi355q.paged_window_attention(t, t, torch.empty(1, **m), torch.empty(1, **m), 1, 0.1, torch.empty(1, **m), torch.empty(1, **m), None, 1,
+                                            1, "auto", None, None, 0, 0)

@@ -667,3 +667,91 @@ def test_generation_over_the_block_scaled_cache(form, window, sinks):
         b.dev = dict(q=b.q.to(DEV), tables=b.tables.to(DEV), ks=c.ks, vs=c.vs)
         filled = [f + n for f, n in zip(filled, new)]
         b.check()
+
+
+@pytest.mark.parametrize("form", FORMS)
+@pytest.mark.parametrize("window,sinks", [(None, 0), (30, 4)])
+def test_attention_layer(form, window, sinks):
+    """plugin.attention.Attention: the cache update and the attention of a prompt, a chunk with a decode row, and a decode step.  The
+    cache is held against a layer of its own making: what it holds is read back and put into the formula."""
+    from mi355q.plugin.attention import Attention, CommonAttentionMetadata, Mi355AttentionBackend, Mi355AttentionMetadataBuilder
+    if window is None and not form.startswith("block"):
+        pytest.skip("the layer without window or block scales is another kernel's")
+    H, KVH, D, bs, n, dtype = 8, 2, 128, 16, 24, torch.bfloat16
+    with torch.device(DEV):
+        layer = Attention(H, D, D ** -0.5, KVH, cache_dtype=form, sliding_window=window, sink_tokens=sinks)
+    if form == "fp8":
+        layer.k_scale.weight_loader(layer.k_scale, torch.tensor(1 / 32))
+        layer.v_scale.weight_loader(layer.v_scale, torch.tensor(1 / 64))
+    layer.process_weights_after_loading()
+    kv = torch.zeros(Mi355AttentionBackend.get_kv_cache_shape(n, bs, KVH, D), dtype=dtype if form == "auto" else torch.uint8, device=DEV)
+    layer.kv_cache = kv
+    if form.startswith("block"):
+        layer.kv_scales = torch.zeros(Mi355AttentionBackend.get_kv_scales_shape(n, KVH), device=DEV)
+    builder = Mi355AttentionMetadataBuilder(bs, DEV)
+    tables = torch.randperm(n, generator=torch.Generator().manual_seed(2))[:16].view(2, 8).to(torch.int32)
+    filled = [0, 0]
+    for step, new in enumerate([(70, 33), (1, 20), (1, 1)]):
+        pos = [[filled[s] + j for j in range(new[s])] for s in range(2)]
+        slots = [int(tables[s, t // bs]) * bs + t % bs for s in range(2) for t in pos[s]]
+        rows = len(slots)
+        g = torch.Generator().manual_seed(step)
+        q, k, v = (torch.randn(rows, h * D, generator=g).to(dtype) for h in (H, KVH, KVH))
+        filled = [f + m for f, m in zip(filled, new)]
+        md = builder.build(0, CommonAttentionMetadata(
+            query_start_loc=torch.tensor([0, new[0], rows], dtype=torch.int32, device=DEV), seq_lens=torch.tensor(filled, dtype=torch.int32, device=DEV),
+            num_actual_tokens=rows, max_query_len=max(new), max_seq_len=max(filled), block_table_tensor=tables.to(DEV),
+            slot_mapping=torch.tensor(slots, device=DEV)))
+        out = layer(q.to(DEV), k.to(DEV), v.to(DEV), md)
+        b = Batch([(filled[s] - new[s], new[s]) for s in range(2)], H, KVH, D, bs, form, dtype, window=window or 0, sinks=sinks)
+        b.q, b.tables, b.blocks = torch.cat([q, q[:1]]).view(-1, H, D), tables, n
+        x = 8 if form == "auto" else 16
+        kc = cpu(kv[0]).view(n, KVH, D // x, bs, x).transpose(2, 3)
+        vc = cpu(kv[1]).view(n, KVH, D, bs).transpose(2, 3)
+        if form == "auto":
+            b.k, b.v = kc.reshape(n, KVH, bs, D).double(), vc.double()
+        else:
+            b.k = kc.reshape(n, KVH, bs, D).contiguous().view(CODE[form]).double()
+            b.v = vc.contiguous().view(CODE[form]).double()
+            ks, vs = (layer._k_scale, layer._v_scale) if form == "fp8" else layer.kv_scales
+            b.k, b.v = (t * (cpu(s).double() if form == "fp8" else cpu(s).double()[..., None, None]) for t, s in ((b.k, ks), (b.v, vs)))
+        tail = torch.full((1, H, D), 3.0, dtype=dtype, device=DEV)
+        b.check(torch.cat([out.view(rows, H, D), tail]))
+        # the newest tokens are in the cache: what is held is within a step of them
+        newest = b.v[[s // bs for s in slots], :, [s % bs for s in slots]]
+        top = newest.abs().amax(2, keepdim=True)
+        step_of = {"auto": 0.0, "fp8": 2.0 ** -4, "block_int8": 1 / 64, "block_fp8": 2.0 ** -4}[form]
+        assert ((newest - v.view(rows, KVH, D).double()).abs() <= step_of * top * 1.5).all()
+
+
+@pytest.mark.parametrize("form,window,sinks", [("block_int8", 0, 0), ("block_fp8", 24, 4), ("auto", 24, 4), ("fp8", 40, 0)])
+def test_model_runner_graph_equals_eager(form, window, sinks):
+    """LlamaRunner over the block-scaled caches and with a window: the captured decode step gives the eager step's tokens and cache."""
+    from mi355q.model import CONFIGS, LlamaRunner
+    prompt = torch.randint(0, 1024, (2, 37), generator=torch.Generator().manual_seed(1))
+    seen = []
+    for graph in (False, True):
+        r = LlamaRunner(CONFIGS["tiny"], quant="gptq", kv_cache_dtype=form, max_batch=2, max_seq_len=96, sliding_window=window, sink_tokens=sinks)
+        tokens = [r.prefill(prompt).cpu().tolist()]
+        if graph:
+            r.capture()
+        for _ in range(12):
+            r.decode_step()
+            tokens.append(r.tokens.cpu().tolist())
+        seen.append((tokens, [t.clone() for t in r.kc + r.vc], r.kv_scales.clone() if r.block_scaled else None))
+    assert seen[0][0] == seen[1][0]
+    # (the page tail past the last token may hold what the warm-up of the capture left, in caches it writes)
+    if form.startswith("block"):
+        assert all(torch.equal(a, b) for a, b in zip(seen[0][1], seen[1][1])) and torch.equal(seen[0][2], seen[1][2])
+
+
+def test_model_runner_window_wider_than_the_context_changes_nothing():
+    """The same prompt with a window that hides nothing: first tokens equal those of the runner without one (both attention kernels
+    round to the same 16 bits; logits of a random model are far apart compared with that)."""
+    from mi355q.model import CONFIGS, LlamaRunner
+    prompt = torch.randint(0, 2048, (2, 50), generator=torch.Generator().manual_seed(3))
+    first = []
+    for window in (0, 128):
+        r = LlamaRunner(CONFIGS["small"], quant="gptq", max_batch=2, max_seq_len=96, sliding_window=window)
+        first.append(r.prefill(prompt).cpu().tolist())
+    assert first[0] == first[1]

@@ -270,8 +270,13 @@ class LlamaRunner:
     def __init__(self, cfg: LlamaConfig, quant: str = "gptq", kv_cache_dtype: str = "auto", group_size: int = 128,
                  dtype=torch.bfloat16, device="cuda:0", tp_rank: int = 0, tp_size: int = 1, tp_group=None,
                  max_batch: int = 1, max_seq_len: int = 512, block_size: int = 16, seed: int = 0,
-                 keep_checkpoint: bool = False):
+                 keep_checkpoint: bool = False, sliding_window: int = 0, sink_tokens: int = 0):
+        """kv_cache_dtype: "auto", "fp8", or "block_int8" / "block_fp8" (8 bits with a scale for each block and kv head).
+        sliding_window > 0: every layer attends the last `sliding_window` tokens and the first `sink_tokens`."""
         assert quant in ("gptq", "awq", "none")
+        self.block_scaled = ops.is_block_scaled(kv_cache_dtype)
+        self.windowed = self.block_scaled or sliding_window > 0
+        self.sliding_window, self.sink_tokens = sliding_window, sink_tokens
         self.cfg, self.quant, self.dtype, self.device = cfg, quant, dtype, torch.device(device)
         self.tp_rank, self.tp_size, self.tp_group = tp_rank, tp_size, tp_group
         # MI355Q_FORCE_TP_PATH=1 with an initialised process group: issue the two all-reduces per layer and the
@@ -354,14 +359,16 @@ class LlamaRunner:
         # paged KV cache, ROCM_ATTN layout (v1/attention/backends/rocm_attn.py:246-256, ops/paged_attn.py:16-29)
         self.blocks_per_seq = (max_seq_len + block_size - 1) // block_size
         nblk = self.blocks_per_seq * max_batch
-        cdt = torch.uint8 if self.fp8 else dtype
-        x = 16 // (1 if self.fp8 else 2)
+        cdt = torch.uint8 if self.fp8 or self.block_scaled else dtype
+        x = 16 // (2 if cdt == dtype else 1)
         self.kc = [torch.zeros((nblk, self.kv_heads, D // x, block_size, x), dtype=cdt, device=self.device)
                    for _ in range(cfg.layers)]
         self.vc = [torch.zeros((nblk, self.kv_heads, D, block_size), dtype=cdt, device=self.device)
                    for _ in range(cfg.layers)]
         self.k_scale = torch.full((), 1.0 / 16 if self.fp8 else 1.0, dtype=torch.float32, device=self.device)
         self.v_scale = torch.full((), 1.0 / 16 if self.fp8 else 1.0, dtype=torch.float32, device=self.device)
+        if self.block_scaled:
+            self.kv_scales = torch.zeros((cfg.layers, 2, nblk, self.kv_heads), dtype=torch.float32, device=self.device)
         self.block_tables = torch.arange(nblk, dtype=torch.int32, device=self.device).view(max_batch, self.blocks_per_seq)
         self.scale = 1.0 / D ** 0.5
         self.P = (max_seq_len + _lib.PA_PARTITION - 1) // _lib.PA_PARTITION
@@ -410,6 +417,12 @@ class LlamaRunner:
         return (self.quant != "none" and not self.tp_collectives and T <= ops.MM_MAX_TOKENS
                 and ops.w4a16_mm_add_rms_norm_preferred(T, lin.w))
 
+    def _window_attention(self, li, q, out, block_tables, seq_lens, query_start_loc, max_query_len, max_seq_len):
+        ks, vs = (self.kv_scales[li, 0], self.kv_scales[li, 1]) if self.block_scaled else (self.k_scale, self.v_scale)
+        ops.paged_window_attention(out, q, self.kc[li], self.vc[li], self.kv_heads, self.scale, block_tables, seq_lens,
+                                   query_start_loc, max_query_len, max_seq_len, self.kv_cache_dtype, ks, vs, self.sliding_window,
+                                   self.sink_tokens)
+
     def _layer(self, L, li, h, residual, positions, slot_mapping, attend, normed=False, next_norm=None):
         """One decoder layer.  `normed`: h already is RMSNorm(residual) (the previous layer's down
         projection finished it).  `next_norm`: weight of the norm that follows this layer; when the
@@ -425,7 +438,7 @@ class LlamaRunner:
             else:
                 h = h.sum()
         # prompt tokens on the tiled kernel: projection, RoPE and cache write as one op
-        qkv_tail = (attend is not None and self.quant != "none" and ops.MM_MIN_TOKENS <= T <= ops.MM_MAX_TOKENS
+        qkv_tail = (attend is not None and self.quant != "none" and not self.block_scaled and ops.MM_MIN_TOKENS <= T <= ops.MM_MAX_TOKENS
                     and ops._mm_supported(L["qkv"].w))
 
         def qkv_proj(x):
@@ -461,7 +474,10 @@ class LlamaRunner:
                                        self.max_seq_len, self.kv_cache_dtype, self.k_scale, self.v_scale)
         else:
             q, k, v = qkv[:, :qs], qkv[:, qs:qs + ks], qkv[:, qs + ks:]
-            if not qkv_tail:
+            if self.block_scaled:
+                ops.rope_and_cache_blocks(positions, q, k, v, D, self.cos_sin, True, self.kc[li], self.vc[li],
+                                          self.kv_scales[li, 0], self.kv_scales[li, 1], slot_mapping, self.kv_cache_dtype)
+            elif not qkv_tail:
                 ops.rope_and_cache(positions, q, k, v, D, self.cos_sin, True, self.kc[li], self.vc[li], slot_mapping,
                                    self.kv_cache_dtype, self.k_scale, self.v_scale)
             attend(li, q.view(T, self.heads, D), attn)
@@ -550,11 +566,14 @@ class LlamaRunner:
         qsl = torch.arange(0, (B + 1) * T, T, dtype=torch.int32, device=dev)
         seq_lens = torch.full((B,), T, dtype=torch.int32, device=dev)
         P = (T + _lib.PA_PARTITION - 1) // _lib.PA_PARTITION
-        tmp = torch.empty((B * T, self.heads, P, self.cfg.head_dim), dtype=self.dtype, device=dev)
-        es = torch.empty((B * T, self.heads, P), dtype=torch.float32, device=dev)
+        rows = 0 if self.windowed else B * T
+        tmp = torch.empty((rows, self.heads, P, self.cfg.head_dim), dtype=self.dtype, device=dev)
+        es = torch.empty((rows, self.heads, P), dtype=torch.float32, device=dev)
         ml = torch.empty_like(es)
 
         def attend(li, q, out):
+            if self.windowed:
+                return self._window_attention(li, q, out, self.block_tables[:B], seq_lens, qsl, T, T)
             ops.paged_prefill_attention(out, es, ml, tmp, q, self.kc[li], self.vc[li], self.kv_heads, self.scale,
                                         self.block_tables[:B], seq_lens, qsl, T, self.block_size, T, None,
                                         self.kv_cache_dtype, self.k_scale, self.v_scale)
@@ -579,7 +598,13 @@ class LlamaRunner:
         leaves the sampled ids in self.tokens and advances the positions."""
         B = self.max_batch
         attend = slot_mapping = None   # the fused attention step derives the slot from the block table
-        if self.fp8 and self.cfg.head_dim != 128:  # the fused step needs head 128 with an fp8 cache
+        if self.windowed:
+            slot_mapping = self.slot_base + self.positions
+
+            def attend(li, q, out):
+                self._window_attention(li, q, out, self.block_tables, self.seq_lens, None, 1, self.max_seq_len)
+
+        elif self.fp8 and self.cfg.head_dim != 128:  # the fused step needs head 128 with an fp8 cache
             slot_mapping = self.slot_base + self.positions
 
             def attend(li, q, out):
@@ -607,6 +632,10 @@ class LlamaRunner:
         v1/worker/gpu_model_runner.py:6834; every op here is capture-safe)."""
         # warm up on a side stream so allocator state and the split-K workspace exist before capture
         state = (self.tokens.clone(), self.positions.clone(), self.seq_lens.clone(), self.h0.clone())
+        # (block-scaled caches are not written meanwhile: a scale that has grown for tokens to come does not shrink again)
+        base = self.slot_base.clone()
+        if self.block_scaled:
+            self.slot_base.fill_(-(1 << 40))
         s = torch.cuda.Stream()
         s.wait_stream(torch.cuda.current_stream())
         with torch.cuda.stream(s):
@@ -614,6 +643,7 @@ class LlamaRunner:
                 self._decode_body()
         torch.cuda.current_stream().wait_stream(s)
         torch.cuda.synchronize()
+        self.slot_base.copy_(base)
         self.tokens.copy_(state[0]); self.positions.copy_(state[1]); self.seq_lens.copy_(state[2]); self.h0.copy_(state[3])
         g = torch.cuda.CUDAGraph()
         # with a process group alive its watchdog thread queries events while this thread captures: only this

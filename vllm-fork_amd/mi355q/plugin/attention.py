@@ -9,6 +9,10 @@ vllm/v1/attention/ops/chunked_prefill_paged_decode.py:271-493.  Unlike the refer
 is allocated per call: the partition scratch is one buffer per device, shared by the impls of all
 layers (their launches are ordered on one stream), reserved up front by the metadata builder and only
 ever grown outside graph capture.
+
+Layers with a sliding window (and first tokens that stay visible), and layers whose cache is held in 8 bits with a scale for
+each (block, kv head) -- kv_cache_dtype "block_int8" / "block_fp8", no scales in the checkpoint -- run on
+ops.paged_window_attention for prompt, draft and decode rows alike; its scratch comes from torch's allocator.
 """
 from dataclasses import dataclass
 
@@ -110,7 +114,7 @@ def reserve_partition_scratch(max_tokens: int, max_seq_len: int, num_heads: int,
 
 class Mi355AttentionBackend:
     supported_dtypes = [torch.float16, torch.bfloat16]
-    supported_kv_cache_dtypes = ["auto", "float16", "bfloat16", "fp8", "fp8_e4m3"]
+    supported_kv_cache_dtypes = ["auto", "float16", "bfloat16", "fp8", "fp8_e4m3", "block_int8", "block_fp8"]
     forward_includes_kv_cache_update = False
 
     @staticmethod
@@ -131,7 +135,7 @@ class Mi355AttentionBackend:
 
     @classmethod
     def supports_sliding_window(cls) -> bool:
-        return False
+        return True
 
     @staticmethod
     def use_cascade_attention(*args, **kwargs) -> bool:
@@ -143,6 +147,11 @@ class Mi355AttentionBackend:
         if block_size % 16 != 0:
             raise ValueError("Block size must be a multiple of 16.")
         return (2, num_blocks, block_size, num_kv_heads, head_size)
+
+    @staticmethod
+    def get_kv_scales_shape(num_blocks: int, num_kv_heads: int) -> tuple[int, int, int]:
+        """fp32 scales of K and V beside a "block_int8" / "block_fp8" cache (`Attention.kv_scales`)."""
+        return (2, num_blocks, num_kv_heads)
 
     @staticmethod
     def get_impl_cls():
@@ -166,9 +175,17 @@ class Mi355AttentionImpl:
     def __init__(self, num_heads: int, head_size: int, scale: float, num_kv_heads: int,
                  alibi_slopes: list[float] | None = None, sliding_window: int | None = None,
                  kv_cache_dtype: str = "auto", logits_soft_cap: float | None = None, attn_type: str = "decoder",
-                 kv_sharing_target_layer_name=None, sinks=None) -> None:
-        if sliding_window is not None or sinks is not None or logits_soft_cap:
-            raise NotImplementedError("sliding window, sinks and logit soft-capping are not supported")
+                 kv_sharing_target_layer_name=None, sinks=None, sink_tokens: int = 0) -> None:
+        # (sinks: learned logits per head; sink_tokens: first tokens that stay visible behind the window)
+        if sinks is not None or logits_soft_cap:
+            raise NotImplementedError("sink logits and logit soft-capping are not supported")
+        if sliding_window is not None and sliding_window <= 0 or sink_tokens < 0:
+            raise ValueError("sliding_window must be positive, sink_tokens not negative")
+        self.block_scaled = ops.is_block_scaled(kv_cache_dtype)
+        self.windowed = self.block_scaled or sliding_window is not None
+        self.sliding_window, self.sink_tokens = sliding_window or 0, sink_tokens
+        if self.windowed and alibi_slopes is not None:
+            raise NotImplementedError("ALiBi with a sliding window or a block-scaled cache is not supported")
         if attn_type != "decoder":
             raise NotImplementedError("only decoder self-attention is supported")
         if head_size not in Mi355AttentionBackend.get_supported_head_sizes():
@@ -191,10 +208,19 @@ class Mi355AttentionImpl:
             self.alibi_slopes = self.alibi_slopes.to(kv_cache.device)
         return k, v
 
+    def _scales(self, layer):
+        """(k, v) scales of the layer: one value each, or [blocks, kv_heads]."""
+        return (layer.kv_scales[0], layer.kv_scales[1]) if self.block_scaled else (layer._k_scale, layer._v_scale)
+
     # -- contract ----------------------------------------------------------
     def do_kv_cache_update(self, layer, key, value, kv_cache, slot_mapping) -> None:
         k, v = self._caches(kv_cache)
         T = slot_mapping.numel()
+        if self.block_scaled:
+            ops.reshape_and_cache_blocks(key[:T].view(T, self.num_kv_heads, self.head_size),
+                                         value[:T].view(T, self.num_kv_heads, self.head_size), k, v, *self._scales(layer),
+                                         slot_mapping, self.kv_cache_dtype)
+            return
         ops.reshape_and_cache(key[:T].view(T, self.num_kv_heads, self.head_size),
                               value[:T].view(T, self.num_kv_heads, self.head_size), k, v, slot_mapping,
                               self.kv_cache_dtype, layer._k_scale, layer._v_scale)
@@ -212,6 +238,11 @@ class Mi355AttentionImpl:
         q = query[:T].view(T, self.num_heads, self.head_size)
         o = output[:T].view(T, self.num_heads, self.head_size)
         k, v = self._caches(kv_cache)
+        if self.windowed:
+            ops.paged_window_attention(o, q, k, v, self.num_kv_heads, self.scale, md.block_table, md.seq_lens,
+                                       md.query_start_loc, md.max_query_len, md.max_seq_len, self.kv_cache_dtype,
+                                       *self._scales(layer), self.sliding_window, self.sink_tokens)
+            return output
         bs = v.shape[3]
         P = (md.max_seq_len + _lib.PA_PARTITION - 1) // _lib.PA_PARTITION
         per_row = self.num_heads * P * self.head_size * q.element_size()
@@ -269,17 +300,23 @@ class Mi355AttentionImpl:
         (rocm_attn.py:522-562)."""
         k, v = self._caches(kv_cache)
         T = layer_slot_mapping.numel()
+        if self.block_scaled:
+            ops.rope_and_cache_blocks(positions[:T], query[:T], key[:T], value[:T], self.head_size, cos_sin_cache, is_neox, k, v,
+                                      *self._scales(layer), layer_slot_mapping, self.kv_cache_dtype)
+            return
         ops.rope_and_cache(positions[:T], query[:T], key[:T], value[:T], self.head_size, cos_sin_cache, is_neox, k, v,
                            layer_slot_mapping, self.kv_cache_dtype, layer._k_scale, layer._v_scale)
 
     def decode_fused_supported(self) -> bool:
-        return self.head_size == 128 or not is_quantized_kv_cache(self.kv_cache_dtype)
+        return not self.windowed and (self.head_size == 128 or not is_quantized_kv_cache(self.kv_cache_dtype))
 
     def forward_decode_fused(self, layer, qkv, positions, cos_sin_cache, kv_cache,
                              attn_metadata: Mi355AttentionMetadata, output):
         """Decode rows only: NeoX RoPE, KV-cache write and attention in one launch from the fused
         qkv projection output (what do_rope_and_kv_cache_update + forward do in two steps,
         rocm_attn.py:522-562,367-469)."""
+        if self.windowed:
+            raise NotImplementedError("the fused decode step has neither windows nor block scales (decode_fused_supported())")
         md = attn_metadata
         S = md.num_actual_tokens
         k, v = self._caches(kv_cache)
@@ -296,7 +333,8 @@ class Attention(torch.nn.Module):
     owns the scale buffers and the impl; forward = cache update, then attention."""
 
     def __init__(self, num_heads: int, head_size: int, scale: float, num_kv_heads: int | None = None,
-                 cache_dtype: str = "auto", quant_config=None, prefix: str = "", alibi_slopes=None):
+                 cache_dtype: str = "auto", quant_config=None, prefix: str = "", alibi_slopes=None,
+                 sliding_window: int | None = None, sink_tokens: int = 0):
         super().__init__()
         self.num_heads, self.head_size = num_heads, head_size
         self.num_kv_heads = num_kv_heads or num_heads
@@ -309,8 +347,10 @@ class Attention(torch.nn.Module):
         self.quant_method = method
         if self.quant_method is not None:
             self.quant_method.create_weights(self)
-        self.impl = Mi355AttentionImpl(num_heads, head_size, scale, self.num_kv_heads, alibi_slopes, None, cache_dtype)
+        self.impl = Mi355AttentionImpl(num_heads, head_size, scale, self.num_kv_heads, alibi_slopes, sliding_window, cache_dtype,
+                                       sink_tokens=sink_tokens)
         self.kv_cache: torch.Tensor | None = None
+        self.kv_scales: torch.Tensor | None = None    # block-scaled caches: fp32 [2, blocks, kv_heads]
 
     def process_weights_after_loading(self) -> None:
         if self.quant_method is not None:

@@ -42,6 +42,14 @@ def register_torch_ops() -> None:
       "Tensor key_cache, Tensor value_cache, int num_kv_heads, float scale, Tensor block_tables, Tensor seq_lens, "
       "Tensor? query_start_loc, int block_size, int max_seq_len, Tensor? alibi_slopes, str kv_cache_dtype, "
       "Tensor k_scale, Tensor v_scale) -> ()")
+    d("rope_and_cache_blocks(Tensor positions, Tensor query, Tensor key, Tensor value, int head_size, Tensor cos_sin_cache, "
+      "bool is_neox, Tensor! key_cache, Tensor! value_cache, Tensor! k_scales, Tensor! v_scales, Tensor slot_mapping, "
+      "str kv_cache_dtype, Tensor! query_out) -> ()")
+    d("reshape_and_cache_blocks(Tensor key, Tensor value, Tensor! key_cache, Tensor! value_cache, Tensor! k_scales, "
+      "Tensor! v_scales, Tensor slot_mapping, str kv_cache_dtype) -> ()")
+    d("paged_window_attention(Tensor! out, Tensor query, Tensor key_cache, Tensor value_cache, int num_kv_heads, float scale, "
+      "Tensor block_tables, Tensor seq_lens, Tensor? query_start_loc, int max_query_len, int max_seq_len, str kv_cache_dtype, "
+      "Tensor? k_scale, Tensor? v_scale, int sliding_window, int sink_tokens) -> ()")
     d("argmax(Tensor logits) -> Tensor")
     d("apply_repetition_penalties_(Tensor! logits, Tensor prompt_mask, Tensor output_mask, Tensor repetition_penalties) -> ()")
 
@@ -104,8 +112,26 @@ def register_torch_ops() -> None:
     def _(logits, prompt_mask, output_mask, repetition_penalties):
         ops.apply_repetition_penalties(logits, prompt_mask, output_mask, repetition_penalties)
 
+    @impl(_lib, "rope_and_cache_blocks", "CUDA")
+    def _(positions, query, key, value, head_size, cos_sin_cache, is_neox, key_cache, value_cache, k_scales, v_scales,
+          slot_mapping, kv_cache_dtype, query_out):
+        ops.rope_and_cache_blocks(positions, query, key, value, head_size, cos_sin_cache, is_neox, key_cache, value_cache,
+                                  k_scales, v_scales, slot_mapping, kv_cache_dtype, query_out)
+
+    @impl(_lib, "reshape_and_cache_blocks", "CUDA")
+    def _(key, value, key_cache, value_cache, k_scales, v_scales, slot_mapping, kv_cache_dtype):
+        ops.reshape_and_cache_blocks(key, value, key_cache, value_cache, k_scales, v_scales, slot_mapping, kv_cache_dtype)
+
+    @impl(_lib, "paged_window_attention", "CUDA")
+    def _(out, query, key_cache, value_cache, num_kv_heads, scale, block_tables, seq_lens, query_start_loc, max_query_len,
+          max_seq_len, kv_cache_dtype, k_scale, v_scale, sliding_window, sink_tokens):
+        ops.paged_window_attention(out, query, key_cache, value_cache, num_kv_heads, scale, block_tables, seq_lens,
+                                   query_start_loc, max_query_len, max_seq_len, kv_cache_dtype, k_scale, v_scale,
+                                   sliding_window, sink_tokens)
+
     for name in ("rms_norm", "fused_add_rms_norm", "rotary_embedding", "silu_and_mul", "reshape_and_cache",
-                 "reshape_and_cache_flash", "paged_attention", "apply_repetition_penalties_"):
+                 "reshape_and_cache_flash", "paged_attention", "apply_repetition_penalties_", "rope_and_cache_blocks",
+                 "reshape_and_cache_blocks", "paged_window_attention"):
         register_fake(f"mi355q::{name}")(lambda *a, **k: None)
 
     @impl(_lib, "argmax", "CUDA")

@@ -23,6 +23,7 @@ import torch
 from vllm.v1.attention.backend import (AttentionBackend, AttentionCGSupport, AttentionImpl, AttentionMetadataBuilder,
                                        AttentionType, CommonAttentionMetadata, MultipleOf)
 
+from .. import ops
 from . import attention as _impl
 
 
@@ -66,6 +67,9 @@ class MI355XAttentionImpl(AttentionImpl[_impl.Mi355AttentionMetadata]):
                  sinks: torch.Tensor | None = None) -> None:
         if kv_sharing_target_layer_name is not None:
             raise NotImplementedError("KV-cache sharing between layers is not supported")
+        if sliding_window is not None:
+            raise NotImplementedError("sliding windows are not offered through the fork's backend (its cache specification "
+                                      "for windowed layers is not wired up); mi355q's own Attention layer has them")
         _impl.Mi355AttentionImpl.__init__(self, num_heads, head_size, scale, num_kv_heads or num_heads, alibi_slopes,
                                           sliding_window, kv_cache_dtype, logits_soft_cap,
                                           "decoder" if attn_type == AttentionType.DECODER else str(attn_type),
@@ -91,7 +95,9 @@ class MI355XAttentionImpl(AttentionImpl[_impl.Mi355AttentionMetadata]):
 class MI355XAttentionBackend(AttentionBackend):
     """Registered as AttentionBackendEnum.CUSTOM; selected with `--attention-backend CUSTOM`."""
     supported_dtypes: ClassVar[list[torch.dtype]] = list(_impl.Mi355AttentionBackend.supported_dtypes)
-    supported_kv_cache_dtypes: ClassVar[list[str]] = list(_impl.Mi355AttentionBackend.supported_kv_cache_dtypes)
+    # (the block-scaled caches need a scale tensor beside the cache, which the fork does not allocate)
+    supported_kv_cache_dtypes: ClassVar[list[str]] = [d for d in _impl.Mi355AttentionBackend.supported_kv_cache_dtypes
+                                                      if not ops.is_block_scaled(d)]
     forward_includes_kv_cache_update: bool = False
 
     @staticmethod
