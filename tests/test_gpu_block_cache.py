@@ -399,15 +399,14 @@ class Batch:
 
     def attention_bound(self, o, mass, vmax, slip, n):
         """What the roundings add up to.  mass = sum w |v|:
-          probabilities rounded to fp16 (8-bit caches) or the model's type: one half step of each, u_p * mass
-          prompt rows over 8-bit caches: a code times its block's relative scale is rounded to fp16 as well, another half step
-            2^-11 of each |v| (a code of 8 bits times a scale of 24 does not fit 11), so u_p is twice 2^-11 there
+          probabilities rounded to fp16 (8-bit caches) or the model's type, in the products with V and in their sum: one half step
+            of each weight in numerator and denominator, 2 u_p * mass
           logits: products summed in fp32 over the head, at most (D + 8) 2^-24 of sum |q k| each, and the base-2 exponent's own
             error of about 2^-22; both as relative errors of the weights, in numerator and denominator: 2 * (...) * mass
           the sums over n tokens in fp32, and the scale factors: (n / 16 + 32) 2^-24 * mass (products are added 16 and more at a time)
           fp16 probabilities below its normal range: n * 2^-32 of the largest |v| (times 4 for the headroom of the scales)
           the result rounded to the model's type: u_out * (|o| + the above)"""
-        u_p = UNIT[self.dtype] if self.form == "auto" else 2 * 2.0 ** -11
+        u_p = 2 * (UNIT[self.dtype] if self.form == "auto" else 2.0 ** -11)
         weights = 2 * ((self.D + 8) * 2.0 ** -24 * slip * 1.5 + 2.0 ** -21)
         e = (u_p + weights + (n / 16 + 32) * 2.0 ** -24) * mass + n * 2.0 ** -30 * vmax
         return e + UNIT[self.dtype] * (o.abs() + e) + 2.0 ** -25

@@ -28,9 +28,11 @@ typedef __attribute__((ext_vector_type(2))) _Float16 wa_f16x2;
 typedef __attribute__((ext_vector_type(2))) __bf16 wa_bf16x2;
 
 constexpr float WA_LOG2E = 1.44269504088896f;
-// Probabilities are kept as 2^(x - m + 7): fp16 then resolves a probability down to 2^-31 of the largest, and the running
-// maximum m may lag behind by up to 8 before the sums are rescaled (the largest value is 2^15).
-constexpr float WA_SHIFT = 7.0f, WA_LAG = 8.0f;
+// Probabilities are kept as 2^(x - m + 6): fp16 then resolves a probability down to 2^-30 of the largest, and the running
+// maximum m may lag behind by up to 8 before the sums are rescaled (with a factor of up to 2 from V's scale, the largest
+// value is 2^15).  The sums of weights are taken over the probabilities as they are rounded for the product with V: where a
+// few tokens carry a row, their rounding cancels.
+constexpr float WA_SHIFT = 6.0f, WA_LAG = 8.0f;
 
 struct WindowParams {
   uint16_t* out;
@@ -145,6 +147,18 @@ __device__ inline bool not_finite(u32x4 v) {
   for (int i = 0; i < 4; i++) bad |= (v[i] & e) == e || ((v[i] >> 16) & e) == e;
   return bad;
 }
+// c + the two 16-bit values of w
+template <typename MT>
+__device__ inline float add_pair(uint32_t w, float c);
+template <>
+__device__ inline float add_pair<BF16>(uint32_t w, float c) {
+  return __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2, w), __builtin_bit_cast(bf16x2, BF16::ones), c, false);
+}
+template <>
+__device__ inline float add_pair<FP16>(uint32_t w, float c) {
+  return __builtin_amdgcn_fdot2(__builtin_bit_cast(wa_f16x2, w), __builtin_bit_cast(wa_f16x2, FP16::ones), c, false);
+}
+
 // value n of eight (none: n outside 0 .. 7), in lanes that are `here`; zeros elsewhere
 template <typename MT>
 __device__ inline u32x4 only(u32x4 v, bool here, int n) {
@@ -310,7 +324,7 @@ __global__ __launch_bounds__(64 * NW, 2) void window_rows_kernel(const WindowPar
   }
 
   f32x4 o[NCT][DT16];
-  float m[NCT], l[NCT], vref = 0.f;
+  float m[NCT], l[NCT], vref = 0.f, vinv = 1.f;
 #pragma unroll
   for (int n = 0; n < NCT; n++) {
     m[n] = -INFINITY;
@@ -410,8 +424,12 @@ __global__ __launch_bounds__(64 * NW, 2) void window_rows_kernel(const WindowPar
     if (KV != KV16 && __any(vtop > vref)) {
       back = vref / (2.f * vtop);      // headroom of 2: the next slightly larger scale changes nothing
       vref = 2.f * vtop;
+      vinv = 1.f / vref;
     }
-    const float r = KV == KV16 ? 1.f : vref > 0.f ? vs / vref : vs;
+    const float r = KV == KV16 || !ok ? 1.f : vs * vinv;
+    // the sum of weights over what is rounded for the product, where V's scale leaves it its bits
+    const bool rounded = KV == KV16 || __all(r >= 0x1p-10f);
+    const float less = KV == KV16 ? 1.f : __builtin_amdgcn_rcpf(r);
     u32x4 pf[NCT][2];
 #pragma unroll
     for (int n = 0; n < NCT; n++) {
@@ -446,18 +464,24 @@ __global__ __launch_bounds__(64 * NW, 2) void window_rows_kernel(const WindowPar
         m[n] = mn;
       }
       const float ms = (m[n] == -INFINITY ? 0.f : m[n]) - WA_ROWS_SHIFT;
+      float sum = 0.f;
 #pragma unroll
-      for (int i = 0; i < 16; i++) {
-        x[i] = exp2_fast(INNER ? __builtin_fmaf(x[i], f, -ms) : x[i] - ms);
-        l[n] += x[i];
+      for (int i = 0; i < 16; i++) x[i] = exp2_fast(INNER ? __builtin_fmaf(x[i], f, -ms) : x[i] - ms);
+      if (!rounded) {
+#pragma unroll
+        for (int i = 0; i < 16; i++) sum += x[i];
+        l[n] += sum;
+        sum = 0.f;
       }
 #pragma unroll
       for (int i = 0; i < 8; i++) {
-        uint32_t w = KV == KV16 ? pack2<MT>(x[2 * i], x[2 * i + 1]) : pack2<MT>(x[2 * i] * r, x[2 * i + 1] * r);
+        uint32_t w = KV == KV16 ? pack_p<MT>(x[2 * i], x[2 * i + 1]) : pack_p<MT>(x[2 * i] * r, x[2 * i + 1] * r);
+        sum = add_pair<MT>(w, sum);
         // (a NaN scale reaches only the columns that see its tokens)
         if (!INNER && KV != KV16) w &= ((seen >> (2 * i)) & 1 ? 0xffffu : 0u) | ((seen >> (2 * i)) & 2 ? 0xffff0000u : 0u);
         pf[n][i >> 2][i & 3] = w;
       }
+      if (rounded) l[n] = KV == KV16 ? l[n] + sum : __builtin_fmaf(sum, less, l[n]);
     }
 
     // ---- O^T += V^T P^T ----------------------------------------------------------------------------------------------
@@ -504,7 +528,7 @@ __global__ __launch_bounds__(64 * NW, 2) void window_rows_kernel(const WindowPar
         f32x4 s[NCT][4];
         logits(s);
         const float ks = KV == KV16 ? 1.f : __shfl(at_ks, g, 64), vs = KV == KV16 ? 1.f : __shfl(at_vs, g, 64);
-        const float r = KV == KV16 ? 1.f : vref > 0.f ? vs / vref : vs;
+        const float r = KV == KV16 || !ok ? 1.f : vs * vinv;
         uint32_t seen[NCT];
         u32x4 pf[NCT][2];
 #pragma unroll
@@ -609,9 +633,9 @@ __global__ __launch_bounds__(64 * NW, 2) void window_rows_kernel(const WindowPar
 //
 // v_mfma_f32_32x32x16.  Row r of a 32-token tile of S^T is token r with bits 2 and 3 exchanged: the 8 logits a lane then holds
 // of each 16-token stretch are tokens 8 h .. 8 h + 7 of it (h = lane / 32), the B operand of O^T as they stand.  A stretch lies
-// in one block, so K's scale is wave-uniform per 8 registers and joins the factor of the exponent; V's scale is applied while
-// widening, as a factor relative to vref, with 2^7 in hand (fp16 then resolves blocks whose scales are 10^-6 of the largest
-// to all 11 bits).
+// in one block, so K's scale is wave-uniform per 8 registers and joins the factor of the exponent.  V's scale is a power of two
+// times a number in [1, 2): the power, relative to that of the largest scale met so far and with 2^7 in hand, goes into the
+// widened codes, exactly (down to scales of 2^-30 of the largest); the number goes into the exponent of the probabilities.
 // ---------------------------------------------------------------------------------------------------------------------
 typedef __attribute__((ext_vector_type(16))) float f32x16;
 
@@ -634,18 +658,6 @@ __device__ inline float pair_sum(float v) {
   auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
   return __uint_as_float(r[0]) + __uint_as_float(r[1]);
 }
-// c + the two 16-bit values of w
-template <typename MT>
-__device__ inline float add_pair(uint32_t w, float c);
-template <>
-__device__ inline float add_pair<BF16>(uint32_t w, float c) {
-  return __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2, w), __builtin_bit_cast(bf16x2, BF16::ones), c, false);
-}
-template <>
-__device__ inline float add_pair<FP16>(uint32_t w, float c) {
-  return __builtin_amdgcn_fdot2(__builtin_bit_cast(wa_f16x2, w), __builtin_bit_cast(wa_f16x2, FP16::ones), c, false);
-}
-
 constexpr float WA_VSHIFT = 128.0f;
 
 template <typename DT, int KV, int HEAD, int NW>
@@ -662,9 +674,10 @@ __global__ __launch_bounds__(64 * NW, HEAD == 64 ? 4 : 2) void window_flash_kern
   constexpr int CHUNK = 64;
   struct Chunk {
     u32x4 at[4 * CHUNK];      // per stretch: block offset (64 bits), token offset in the block, tokens somebody sees
-    float ks[4 * CHUNK], vs[4 * CHUNK];
+    float ks[4 * CHUNK];
+    float vpow[4 * CHUNK], vlog[4 * CHUNK], vinv[4 * CHUNK];   // V's scale: 2^7 power / vref, log2 and reciprocal of the rest
     int ok[CHUNK];            // per tile: stretches whose page exists and that begin before the end
-    float vref;
+    float vref;               // a power of two above every scale so far
   };
   __shared__ __attribute__((aligned(1024))) unsigned char lds[LDS];
   __shared__ __attribute__((aligned(16))) Chunk chunks[2];
@@ -780,10 +793,19 @@ __global__ __launch_bounds__(64 * NW, HEAD == 64 ? 4 : 2) void window_flash_kern
     }
     if constexpr (KV != KV16) {
       top = wave_max(top);
+      top = top > 0.f ? __uint_as_float((__float_as_uint(fminf(top, 0x1p125f)) & 0x7f800000u) + 0x00800000u) : 0.f;
       if (first > begin) top = fmaxf(top, chunks[((first - begin) / CHUNK & 1) ^ 1].vref);   // never falls
       const float inv = top > 0.f ? WA_VSHIFT / top : 0.f;
 #pragma unroll
-      for (int i = 0; i < CHUNK / 16; i++) ch.vs[64 * i + lane] = v[i] * inv + (v[i] - v[i]);   // (a NaN stays one where top is 0)
+      for (int i = 0; i < CHUNK / 16; i++) {
+        const int n = 64 * i + lane;
+        const uint32_t bits = __float_as_uint(v[i]);
+        const bool split = v[i] > 0x1p-100f && v[i] < INFINITY;      // (else as it is: zero, next to it, or a NaN that stays one)
+        const float rest = split ? __uint_as_float((bits & 0x007fffffu) | 0x3f800000u) : 1.f;
+        ch.vpow[n] = split ? __uint_as_float(bits & 0x7f800000u) * inv : v[i] * inv + (v[i] - v[i]);
+        ch.vlog[n] = __builtin_amdgcn_logf(rest);
+        ch.vinv[n] = 1.f / rest;
+      }
       if (lane == 0) ch.vref = top;
     }
   };
@@ -844,7 +866,7 @@ __global__ __launch_bounds__(64 * NW, HEAD == 64 ? 4 : 2) void window_flash_kern
       const uint32_t seen = __builtin_amdgcn_readfirstlane(chunk_of(n).at[e0][3]);
       u32x4 v[EB == 1 ? 2 : 1];
       if constexpr (EB == 1) {
-        const _Float16 r16 = (_Float16)chunk_of(n).vs[e0];
+        const _Float16 r16 = (_Float16)chunk_of(n).vpow[e0];
         const wa_f16x2 rr = {r16, r16};
 #pragma unroll
         for (int h = 0; h < 2; h++) {
@@ -1006,22 +1028,30 @@ __global__ __launch_bounds__(64 * NW, HEAD == 64 ? 4 : 2) void window_flash_kern
       m = mn;
     }
     const float ms = (m == -INFINITY ? 0.f : m) - WA_SHIFT;
+    f32x4 plus = {-ms, -ms, -ms, -ms}, less = {1.f, 1.f, 1.f, 1.f};
+    if constexpr (KV != KV16) {
+      plus += *reinterpret_cast<const f32x4*>(&ch.vlog[n % CHUNK * 4]);
+      less = *reinterpret_cast<const f32x4*>(&ch.vinv[n % CHUNK * 4]);
+    }
     u32x4 pf[4];
 #pragma unroll
     for (int j = 0; j < 4; j++) {
 #pragma unroll
       for (int e = 0; e < 8; e++) {
         const float x = s[j >> 1][8 * (j & 1) + e];
-        s[j >> 1][8 * (j & 1) + e] = exp2_fast(INNER ? __builtin_fmaf(x, f[j], -ms) : x - ms);
+        s[j >> 1][8 * (j & 1) + e] = exp2_fast(INNER ? __builtin_fmaf(x, f[j], plus[j]) : x + plus[j]);
       }
     }
 #pragma unroll
-    for (int j = 0; j < 4; j++)
+    for (int j = 0; j < 4; j++) {
+      float sum = 0.f;
 #pragma unroll
       for (int e = 0; e < 4; e++) {
         pf[j][e] = pack_p<MT>(s[j >> 1][8 * (j & 1) + 2 * e], s[j >> 1][8 * (j & 1) + 2 * e + 1]);
-        l = add_pair<MT>(pf[j][e], l);
+        sum = add_pair<MT>(pf[j][e], sum);
       }
+      l = KV == KV16 ? l + sum : __builtin_fmaf(sum, less[j], l);
+    }
 
     // ---- O^T += V^T P^T -------------------------------------------------------------------------------------------------
     const unsigned char* vt = st0 + KBYTES;
