@@ -463,6 +463,52 @@ def test_long_contexts_are_cut_and_joined(form, window, sinks):
 
 
 @pytest.mark.parametrize("form", FORMS)
+def test_one_long_context_among_many_short_ones(form):
+    """More sequences than the chip has room for at once, one of them cut into stretches: alone, with drafts, and with a prompt."""
+    short = [(7 * i % 150, 1) for i in range(39)]
+    for more, n in (((9000, 1), 1), ((8300, 5), 5), ((4500, 70), 70)):
+        b = Batch(short[:20] + [more] + short[20:] + [(4200, n // 2 + 1)], 8, 2, 64, 16, form, torch.bfloat16, seed=16)
+        assert ops.paged_window_attention_workspace_bytes(len(b.lens), b.rows + 1, 8, 2, 64, n, b.max_len, form) > 0
+        b.check()
+        b.check(b.run(max_seq_len=1 << 17))
+        b.check(b.run(max_query_len=n + 20))
+
+
+def test_one_scale_that_is_no_number():
+    """Rows that see nothing stay zero whatever the scale is."""
+    b = Batch([(0, 3), (20, 2), (0, 300)], 4, 2, 64, 16, "fp8", torch.bfloat16, seed=17)
+    b.seq_lens.copy_(torch.tensor([0, 22, 100]))
+    for name in ("ks", "vs"):
+        held, b.dev[name] = b.dev[name], torch.tensor(float("nan"), device=DEV)
+        got = cpu(b.run())
+        b.dev[name] = held
+        assert torch.equal(got[:3], torch.zeros_like(got[:3])) and torch.isnan(got[3:5]).all()
+        assert torch.equal(got[5:205], torch.zeros_like(got[5:205])) and torch.isnan(got[205:305]).all()
+
+
+@pytest.mark.parametrize("form", FORMS)
+def test_query_that_is_no_number(form):
+    """A NaN in a query row makes that row of that head NaN, nothing else, and no zero of it."""
+    b = Batch([(20, 2), (0, 300), (4500, 1)], 4, 2, 64, 16, form, torch.bfloat16, seed=18)
+    clean = cpu(b.run())
+    for row, head in ((1, 2), (2, 0), (150, 3), (301, 1), (302, 0)):
+        b.dev["q"][row, head, 5] = float("nan")
+        clean[row, head] = float("nan")
+    got = cpu(b.run())
+    assert torch.equal(torch.isnan(got), torch.isnan(clean)) and torch.equal(got.nan_to_num(7.0), clean.nan_to_num(7.0))
+
+
+def test_scale_zero_and_pages_out_of_range():
+    """Every token seen weighs the same; a page outside the cache is nobody's, inside a tile that every row sees whole too."""
+    for form in FORMS:
+        b = Batch([(300, 1), (290, 40)], 8, 2, 64, 16, form, torch.bfloat16, seed=19)
+        b.scale = 0.0
+        b.tables[0, 2], b.tables[1, 5] = -1, b.blocks
+        b.dev["tables"] = b.tables.to(DEV)
+        b.check()
+
+
+@pytest.mark.parametrize("form", FORMS)
 @pytest.mark.parametrize("window,sinks", [(0, 0), (70, 4)])
 def test_longer_prompts(form, window, sinks):
     """Prompt rows past several tiles and column blocks, with a context whose end is inside a page."""

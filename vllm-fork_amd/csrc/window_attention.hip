@@ -11,9 +11,11 @@
 //
 // 8-bit codes become fp16 (every int8 and every e4m3 value is one) and are multiplied with fp16 queries: a bf16 query row is
 // first brought to [2^13, 2^14) by a power of two, which keeps all 8 bits of every element within 2^-28 of the row's
-// largest.  Scales stay outside the products: the 16 tokens of a lane group lie in one block, so K's scale is one factor
-// per lane on the logits and V's one factor per lane on the probabilities, relative to the largest V scale met so far
-// (vref, rescaled like the running maximum) so that fp16 holds them.
+// largest.  K's and V's block scales stay outside the products, for the 16 tokens of a lane group lie in one block.  K's is
+// one factor per lane on the logits.  V's is taken relative to the largest V scale met so far (vref, rescaled like the running
+// maximum), so that fp16 holds it: for decode rows one factor per lane on the probabilities; for prompts a power of two, exact
+// on V's codes, and the rest in [1, 2), which goes into the exponent of the probabilities.  One scale for the whole cache
+// goes into the softmax scale and into the result.  Scales are 0 or more, or NaN.
 #include <limits.h>
 #include <math.h>
 
@@ -44,7 +46,7 @@ struct WindowParams {
   const int32_t* tables;
   const int32_t* seq_lens;
   const int32_t* starts;        // query_start_loc, or null: one row per sequence
-  float* part_o;                // [rows, heads, splits, head] partial sums
+  float* part_o;                // [rows, heads, splits, head] partial sums (`rows` as part_row counts them)
   float* part_ml;               // [rows, heads, splits, 2] their maxima (base 2) and sums
   int64_t out_stride, q_stride;
   int64_t block_stride, head_stride;   // bytes
@@ -56,7 +58,7 @@ struct WindowParams {
   int bs, page_magic;
   int window, sinks;            // window 0: none
   int splits, split_tiles;      // the context in stretches of split_tiles 64-token tiles, at most `splits` of them
-  int part_stride;              // partial sums are laid out for so many stretches
+  int part_rows;                // decode rows: room for so many rows of a sequence (0: rows as they are numbered)
   int col_tiles;                // column tiles of the longest query that this launch serves
   int longest_cols;             // columns of the longest query, at most WA_ROWS_COLS
   int lds_cols;                 // rows kernel: columns of a 16-column tile that any sequence has
@@ -72,6 +74,10 @@ __device__ inline T sload(const T* p) {
 }
 
 // what a sequence's rows [first column, last column] see: sink tokens [0, sink_end) and [low, end), 64 at a time
+__device__ inline int64_t part_row(const WindowParams& p, int seq, int start, int row) {
+  return p.part_rows ? (int64_t)seq * p.part_rows + (row - start) : row;
+}
+
 struct Span {
   int sink_end, low, end, sink_tiles, tiles;
   __device__ inline int base(int i) const { return i < sink_tiles ? 64 * i : low + 64 * (i - sink_tiles); }
@@ -88,7 +94,7 @@ __device__ inline Span span_of(const WindowParams& p, int pos_first, int pos_las
   return s;
 }
 
-enum { KV16 = MI355Q_KV_16, KVF8 = MI355Q_KV_FP8, KVI8 = MI355Q_KV_INT8 };
+enum { KV16 = MI355Q_KV_16, KVF8 = MI355Q_KV_FP8, KVI8 = MI355Q_KV_INT8, KVF8_ONE = 3 };   // (3: one scale for the tensor)
 
 // type of the products
 template <typename DT, int KV>
@@ -199,9 +205,9 @@ __global__ __launch_bounds__(64 * NW, 2) void window_rows_kernel(const WindowPar
 
   const int kvh = blockIdx.x % p.num_kv_heads;
   int b = blockIdx.x / p.num_kv_heads;
-  const int split = b % p.splits;
-  b /= p.splits;
-  const int ct = b % p.col_tiles, seq = b / p.col_tiles;
+  const int ct = b % p.col_tiles;
+  b /= p.col_tiles;
+  const int seq = b % p.num_seqs, split = b / p.num_seqs;   // later stretches, which few sequences reach, last
   const int G = p.group;
 
   const int start = p.starts ? sload(p.starts + seq) : seq;
@@ -433,13 +439,14 @@ __global__ __launch_bounds__(64 * NW, 2) void window_rows_kernel(const WindowPar
     u32x4 pf[NCT][2];
 #pragma unroll
     for (int n = 0; n < NCT; n++) {
-      const float f = KV == KV16 ? qscale[n] : qscale[n] * ks;
+      float f = KV == KV16 ? qscale[n] : qscale[n] * ks;
       uint32_t seen = 0xffffu;
       float x[16], mx = -INFINITY;
 #pragma unroll
       for (int i = 0; i < 16; i++) x[i] = s[n][i >> 2][i & 3];
       if constexpr (INNER) {
         if (ok_tile != 15 && !ok) {
+          f = 1.f;
 #pragma unroll
           for (int i = 0; i < 16; i++) x[i] = -INFINITY;
         }
@@ -570,6 +577,7 @@ __global__ __launch_bounds__(64 * NW, 2) void window_rows_kernel(const WindowPar
 #pragma unroll
   for (int n = 0; n < NCT; n++) {
     l[n] = group_sum(l[n]);
+    if (m[n] == -INFINITY && l[n] != 0.f) m[n] = 0.f;   // every logit was NaN: so is the result, and not a row that sees nothing
     if (g == 0) {
       stat[wave][0][16 * n + col] = m[n];
       stat[wave][1][16 * n + col] = l[n];
@@ -614,7 +622,7 @@ __global__ __launch_bounds__(64 * NW, 2) void window_rows_kernel(const WindowPar
 #pragma unroll
       for (int i = 0; i < PER / 2; i++) out[i] = top == -INFINITY ? 0u : pack2<DT>(v[i >> 1][2 * (i & 1)] * inv, v[i >> 1][2 * (i & 1) + 1] * inv);
     } else {
-      const int64_t to = ((int64_t)orow * p.num_heads + ohead) * p.part_stride + split;
+      const int64_t to = (part_row(p, seq, start, orow) * p.num_heads + ohead) * p.splits + split;
 #pragma unroll
       for (int i = 0; i < PER / 4; i++) *reinterpret_cast<f32x4*>(p.part_o + to * HEAD + d0 + 4 * i) = v[i];
       if (d0 == 0) {
@@ -663,6 +671,8 @@ constexpr float WA_VSHIFT = 128.0f;
 template <typename DT, int KV, int HEAD, int NW>
 __global__ __launch_bounds__(64 * NW, HEAD == 64 ? 4 : 2) void window_flash_kernel(const WindowParams p) {
   typedef typename MathOf<DT, KV>::T MT;
+  constexpr bool SCALED = KV == KVF8 || KV == KVI8;      // a scale for each (block, kv head)
+  constexpr int CODE = KV == KVF8_ONE ? KVF8 : KV;
   constexpr int EB = KV == KV16 ? 2 : 1, NT = 64 * NW, COLS = 32 * NW;
   constexpr int KS = HEAD / 16, DTL = HEAD / 32;
   constexpr int KBYTES = 64 * HEAD * 2, STAGE = 2 * KBYTES;
@@ -672,10 +682,11 @@ __global__ __launch_bounds__(64 * NW, HEAD == 64 ? 4 : 2) void window_flash_kern
   constexpr int LDS = 2 * STAGE > COLS * OLD * 2 ? 2 * STAGE : COLS * OLD * 2;
   static_assert(2 * PIECES % NT == 0, "pieces are shared out evenly");
   constexpr int CHUNK = 64;
+  constexpr int SCALES = SCALED ? 4 * CHUNK : 4;
   struct Chunk {
     u32x4 at[4 * CHUNK];      // per stretch: block offset (64 bits), token offset in the block, tokens somebody sees
-    float ks[4 * CHUNK];
-    float vpow[4 * CHUNK], vlog[4 * CHUNK], vinv[4 * CHUNK];   // V's scale: 2^7 power / vref, log2 and reciprocal of the rest
+    float ks[SCALES];
+    float vpow[SCALES], vlog[SCALES], vinv[SCALES];   // V's scale: 2^7 power / vref, log2 and reciprocal of the rest
     int ok[CHUNK];            // per tile: stretches whose page exists and that begin before the end
     float vref;               // a power of two above every scale so far
   };
@@ -715,6 +726,7 @@ __global__ __launch_bounds__(64 * NW, HEAD == 64 ? 4 : 2) void window_flash_kern
   const int wpos0 = seq_len - qlen + min(wc0, c1) / G, wpos1 = seq_len - qlen + min(wc0 + 31, c1) / G;
   u32x4 qf[KS];
   float qscale = fabsf(p.scale) * WA_LOG2E;
+  if constexpr (KV == KVF8_ONE) qscale *= *p.ks;
   {
     const uint16_t* qp = p.q + (int64_t)row * p.q_stride + (int64_t)head * HEAD + 8 * half;
 #pragma unroll
@@ -781,7 +793,7 @@ __global__ __launch_bounds__(64 * NW, HEAD == 64 ? 4 : 2) void window_flash_kern
       if (!in) seen = 0;
       const uint64_t ok = __ballot(in && t < lim);
       v[i] = 0.f;
-      if constexpr (KV != KV16) {
+      if constexpr (SCALED) {
         const int64_t si = at * p.scale_block_stride + kvh * p.scale_head_stride;
         ch.ks[n] = in ? p.ks[si] : 1.f;
         v[i] = seen ? p.vs[si] : 0.f;
@@ -791,7 +803,7 @@ __global__ __launch_bounds__(64 * NW, HEAD == 64 ? 4 : 2) void window_flash_kern
       ch.at[n] = u32x4{(uint32_t)byte, (uint32_t)(byte >> 32), (uint32_t)((n16 - pg * blocks16) * 16), seen};
       if (j == 0) ch.ok[n >> 2] = (int)(ok >> (lane & ~3)) & 15;
     }
-    if constexpr (KV != KV16) {
+    if constexpr (SCALED) {
       top = wave_max(top);
       top = top > 0.f ? __uint_as_float((__float_as_uint(fminf(top, 0x1p125f)) & 0x7f800000u) + 0x00800000u) : 0.f;
       if (first > begin) top = fmaxf(top, chunks[((first - begin) / CHUNK & 1) ^ 1].vref);   // never falls
@@ -852,8 +864,8 @@ __global__ __launch_bounds__(64 * NW, HEAD == 64 ? 4 : 2) void window_flash_kern
       const int ch = (g0 + i) % GPJ * 4 + (lane >> 4);      // 16-byte chunk of the head
       if constexpr (EB == 1) {
         unsigned char* at = to + (((jw >> 1) * KS + ch) * 64 + rho) * 16;
-        *reinterpret_cast<u32x4*>(at) = widen8<KV>(w, 0);
-        *reinterpret_cast<u32x4*>(at + 512) = widen8<KV>(w, 1);
+        *reinterpret_cast<u32x4*>(at) = widen8<CODE>(w, 0);
+        *reinterpret_cast<u32x4*>(at + 512) = widen8<CODE>(w, 1);
       } else {
         *reinterpret_cast<u32x4*>(to + (((jw >> 1) * KS + (ch >> 1)) * 64 + (ch & 1) * 32 + rho) * 16) = w;
       }
@@ -866,16 +878,18 @@ __global__ __launch_bounds__(64 * NW, HEAD == 64 ? 4 : 2) void window_flash_kern
       const uint32_t seen = __builtin_amdgcn_readfirstlane(chunk_of(n).at[e0][3]);
       u32x4 v[EB == 1 ? 2 : 1];
       if constexpr (EB == 1) {
-        const _Float16 r16 = (_Float16)chunk_of(n).vpow[e0];
-        const wa_f16x2 rr = {r16, r16};
+        v[0] = widen8<CODE>(w, 0);
+        v[1] = widen8<CODE>(w, 1);
+        if constexpr (SCALED) {
+          const _Float16 r16 = (_Float16)chunk_of(n).vpow[e0];
+          const wa_f16x2 rr = {r16, r16};
 #pragma unroll
-        for (int h = 0; h < 2; h++) {
-          v[h] = widen8<KV>(w, h);
+          for (int h = 0; h < 2; h++)
 #pragma unroll
-          for (int e = 0; e < 4; e++) {
-            const uint32_t x = v[h][e];   // (a bit cast of the vector element itself would take element 0)
-            v[h][e] = __builtin_bit_cast(uint32_t, __builtin_bit_cast(wa_f16x2, x) * rr);
-          }
+            for (int e = 0; e < 4; e++) {
+              const uint32_t x = v[h][e];   // (a bit cast of the vector element itself would take element 0)
+              v[h][e] = __builtin_bit_cast(uint32_t, __builtin_bit_cast(wa_f16x2, x) * rr);
+            }
         }
       } else {
         v[0] = w;
@@ -965,7 +979,7 @@ __global__ __launch_bounds__(64 * NW, HEAD == 64 ? 4 : 2) void window_flash_kern
       __builtin_amdgcn_sched_group_barrier(0x008, 6, 0);
     }
     float f[4];
-    if constexpr (KV == KV16) {
+    if constexpr (!SCALED) {
 #pragma unroll
       for (int j = 0; j < 4; j++) f[j] = qscale;
     } else {
@@ -1015,12 +1029,12 @@ __global__ __launch_bounds__(64 * NW, HEAD == 64 ? 4 : 2) void window_flash_kern
       mx = fmaxf(mx, INNER ? a * f[j] : a);
     }
     mx = pair_max(mx);
-    const float vref_tile = KV == KV16 ? 0.f : ch.vref;
-    if (__any(mx > m + WA_LAG) || (KV != KV16 && __any(vref_tile > oref))) {
+    const float vref_tile = SCALED ? ch.vref : 0.f;
+    if (__any(mx > m + WA_LAG) || (SCALED && __any(vref_tile > oref))) {
       const float mn = mx > m + WA_LAG ? mx : m;
       float a = m == -INFINITY ? 0.f : exp2_fast(m - mn);
       l *= a;
-      if constexpr (KV != KV16) {
+      if constexpr (SCALED) {
         if (vref_tile > oref) a *= oref / vref_tile, oref = vref_tile;
       }
 #pragma unroll
@@ -1029,7 +1043,7 @@ __global__ __launch_bounds__(64 * NW, HEAD == 64 ? 4 : 2) void window_flash_kern
     }
     const float ms = (m == -INFINITY ? 0.f : m) - WA_SHIFT;
     f32x4 plus = {-ms, -ms, -ms, -ms}, less = {1.f, 1.f, 1.f, 1.f};
-    if constexpr (KV != KV16) {
+    if constexpr (SCALED) {
       plus += *reinterpret_cast<const f32x4*>(&ch.vlog[n % CHUNK * 4]);
       less = *reinterpret_cast<const f32x4*>(&ch.vinv[n % CHUNK * 4]);
     }
@@ -1050,7 +1064,7 @@ __global__ __launch_bounds__(64 * NW, HEAD == 64 ? 4 : 2) void window_flash_kern
         pf[j][e] = pack_p<MT>(s[j >> 1][8 * (j & 1) + 2 * e], s[j >> 1][8 * (j & 1) + 2 * e + 1]);
         sum = add_pair<MT>(pf[j][e], sum);
       }
-      l = KV == KV16 ? l + sum : __builtin_fmaf(sum, less[j], l);
+      l = SCALED ? __builtin_fmaf(sum, less[j], l) : l + sum;
     }
 
     // ---- O^T += V^T P^T -------------------------------------------------------------------------------------------------
@@ -1092,7 +1106,8 @@ __global__ __launch_bounds__(64 * NW, HEAD == 64 ? 4 : 2) void window_flash_kern
 
   // ---- out ----------------------------------------------------------------------------------------------------------------
   l = pair_sum(l);
-  const float unit = KV == KV16 ? 1.f : oref / WA_VSHIFT;
+  if (m == -INFINITY && l != 0.f) m = 0.f;   // every logit was NaN: so is the result, and not a row that sees nothing
+  const float unit = SCALED ? oref / WA_VSHIFT : KV == KVF8_ONE ? *p.vs : 1.f;
   if (whole) {
     arrive();               // the last tile has been read by every wave: LDS takes the output rows
     const float inv = m == -INFINITY ? 0.f : unit / l;
@@ -1121,7 +1136,7 @@ __global__ __launch_bounds__(64 * NW, HEAD == 64 ? 4 : 2) void window_flash_kern
         for (int e = 0; e < 4; e++) reinterpret_cast<uint32_t*>(to)[e] = w[e];
     }
   } else if (wc0 + col <= wc1) {
-    const int64_t at = ((int64_t)row * p.num_heads + head) * p.part_stride + split;
+    const int64_t at = (part_row(p, seq, start, row) * p.num_heads + head) * p.splits + split;
     float* to = p.part_o + at * HEAD + 4 * half;
 #pragma unroll
     for (int d = 0; d < DTL; d++)
@@ -1150,15 +1165,15 @@ __global__ __launch_bounds__(256) void window_merge_kernel(const WindowParams p,
   const int kvh = b % p.num_kv_heads, seq = b / p.num_kv_heads;
   const int start = p.starts ? sload(p.starts + seq) : seq;
   const int qlen = p.starts ? sload(p.starts + seq + 1) - start : 1;
-  const int cols = min(qlen, p.num_rows - start) * p.group;
-  if (start < 0 || c >= cols || cols < p.min_cols || cols > p.max_cols) return;
+  const int all = min(qlen, p.num_rows - start) * p.group, cols = p.part_rows ? min(all, p.longest_cols) : all;
+  if (start < 0 || c >= cols || cols < p.min_cols || all > p.max_cols) return;
   const int seq_len = sload(p.seq_lens + seq);
   const int c0 = c / COLS * COLS, c1 = min(c0 + COLS, cols) - 1;
   const Span span = span_of(p, seq_len - qlen + c0 / p.group, seq_len - qlen + c1 / p.group);
   if (span.tiles <= p.split_tiles) return;    // written by its only workgroup
   const int n = min(p.splits, (span.tiles + p.split_tiles - 1) / p.split_tiles);
   const int row = start + c / p.group, head = kvh * p.group + c % p.group;
-  const int64_t at = ((int64_t)row * p.num_heads + head) * p.part_stride;
+  const int64_t at = (part_row(p, seq, start, row) * p.num_heads + head) * p.splits;
   const float* ml = p.part_ml + 2 * at;
   const float* po = p.part_o + at * HEAD + lane * PER;
   float top = -INFINITY;
@@ -1173,7 +1188,10 @@ __global__ __launch_bounds__(256) void window_merge_kernel(const WindowParams p,
     const float w = mi == -INFINITY ? 0.f : exp2_fast(mi - top);
     sum += ml[2 * i + 1] * w;
 #pragma unroll
-    for (int j = 0; j < PER; j++) v[j] += po[(int64_t)i * HEAD + j] * w;
+    for (int j = 0; j < PER; j++) {
+      const float x = po[(int64_t)i * HEAD + j] * w;
+      v[j] += mi == -INFINITY ? 0.f : x;   // (a stretch of which nothing is seen, whatever its scales)
+    }
   }
   uint16_t* out = p.out + (int64_t)row * p.out_stride + (int64_t)head * HEAD + lane * PER;
 #pragma unroll
@@ -1187,7 +1205,6 @@ struct WindowPart { int cols, waves, col_tiles, splits, split_tiles; };
 struct WindowPlan {
   WindowPart rows, flash;       // col_tiles 0: not launched
   bool all_flash;               // sequences of few rows too
-  int part_stride;
 };
 
 // columns (rows x heads per kv head) up to which a sequence is served 16 or 32 at a time
@@ -1226,7 +1243,13 @@ static WindowPlan window_plan(int num_seqs, int num_rows, int num_heads, int num
     const int64_t tiles = window_tiles(w.rows.cols, G, max_seq_len, window, sinks);
     const int64_t groups = (int64_t)num_seqs * num_kv_heads * w.rows.col_tiles;
     w.rows.waves = groups <= 256 || w.rows.cols == 32 ? 8 : 4;
-    window_cut(w.rows, tiles, groups <= 256 ? 256 / groups : (2048 + groups - 1) / groups, (tiles <= 4 * w.rows.waves ? 4 : 2) * w.rows.waves);
+    // One workgroup to a CU is what up to 64 of them are cut into.  More (9 sequences of 8 kv heads) fill the chip by
+    // themselves, but lengths differ: contexts are cut into stretches of 4096 tokens, 32 at most.  Against no cut: one context of
+    // 131072 among 31 of 2000 701 -> 171 us, 16 / 32 / 64 contexts spread from 1000 to 30000 132 -> 125, 258 -> 228, 465 -> 427,
+    // 32 of 16384 each 201 -> 211; contexts up to 4096 under a bound of 131072 70 -> 76 (156 with a sequence's stretches
+    // side by side in the grid).  Contexts up to 4096 are not cut: 64 of them in four stretches took 84 us, whole 71.
+    const int64_t stretches = groups <= 64 ? 256 / groups : std::max<int64_t>(256 / groups, std::min<int64_t>((tiles + 63) / 64, 32));
+    window_cut(w.rows, tiles, stretches, (tiles <= 4 * w.rows.waves ? 4 : 2) * w.rows.waves);
   }
   if (prompts) {
     w.flash.cols = WA_FLASH_COLS;
@@ -1235,16 +1258,23 @@ static WindowPlan window_plan(int num_seqs, int num_rows, int num_heads, int num
     const int64_t groups = (int64_t)num_seqs * num_kv_heads * w.flash.col_tiles;
     window_cut(w.flash, flash_tiles, std::max<int64_t>(1, (256 + groups - 1) / groups), 16);
   }
-  w.part_stride = std::max(w.rows.splits, w.flash.splits);
   return w;
 }
 
-static size_t window_workspace(const WindowPlan& w, int num_rows, int num_heads, int head_size) {
-  return w.part_stride <= 1 ? 0 : (size_t)num_rows * num_heads * w.part_stride * (head_size + 2) * sizeof(float);
+// rows of a sequence that the decode kernel may meet
+static int window_part_rows(int max_query_len, int G) {
+  return (int)((std::min<int64_t>((int64_t)max_query_len * G, WA_ROWS_COLS) + G - 1) / G);
+}
+
+// floats of the partial sums' outputs (maxima and sums follow); the two kinds of row take turns with them
+static int64_t window_partials(const WindowPlan& w, int num_seqs, int num_rows, int num_heads, int num_kv_heads, int max_query_len) {
+  const int64_t rows = w.rows.splits > 1 ? (int64_t)num_seqs * window_part_rows(max_query_len, num_heads / num_kv_heads) * w.rows.splits : 0;
+  const int64_t flash = w.flash.splits > 1 ? (int64_t)num_rows * w.flash.splits : 0;
+  return std::max(rows, flash) * num_heads;
 }
 
 template <typename DT, int KV, int HEAD>
-static int launch_window(WindowParams p, const WindowPlan& w, hipStream_t s) {
+static int launch_window(WindowParams p, const WindowPlan& w, int part_rows, hipStream_t s) {
   auto groups = [&](const WindowPart& a) { return (int64_t)p.num_seqs * p.num_kv_heads * a.col_tiles * a.splits; };
   auto merges = [&](const WindowPart& a) { return (int64_t)p.num_seqs * p.num_kv_heads * a.col_tiles * (a.cols / 4); };
   const int64_t most = (int64_t)1 << 31;
@@ -1255,13 +1285,19 @@ static int launch_window(WindowParams p, const WindowPlan& w, hipStream_t s) {
     if (!a.col_tiles) continue;
     p.col_tiles = a.col_tiles, p.splits = a.splits;
     p.split_tiles = a.splits == 1 ? INT_MAX : a.split_tiles;
+    p.part_rows = kind ? 0 : part_rows;
     p.min_cols = kind && !w.all_flash ? WA_ROWS_COLS + 1 : 0;
     p.max_cols = kind ? INT_MAX : WA_ROWS_COLS;
     p.lds_cols = std::min(16, p.longest_cols);
     const dim3 grid((unsigned)groups(a)), wg(64 * a.waves);
     const size_t lds = (size_t)a.waves * p.lds_cols * (HEAD + 4) * sizeof(float);
     if (kind) {
-      hipLaunchKernelGGL((window_flash_kernel<DT, KV, HEAD, WA_WAVES>), grid, wg, 0, s, p);
+      // One scale for the whole cache goes into the logits' factor and the result's: no scales are read, no codes multiplied.
+      // Prompts of 2047 rows and less on 64-wide heads behind a window of 512: 57.1 us as block scales, 47.0 us so.
+      if (KV == KVF8 && p.scale_block_stride == 0 && p.scale_head_stride == 0)
+        hipLaunchKernelGGL((window_flash_kernel<DT, KV == KVF8 ? KVF8_ONE : KV, HEAD, WA_WAVES>), grid, wg, 0, s, p);
+      else
+        hipLaunchKernelGGL((window_flash_kernel<DT, KV, HEAD, WA_WAVES>), grid, wg, 0, s, p);
     } else if (a.cols == 32) {
       if constexpr (KV != KV16) hipLaunchKernelGGL((window_rows_kernel<DT, KV, HEAD, 2, 8>), grid, wg, lds, s, p);
     } else if (a.waves == 8) {
@@ -1285,8 +1321,8 @@ using namespace mi355q;
 extern "C" size_t mi355q_paged_window_attention_workspace_bytes(int num_seqs, int num_rows, int num_heads, int num_kv_heads, int head_size,
                                                                 int max_query_len, int max_seq_len, int window, int sinks, int kv_type) {
   if (num_seqs <= 0 || num_rows <= 0 || num_kv_heads <= 0 || num_heads <= 0 || max_query_len <= 0 || max_seq_len <= 0) return 0;
-  return window_workspace(window_plan(num_seqs, num_rows, num_heads, num_kv_heads, kv_type, max_query_len, max_seq_len, window, sinks), num_rows, num_heads,
-                          head_size);
+  const WindowPlan w = window_plan(num_seqs, num_rows, num_heads, num_kv_heads, kv_type, max_query_len, max_seq_len, window, sinks);
+  return (size_t)window_partials(w, num_seqs, num_rows, num_heads, num_kv_heads, max_query_len) * (head_size + 2) * sizeof(float);
 }
 
 extern "C" int mi355q_paged_window_attention(void* out, int64_t out_stride, const void* query, int64_t q_stride, const void* key_cache,
@@ -1319,7 +1355,8 @@ extern "C" int mi355q_paged_window_attention(void* out, int64_t out_stride, cons
                  "paged_window_attention: caches and query rows must be 16-byte aligned");
   MI355Q_REQUIRE(((uintptr_t)out & 3) == 0 && out_stride % 2 == 0, "paged_window_attention: output rows must be 4-byte aligned");
   const WindowPlan w = window_plan(num_seqs, num_rows, num_heads, num_kv_heads, kv_type, max_query_len, max_seq_len, window, sinks);
-  const size_t need = window_workspace(w, num_rows, num_heads, head_size);
+  const int64_t partials = window_partials(w, num_seqs, num_rows, num_heads, num_kv_heads, max_query_len);
+  const size_t need = (size_t)partials * (head_size + 2) * sizeof(float);
   if (need && (!workspace || workspace_bytes < need))
     return set_error(MI355Q_ENOSPACE, "paged_window_attention: workspace of %zu bytes, %zu needed", workspace ? workspace_bytes : (size_t)0, need);
   MI355Q_REQUIRE(!need || ((uintptr_t)workspace & 15) == 0, "paged_window_attention: workspace must be 16-byte aligned");
@@ -1331,7 +1368,7 @@ extern "C" int mi355q_paged_window_attention(void* out, int64_t out_stride, cons
   p.ks = k_scale, p.vs = v_scale;
   p.tables = block_tables, p.seq_lens = seq_lens, p.starts = query_start_loc;
   p.part_o = (float*)workspace;
-  p.part_ml = (float*)workspace + (size_t)num_rows * num_heads * w.part_stride * head_size;
+  p.part_ml = (float*)workspace + partials * head_size;
   p.out_stride = out_stride, p.q_stride = q_stride;
   p.block_stride = kv_block_stride * eb, p.head_stride = kv_head_stride * eb;
   p.scale_block_stride = scale_block_stride, p.scale_head_stride = scale_head_stride;
@@ -1342,13 +1379,13 @@ extern "C" int mi355q_paged_window_attention(void* out, int64_t out_stride, cons
   const int pieces = block_size / 16;
   p.page_magic = pieces == 1 ? 0 : (int)(((1ull << 32) + pieces - 1) / pieces);
   p.window = std::min(window, 1 << 30), p.sinks = sinks;
-  p.part_stride = w.part_stride;
+  const int part_rows = window_part_rows(max_query_len, p.group);
   p.longest_cols = (int)std::min<int64_t>((int64_t)max_query_len * p.group, WA_ROWS_COLS);
   p.out16 = ((uintptr_t)out & 15) == 0 && out_stride % 8 == 0;
   hipStream_t s = (hipStream_t)stream;
 #define BY_KV(DT, HD)                                                                                                     \
-  (kv_type == MI355Q_KV_16 ? launch_window<DT, KV16, HD>(p, w, s)                                                        \
-                           : kv_type == MI355Q_KV_FP8 ? launch_window<DT, KVF8, HD>(p, w, s) : launch_window<DT, KVI8, HD>(p, w, s))
+  (kv_type == MI355Q_KV_16 ? launch_window<DT, KV16, HD>(p, w, part_rows, s)                                                        \
+                           : kv_type == MI355Q_KV_FP8 ? launch_window<DT, KVF8, HD>(p, w, part_rows, s) : launch_window<DT, KVI8, HD>(p, w, part_rows, s))
   if (dtype == MI355Q_BF16) return head_size == 128 ? BY_KV(BF16, 128) : BY_KV(BF16, 64);
   return head_size == 128 ? BY_KV(FP16, 128) : BY_KV(FP16, 64);
 #undef BY_KV
