@@ -474,6 +474,22 @@ def test_one_long_context_among_many_short_ones(form):
         b.check(b.run(max_query_len=n + 20))
 
 
+@pytest.mark.parametrize("form", FORMS)
+@pytest.mark.parametrize("window", [0, 100])
+def test_prompts_among_many_sequences(form, window):
+    """Prompts find their rows in batches of more sequences than a wave has lanes; sequences without rows among them."""
+    for long in (150, 2500):
+        lens = [(5 * i % 90, 1) for i in range(140)]
+        for at, prompt in ((0, (0, 65)), (3, (long, 33)), (63, (10, 90)), (64, (0, 129)), (66, (20, 0)), (128, (7, 64)), (139, (60, 40))):
+            lens[at] = prompt
+        b = Batch(lens, 8, 2, 64, 16, form, torch.float16, window=window, sinks=3 if window else 0, seed=20)
+        b.check()
+        b.seq_lens = torch.cat([b.seq_lens, torch.zeros(60, dtype=torch.int32, device=DEV)])       # a batch padded with empty sequences
+        b.starts = torch.cat([b.starts, torch.full((60,), b.rows, dtype=torch.int32, device=DEV)])
+        b.dev["tables"] = torch.cat([b.dev["tables"], torch.zeros(60, b.tables.shape[1], dtype=torch.int32, device=DEV)])
+        b.check()
+
+
 def test_one_scale_that_is_no_number():
     """Rows that see nothing stay zero whatever the scale is."""
     b = Batch([(0, 3), (20, 2), (0, 300)], 4, 2, 64, 16, "fp8", torch.bfloat16, seed=17)

@@ -36,6 +36,9 @@ constexpr float WA_LOG2E = 1.44269504088896f;
 // few tokens carry a row, their rounding cancels.
 constexpr float WA_SHIFT = 6.0f, WA_LAG = 8.0f;
 
+// The prompt kernel: 8 waves of 32 columns.
+constexpr int WA_WAVES = 8, WA_FLASH_COLS = 32 * WA_WAVES;
+
 struct WindowParams {
   uint16_t* out;
   const uint16_t* q;
@@ -59,7 +62,7 @@ struct WindowParams {
   int window, sinks;            // window 0: none
   int splits, split_tiles;      // the context in stretches of split_tiles 64-token tiles, at most `splits` of them
   int part_rows;                // decode rows: room for so many rows of a sequence (0: rows as they are numbered)
-  int col_tiles;                // column tiles of the longest query that this launch serves
+  int col_tiles;                // decode rows: column tiles of the longest query
   int longest_cols;             // columns of the longest query, at most WA_ROWS_COLS
   int lds_cols;                 // rows kernel: columns of a 16-column tile that any sequence has
   int min_cols, max_cols;       // sequences with fewer or more columns (rows x heads per kv head) are another launch's
@@ -74,6 +77,37 @@ __device__ inline T sload(const T* p) {
 }
 
 // what a sequence's rows [first column, last column] see: sink tokens [0, sink_end) and [low, end), 64 at a time
+// Prompt rows: column tile `slot` of the batch, counted over the sequences that have any (seq < 0: there are fewer).  The grid
+// is as large as num_rows allows, not sequences times the longest: every wave counts for itself, a sequence per lane.
+struct Slot { int seq, ct, start, qlen; };
+template <int COLS>
+__device__ inline Slot slot_of(const WindowParams& p, int slot) {
+  const int lane = threadIdx.x & 63;
+  auto first_row = [&](int s) { return p.starts ? p.starts[min(s, p.num_seqs)] : min(s, p.num_seqs); };
+  int from = first_row(lane), to = first_row(lane + 1);
+  for (int s0 = 0; s0 < p.num_seqs; s0 += 64) {
+    const int start = from, qlen = to - from;
+    if (s0 + 64 < p.num_seqs) from = first_row(s0 + 64 + lane), to = first_row(s0 + 65 + lane);   // on their way meanwhile
+    const int cols = min(qlen, p.num_rows - start) * p.group;
+    const int n = start < 0 || cols < p.min_cols ? 0 : (max(cols, 0) + COLS - 1) / COLS;
+    int upto = n;
+#pragma unroll
+    for (int d = 1; d < 64; d *= 2) {
+      const int x = __shfl_up(upto, d, 64);
+      upto += lane >= d ? x : 0;
+    }
+    const uint64_t past = __ballot(upto > slot);
+    if (past) {
+      const int l = __builtin_ctzll(past);
+      const int end = __builtin_amdgcn_readlane(upto, l);
+      // a sequence's last rows, which see most under the causal mask, first
+      return {s0 + l, end - 1 - slot, __builtin_amdgcn_readlane(start, l), __builtin_amdgcn_readlane(qlen, l)};
+    }
+    slot -= __builtin_amdgcn_readlane(upto, 63);
+  }
+  return {-1, 0, 0, 0};
+}
+
 __device__ inline int64_t part_row(const WindowParams& p, int seq, int start, int row) {
   return p.part_rows ? (int64_t)seq * p.part_rows + (row - start) : row;
 }
@@ -205,9 +239,9 @@ __global__ __launch_bounds__(64 * NW, 2) void window_rows_kernel(const WindowPar
 
   const int kvh = blockIdx.x % p.num_kv_heads;
   int b = blockIdx.x / p.num_kv_heads;
-  const int ct = b % p.col_tiles;
-  b /= p.col_tiles;
-  const int seq = b % p.num_seqs, split = b / p.num_seqs;   // later stretches, which few sequences reach, last
+  const int seq = b % p.num_seqs;
+  b /= p.num_seqs;
+  const int split = b % p.splits, ct = b / p.splits;   // what few sequences have, stretches and column tiles, last
   const int G = p.group;
 
   const int start = p.starts ? sload(p.starts + seq) : seq;
@@ -700,14 +734,11 @@ __global__ __launch_bounds__(64 * NW, HEAD == 64 ? 4 : 2) void window_flash_kern
   const int kvh = blockIdx.x % p.num_kv_heads;
   int b = blockIdx.x / p.num_kv_heads;
   const int split = b % p.splits;
-  b /= p.splits;
-  // a sequence's last rows, which see most under the causal mask, first
-  const int ct = p.col_tiles - 1 - b % p.col_tiles, seq = b / p.col_tiles;
+  const Slot slot = slot_of<COLS>(p, b / p.splits);
+  if (slot.seq < 0) return;
+  const int seq = slot.seq, ct = slot.ct, start = slot.start, qlen = slot.qlen;
   const int G = p.group;
-  const int start = p.starts ? sload(p.starts + seq) : seq;
-  const int qlen = p.starts ? sload(p.starts + seq + 1) - start : 1;
   const int cols = min(qlen, p.num_rows - start) * G;
-  if (start < 0 || ct * COLS >= cols || cols < p.min_cols) return;
   const int seq_len = sload(p.seq_lens + seq);
   const int c0 = ct * COLS, c1 = min(c0 + COLS, cols) - 1;
   const int pos0 = seq_len - qlen + c0 / G, pos1 = seq_len - qlen + c1 / G;
@@ -1152,21 +1183,32 @@ __global__ __launch_bounds__(64 * NW, HEAD == 64 ? 4 : 2) void window_flash_kern
 }
 
 // Joins the stretches of a long context: one wave per column (query row and head).  COLS: columns of a workgroup of the
-// launch before, whose span decides how many stretches there are.
-template <typename DT, int HEAD>
-__global__ __launch_bounds__(256) void window_merge_kernel(const WindowParams p, int COLS) {
+// launch before, whose span decides how many stretches there are and which row they belong to.
+template <typename DT, int HEAD, int COLS>
+__global__ __launch_bounds__(256) void window_merge_kernel(const WindowParams p) {
+  constexpr bool FLASH = COLS == WA_FLASH_COLS;
   constexpr int PER = HEAD / 64;
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  int b = blockIdx.x;
-  const int per_seq = p.col_tiles * COLS / 4;
-  const int c = (b % per_seq) * 4 + wave;
-  b /= per_seq;
-  const int kvh = b % p.num_kv_heads, seq = b / p.num_kv_heads;
-  const int start = p.starts ? sload(p.starts + seq) : seq;
-  const int qlen = p.starts ? sload(p.starts + seq + 1) - start : 1;
-  const int all = min(qlen, p.num_rows - start) * p.group, cols = p.part_rows ? min(all, p.longest_cols) : all;
-  if (start < 0 || c >= cols || cols < p.min_cols || all > p.max_cols) return;
+  int b = blockIdx.x, c, kvh, seq, start, qlen;
+  if (FLASH) {
+    c = b % (COLS / 4) * 4 + wave;
+    b /= COLS / 4;
+    kvh = b % p.num_kv_heads;
+    const Slot slot = slot_of<COLS>(p, b / p.num_kv_heads);
+    if (slot.seq < 0) return;
+    seq = slot.seq, start = slot.start, qlen = slot.qlen;
+    c += slot.ct * COLS;
+  } else {
+    const int per_seq = p.col_tiles * COLS / 4;
+    c = (b % per_seq) * 4 + wave;
+    b /= per_seq;
+    kvh = b % p.num_kv_heads, seq = b / p.num_kv_heads;
+    start = p.starts ? sload(p.starts + seq) : seq;
+    qlen = p.starts ? sload(p.starts + seq + 1) - start : 1;
+  }
+  const int all = min(qlen, p.num_rows - start) * p.group, cols = FLASH ? all : min(all, p.longest_cols);
+  if (start < 0 || c >= cols || all > p.max_cols) return;
   const int seq_len = sload(p.seq_lens + seq);
   const int c0 = c / COLS * COLS, c1 = min(c0 + COLS, cols) - 1;
   const Span span = span_of(p, seq_len - qlen + c0 / p.group, seq_len - qlen + c1 / p.group);
@@ -1201,15 +1243,15 @@ __global__ __launch_bounds__(256) void window_merge_kernel(const WindowParams p,
 // ---------------------------------------------------------------------------------------------------------------------
 // how a call is cut: host side, from what the caller bounds
 // ---------------------------------------------------------------------------------------------------------------------
-struct WindowPart { int cols, waves, col_tiles, splits, split_tiles; };
+struct WindowPart { int cols, waves, col_tiles, splits, split_tiles; };   // col_tiles: of a sequence (rows), of the batch (flash)
 struct WindowPlan {
   WindowPart rows, flash;       // col_tiles 0: not launched
   bool all_flash;               // sequences of few rows too
+  int row_cols;                 // sequences of more columns are prompts
 };
 
 // columns (rows x heads per kv head) up to which a sequence is served 16 or 32 at a time
 constexpr int WA_ROWS_COLS = 64;
-constexpr int WA_WAVES = 8, WA_FLASH_COLS = 32 * WA_WAVES;
 
 // 64-token tiles that `cols` columns see at most: the window of their first row, their own rows, an unaligned start, the sinks
 static int64_t window_tiles(int cols, int G, int max_seq_len, int window, int sinks) {
@@ -1231,52 +1273,68 @@ static WindowPlan window_plan(int num_seqs, int num_rows, int num_heads, int num
   const int64_t cols = (int64_t)max_query_len * G;
   const bool prompts = cols > WA_ROWS_COLS;
   const int64_t flash_tiles = window_tiles(WA_FLASH_COLS, G, max_seq_len, window, sinks);
-  // Decode rows between prompts go to the rows kernel, unless no context is longer than 32 tiles: a workgroup of the prompt
-  // kernel then walks it while the prompts' own run, which costs less than a launch (57 -> 47 us for five sequences under a
-  // window of 512), or the bounds say that every sequence has max_query_len rows.
-  w.all_flash = prompts && (flash_tiles <= 32 || (int64_t)num_seqs * max_query_len == num_rows);
+  // Next to prompts the decode kernel takes rows of up to 16 columns, which is one query each, and drafts go with the prompts:
+  // 200 decode rows and a prompt of 1800 354 -> 265 us, 64 drafts of five rows and one of 1500 204 -> 183.  Not over contexts
+  // past 8192, which a workgroup of the prompt kernel walks whole (one draft at 30000 679 us, with the decode kernel 149).
+  w.row_cols = prompts && flash_tiles <= 128 ? 16 : WA_ROWS_COLS;
+  // Decode rows between prompts have the decode kernel, unless they are few and no context is longer than 32 tiles: workgroups
+  // of the prompt kernel then walk them while the prompts' own run, which costs less than a launch (five sequences under a
+  // window of 512 50 us, apart 57; eight decode rows and two prompts 45 and 54; but 30 rows and a prompt 44 and 43, 100 rows 57 and
+  // 40, 200 rows of 1500 tokens 202 and 109).  And the bounds may say that every sequence has max_query_len rows.
+  w.all_flash = prompts && ((flash_tiles <= 32 && (int64_t)num_seqs * num_kv_heads <= 128) || (int64_t)num_seqs * max_query_len == num_rows);
   if (!w.all_flash) {
-    const int64_t mine = std::min<int64_t>(cols, WA_ROWS_COLS);
-    // 32 columns to a workgroup read a draft's K and V once instead of twice; a 16-bit tile leaves no registers for it
-    w.rows.cols = mine > 16 && kv_type != MI355Q_KV_16 ? 32 : 16;
+    const int64_t mine = std::min<int64_t>(cols, w.row_cols);
+    // 32 columns to a workgroup read a draft's K and V once instead of twice; a 16-bit tile leaves no registers for it, and next to
+    // prompts most sequences have one row
+    w.rows.cols = !prompts && mine > 16 && kv_type != MI355Q_KV_16 ? 32 : 16;
     w.rows.col_tiles = (int)((mine + w.rows.cols - 1) / w.rows.cols);
     const int64_t tiles = window_tiles(w.rows.cols, G, max_seq_len, window, sinks);
     const int64_t groups = (int64_t)num_seqs * num_kv_heads * w.rows.col_tiles;
     w.rows.waves = groups <= 256 || w.rows.cols == 32 ? 8 : 4;
     // One workgroup to a CU is what up to 64 of them are cut into.  More (9 sequences of 8 kv heads) fill the chip by
-    // themselves, but lengths differ: contexts are cut into stretches of 4096 tokens, 32 at most.  Against no cut: one context of
+    // themselves, but lengths differ: contexts are cut into stretches of 4096 tokens and more, 32 at
+    // most, and fewer of more sequences (their sums take room).  Against no cut: one context of
     // 131072 among 31 of 2000 701 -> 171 us, 16 / 32 / 64 contexts spread from 1000 to 30000 132 -> 125, 258 -> 228, 465 -> 427,
     // 32 of 16384 each 201 -> 211; contexts up to 4096 under a bound of 131072 70 -> 76 (156 with a sequence's stretches
-    // side by side in the grid).  Contexts up to 4096 are not cut: 64 of them in four stretches took 84 us, whole 71.
-    const int64_t stretches = groups <= 64 ? 256 / groups : std::max<int64_t>(256 / groups, std::min<int64_t>((tiles + 63) / 64, 32));
+    // side by side in the grid).  What is shorter than two stretches stays whole: 64 contexts up to 4096 in four stretches took 84 us,
+    // whole 71; 32 decode rows under a window of 4096 in two 91, whole 84.
+    const int64_t stretches = groups <= 64 ? 256 / groups : std::max<int64_t>(256 / groups, std::clamp<int64_t>(std::min(tiles / 64, 16384 / groups), 1, 32));
     window_cut(w.rows, tiles, stretches, (tiles <= 4 * w.rows.waves ? 4 : 2) * w.rows.waves);
   }
   if (prompts) {
-    w.flash.cols = WA_FLASH_COLS;
-    w.flash.waves = WA_WAVES;
-    w.flash.col_tiles = (int)((cols + WA_FLASH_COLS - 1) / WA_FLASH_COLS);
-    const int64_t groups = (int64_t)num_seqs * num_kv_heads * w.flash.col_tiles;
-    window_cut(w.flash, flash_tiles, std::max<int64_t>(1, (256 + groups - 1) / groups), 16);
+    // Column tiles of the whole batch at most.  (Sequences times the longest one's tiles were 445 us for 200 decode rows and
+    // a prompt of 1800, against 354.)
+    const int64_t all = (int64_t)num_rows * G, least = w.all_flash ? 1 : w.row_cols + 1;
+    const int64_t tiles = std::min(num_seqs * ((cols + WA_FLASH_COLS - 1) / WA_FLASH_COLS), all / WA_FLASH_COLS + std::min<int64_t>(num_seqs, all / least));
+    if (tiles > 0) {              // (0: fewer rows than a prompt has)
+      w.flash.cols = WA_FLASH_COLS;
+      w.flash.waves = WA_WAVES;
+      w.flash.col_tiles = (int)tiles;
+      window_cut(w.flash, flash_tiles, std::max<int64_t>(1, (256 + num_kv_heads * tiles - 1) / (num_kv_heads * tiles)), 16);
+    }
   }
   return w;
 }
 
-// rows of a sequence that the decode kernel may meet
-static int window_part_rows(int max_query_len, int G) {
-  return (int)((std::min<int64_t>((int64_t)max_query_len * G, WA_ROWS_COLS) + G - 1) / G);
+// Partial sums of decode rows: room for so many rows of a sequence, or (0) for the rows as they are numbered, if that is less.
+static int window_part_rows(const WindowPlan& w, int num_seqs, int num_rows, int max_query_len, int G) {
+  const int64_t of_seq = (std::min<int64_t>((int64_t)max_query_len * G, w.row_cols) + G - 1) / G;
+  return num_seqs * of_seq < num_rows ? (int)of_seq : 0;
 }
 
-// floats of the partial sums' outputs (maxima and sums follow); the two kinds of row take turns with them
+// floats of the partial sums' outputs, of one head dim (maxima and sums follow); the two kinds of row take turns with them
 static int64_t window_partials(const WindowPlan& w, int num_seqs, int num_rows, int num_heads, int num_kv_heads, int max_query_len) {
-  const int64_t rows = w.rows.splits > 1 ? (int64_t)num_seqs * window_part_rows(max_query_len, num_heads / num_kv_heads) * w.rows.splits : 0;
+  const int of_seq = window_part_rows(w, num_seqs, num_rows, max_query_len, num_heads / num_kv_heads);
+  const int64_t rows = w.rows.splits > 1 ? (of_seq ? (int64_t)num_seqs * of_seq : num_rows) * w.rows.splits : 0;
   const int64_t flash = w.flash.splits > 1 ? (int64_t)num_rows * w.flash.splits : 0;
   return std::max(rows, flash) * num_heads;
 }
 
 template <typename DT, int KV, int HEAD>
 static int launch_window(WindowParams p, const WindowPlan& w, int part_rows, hipStream_t s) {
-  auto groups = [&](const WindowPart& a) { return (int64_t)p.num_seqs * p.num_kv_heads * a.col_tiles * a.splits; };
-  auto merges = [&](const WindowPart& a) { return (int64_t)p.num_seqs * p.num_kv_heads * a.col_tiles * (a.cols / 4); };
+  auto tiles = [&](const WindowPart& a) { return (int64_t)(&a == &w.rows ? p.num_seqs : 1) * p.num_kv_heads * a.col_tiles; };
+  auto groups = [&](const WindowPart& a) { return tiles(a) * a.splits; };
+  auto merges = [&](const WindowPart& a) { return tiles(a) * (a.cols / 4); };
   const int64_t most = (int64_t)1 << 31;
   MI355Q_REQUIRE(groups(w.rows) < most && groups(w.flash) < most && merges(w.rows) < most && merges(w.flash) < most,
                  "paged_window_attention: too many workgroups");
@@ -1286,8 +1344,8 @@ static int launch_window(WindowParams p, const WindowPlan& w, int part_rows, hip
     p.col_tiles = a.col_tiles, p.splits = a.splits;
     p.split_tiles = a.splits == 1 ? INT_MAX : a.split_tiles;
     p.part_rows = kind ? 0 : part_rows;
-    p.min_cols = kind && !w.all_flash ? WA_ROWS_COLS + 1 : 0;
-    p.max_cols = kind ? INT_MAX : WA_ROWS_COLS;
+    p.min_cols = kind && !w.all_flash ? w.row_cols + 1 : 0;
+    p.max_cols = kind ? INT_MAX : w.row_cols;
     p.lds_cols = std::min(16, p.longest_cols);
     const dim3 grid((unsigned)groups(a)), wg(64 * a.waves);
     const size_t lds = (size_t)a.waves * p.lds_cols * (HEAD + 4) * sizeof(float);
@@ -1307,7 +1365,10 @@ static int launch_window(WindowParams p, const WindowPlan& w, int part_rows, hip
     }
     if (int e = check_launch("paged_window_attention")) return e;
     if (a.splits > 1) {
-      hipLaunchKernelGGL((window_merge_kernel<DT, HEAD>), dim3((unsigned)merges(a)), dim3(256), 0, s, p, a.cols);
+      const dim3 joins((unsigned)merges(a));
+      if (kind) hipLaunchKernelGGL((window_merge_kernel<DT, HEAD, WA_FLASH_COLS>), joins, dim3(256), 0, s, p);
+      else if (a.cols == 32) hipLaunchKernelGGL((window_merge_kernel<DT, HEAD, 32>), joins, dim3(256), 0, s, p);
+      else hipLaunchKernelGGL((window_merge_kernel<DT, HEAD, 16>), joins, dim3(256), 0, s, p);
       if (int e = check_launch("paged_window_attention")) return e;
     }
   }
@@ -1379,8 +1440,8 @@ extern "C" int mi355q_paged_window_attention(void* out, int64_t out_stride, cons
   const int pieces = block_size / 16;
   p.page_magic = pieces == 1 ? 0 : (int)(((1ull << 32) + pieces - 1) / pieces);
   p.window = std::min(window, 1 << 30), p.sinks = sinks;
-  const int part_rows = window_part_rows(max_query_len, p.group);
-  p.longest_cols = (int)std::min<int64_t>((int64_t)max_query_len * p.group, WA_ROWS_COLS);
+  const int part_rows = window_part_rows(w, num_seqs, num_rows, max_query_len, p.group);
+  p.longest_cols = (int)std::min<int64_t>((int64_t)max_query_len * p.group, w.row_cols);
   p.out16 = ((uintptr_t)out & 15) == 0 && out_stride % 8 == 0;
   hipStream_t s = (hipStream_t)stream;
 #define BY_KV(DT, HD)                                                                                                     \
