@@ -1,5 +1,6 @@
 """Refusals and sizing of the block-scaled cache and of windowed attention: host checks only, no kernel is launched."""
 import ctypes
+import random
 
 import pytest
 import torch
@@ -40,6 +41,11 @@ def test_append_refusals(over, message):
     refused(_lib.lib().mi355q_rope_and_cache_blocks, APPEND, message, **over)
 
 
+def test_more_than_a_launch_holds_is_refused():
+    refused(_lib.lib().mi355q_rope_and_cache_blocks, APPEND, "too many", num_tokens=(1 << 31) - 1)
+    refused(_lib.lib().mi355q_paged_window_attention, ATTEND, "too many", num_seqs=1 << 24, num_rows=1 << 24, max_query_len=1)
+
+
 def test_nothing_to_append_is_no_error():
     assert _lib.lib().mi355q_rope_and_cache_blocks(*{**APPEND, "num_tokens": 0}.values()) == _lib.OK
 
@@ -69,6 +75,18 @@ def test_workspace_is_asked_for_and_checked():
     refused(L.mi355q_paged_window_attention, ATTEND, "workspace", _lib.ENOSPACE, **long)
     refused(L.mi355q_paged_window_attention, ATTEND, "workspace", _lib.ENOSPACE, **long, workspace=PTR, workspace_bytes=16)
     refused(L.mi355q_paged_window_attention, ATTEND, "16-byte", **long, workspace=PTR + 4, workspace_bytes=1 << 30)
+
+
+def test_every_batch_has_a_plan_of_bounded_scratch():
+    """Any bounds a caller may give, those that contradict each other among them.  Decode rows: at most 32 stretches, or 256
+    workgroups of 32 columns; prompts: 256 workgroups of 256 columns, rounded up by less than one stretch of every column."""
+    size, rng = _lib.lib().mi355q_paged_window_attention_workspace_bytes, random.Random(1)
+    spread = lambda top: int(2 ** rng.uniform(0, top))
+    for _ in range(20000):
+        seqs, longest, kvh, group, head = spread(10), spread(14), rng.choice([1, 2, 4, 8]), rng.choice([1, 2, 3, 4, 7, 8, 16]), rng.choice([64, 128])
+        rows = rng.choice([seqs, max(seqs, longest), seqs + longest, rng.randint(1, seqs + longest)])
+        got = size(seqs, rows, kvh * group, kvh, head, longest, spread(20), rng.choice([0, 0, 1, 100, 4096]), rng.choice([0, 4]), rng.choice([0, 1, 2]))
+        assert got % ((head + 2) * 4) == 0 and got <= max(32 * rows * kvh * group, 256 * 256 * 2) * (head + 2) * 4
 
 
 def test_nothing_to_attend_is_no_error():

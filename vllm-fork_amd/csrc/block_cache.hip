@@ -708,9 +708,11 @@ extern "C" int mi355q_rope_and_cache_blocks(const int64_t* positions, const void
   // a wave looks at one position where a step holds few tokens (every one begins a run of its own), at 8 where they come
   // as prompts: most positions then continue a run, and waves that find nothing to begin are pure dispatch
   p.tokens_per_wave = num_tokens <= 512 ? 1 : 8;
-  const int64_t units = (int64_t)((num_tokens + p.tokens_per_wave - 1) / p.tokens_per_wave) * num_kv_heads;
-  p.kv_groups = (int)((units + 3) / 4);
-  const int q_groups = num_heads ? (num_tokens + 3) / 4 : 0;
+  const int64_t units = ((int64_t)num_tokens + p.tokens_per_wave - 1) / p.tokens_per_wave * num_kv_heads;
+  const int64_t kv_groups = (units + 3) / 4;
+  const int q_groups = num_heads ? (int)(((int64_t)num_tokens + 3) / 4) : 0;
+  MI355Q_REQUIRE((kv_groups + q_groups) * 256 < (int64_t)1 << 32, "rope_and_cache_blocks: %d tokens are too many for a launch", num_tokens);
+  p.kv_groups = (int)kv_groups;
   const size_t lds = (size_t)4 * head_size * block_size;
   hipStream_t s = (hipStream_t)stream;
   const dim3 grid(p.kv_groups + q_groups), wg(256);

@@ -1335,9 +1335,10 @@ static int launch_window(WindowParams p, const WindowPlan& w, int part_rows, hip
   auto tiles = [&](const WindowPart& a) { return (int64_t)(&a == &w.rows ? p.num_seqs : 1) * p.num_kv_heads * a.col_tiles; };
   auto groups = [&](const WindowPart& a) { return tiles(a) * a.splits; };
   auto merges = [&](const WindowPart& a) { return tiles(a) * (a.cols / 4); };
-  const int64_t most = (int64_t)1 << 31;
-  MI355Q_REQUIRE(groups(w.rows) < most && groups(w.flash) < most && merges(w.rows) < most && merges(w.flash) < most,
-                 "paged_window_attention: too many workgroups");
+  auto fits = [&](const WindowPart& a) {      // a launch has fewer than 2^32 threads
+    return groups(a) * 64 * a.waves < (int64_t)1 << 32 && (a.splits <= 1 || merges(a) * 256 < (int64_t)1 << 32);
+  };
+  MI355Q_REQUIRE(fits(w.rows) && fits(w.flash), "paged_window_attention: too many workgroups");
   for (int kind = 0; kind < 2; kind++) {
     const WindowPart& a = kind ? w.flash : w.rows;
     if (!a.col_tiles) continue;

@@ -1426,8 +1426,8 @@ def paged_window_attention(out: torch.Tensor, query: torch.Tensor, key_cache: to
     if query_start_loc is not None and (query_start_loc.dtype != torch.int32 or query_start_loc.shape != (S + 1,)
                                         or not query_start_loc.is_contiguous()):
         raise RuntimeError(f"{what}: query_start_loc must be contiguous int32 [{S + 1}]")
-    if sliding_window < 0 or sink_tokens < 0:
-        raise RuntimeError(f"{what}: sliding_window and sink_tokens must not be negative")
+    if sliding_window >> 31 or sink_tokens >> 31:
+        raise RuntimeError(f"{what}: sliding_window and sink_tokens must not be negative, and fit 31 bits")
     kv = _kv_type(kv_cache_dtype)
     element = 2 if kv == _lib.KV_16 else 1
     if element == 2 and (key_cache.dtype != query.dtype or value_cache.dtype != query.dtype):
