@@ -665,6 +665,31 @@ def test_strided_rows_tables_and_cache_heads():
     b.check(got)
 
 
+@pytest.mark.parametrize("form", ["auto", "fp8", "block_int8"])
+def test_pages_past_four_gib(form):
+    """The same pages at the far end of a cache of more than 2^32 bytes: same results, bit for bit."""
+    b = Batch([(100, 1), (60, 40), (2500, 3)], 8, 2, 64, 16, form, torch.bfloat16, seed=21)
+    want = cpu(b.run())
+    page = b.kc[0].numel() * b.kc.element_size()
+    blocks = (1 << 32) // page + 1000 + b.blocks
+    kc, vc = (torch.empty(blocks, *c.shape[1:], dtype=c.dtype, device=DEV) for c in (b.kc, b.vc))
+    kc[-b.blocks:], vc[-b.blocks:] = b.kc, b.vc
+    more = dict(key_cache=kc, value_cache=vc, block_tables=torch.where(b.dev["tables"] >= 0, b.dev["tables"] + (blocks - b.blocks), b.dev["tables"]))
+    if form == "block_int8":
+        scales = [torch.zeros(blocks, 2, device=DEV) for _ in range(2)]
+        for far, near in zip(scales, ("ks", "vs")):
+            far[-b.blocks:] = b.dev[near]
+        more.update(k_scale=scales[0], v_scale=scales[1])
+    assert torch.equal(cpu(b.run(**more)), want)
+    if form == "block_int8":
+        x = qkv_rows(50, 8, 2, 64, torch.bfloat16, seed=22).to(DEV)
+        slots = torch.arange(5, 55, device=DEV)
+        for k, v, s, at in ((b.kc, b.vc, [b.dev["ks"], b.dev["vs"]], slots), (kc, vc, scales, slots + (blocks - b.blocks) * 16)):
+            ops.reshape_and_cache_blocks(x[:, 512:640].unflatten(1, (2, 64)), x[:, 640:].unflatten(1, (2, 64)), k, v, *s, at, form)
+        assert torch.equal(kc[-b.blocks:], b.kc) and torch.equal(vc[-b.blocks:], b.vc)
+        assert torch.equal(scales[0][-b.blocks:], b.dev["ks"]) and torch.equal(scales[1][-b.blocks:], b.dev["vs"])
+
+
 def test_streams_graphs_and_a_workspace_of_ones_own():
     b = Batch([(2999, 1), (700, 3)], 4, 1, 128, 16, "block_int8", torch.bfloat16, seed=14)
     want = cpu(b.run())
