@@ -490,6 +490,24 @@ def test_prompts_among_many_sequences(form, window):
         b.check()
 
 
+@pytest.mark.parametrize("form", ["fp8", "block_int8", "block_fp8"])
+def test_values_next_to_nothing(form):
+    """V scales that are subnormal in 32 bits: the same rows, smaller by a power of two.  Two results rounded to bf16, half a step
+    2^-8 each, of values or (subnormal ones) of 2^-133 steps; where scales are this small, prompt rows round a scale and its
+    products with the codes to fp16, 2^-11 each of the largest value."""
+    b = Batch([(100, 1), (60, 200), (300, 3), (0, 1)], 4, 2, 64, 16, form, torch.bfloat16, seed=23, loud=0.3)
+    want = cpu(b.run())[:b.rows].double() * 2.0 ** -124
+    top = b.v.abs().max().item() * 2.0 ** -124
+    b.dev["vs"] = b.dev["vs"] * 2.0 ** -62 * 2.0 ** -62
+    assert 0 < b.dev["vs"].min().item() < 2.0 ** -127
+    got = cpu(b.run())[:b.rows].double()
+    assert torch.isfinite(got).all()
+    assert ((got - want).abs() <= 2.0 ** -7 * want.abs() + 2.0 ** -133 + 2.0 ** -10 * top).all()
+    if form != "fp8":       # next to blocks of zeros
+        b.dev["vs"][::2] = 0.0
+        assert torch.isfinite(cpu(b.run())).all()
+
+
 def test_one_scale_that_is_no_number():
     """Rows that see nothing stay zero whatever the scale is."""
     b = Batch([(0, 3), (20, 2), (0, 300)], 4, 2, 64, 16, "fp8", torch.bfloat16, seed=17)

@@ -467,8 +467,9 @@ __global__ __launch_bounds__(64 * NW, 2) void window_rows_kernel(const WindowPar
     if constexpr (KV != KV16) vtop = group_max(vs);
     float back = 1.f;                  // what a new reference for V's scales does to the sums
     if (KV != KV16 && __any(vtop > vref)) {
-      back = vref / (2.f * vtop);      // headroom of 2: the next slightly larger scale changes nothing
-      vref = 2.f * vtop;
+      const float next = fmaxf(2.f * vtop, 0x1p-125f);   // headroom of 2: the next slightly larger scale changes nothing; 1 / vref is finite
+      back = vref / next;
+      vref = next;
       vinv = 1.f / vref;
     }
     const float r = KV == KV16 || !ok ? 1.f : vs * vinv;
@@ -850,7 +851,7 @@ __global__ __launch_bounds__(64 * NW, HEAD == 64 ? 4 : 2) void window_flash_kern
     }
     if constexpr (SCALED) {
       top = wave_max(top);
-      top = top > 0.f ? __uint_as_float((__float_as_uint(fminf(top, 0x1p125f)) & 0x7f800000u) + 0x00800000u) : 0.f;
+      top = top > 0.f ? __uint_as_float((__float_as_uint(fminf(fmaxf(top, 0x1p-110f), 0x1p125f)) & 0x7f800000u) + 0x00800000u) : 0.f;
       if (first > begin) top = fmaxf(top, chunks[((first - begin) / CHUNK & 1) ^ 1].vref);   // never falls
       const float inv = top > 0.f ? WA_VSHIFT / top : 0.f;
 #pragma unroll
