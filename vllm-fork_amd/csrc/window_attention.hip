@@ -686,10 +686,10 @@ __global__ __launch_bounds__(64 * NW, 2) void window_rows_kernel(const WindowPar
 // widened codes, exactly (down to scales of 2^-30 of the largest); the number goes into the exponent of the probabilities.
 //
 // Bound by the matrix cores and the exponentials in turn: a SIMD holds two waves of 128-wide heads, and while both are in their
-// softmax no product runs.  8192 rows of 32 heads of 128 under a window of 4096, bf16: 440 us, 940 TFLOP/s of what is visible
+// softmax no product runs.  8192 rows of 32 heads of 128 under a window of 4096, bf16: 430 to 475 us from card to card, 870 to 960 TFLOP/s of what is visible
 // (a large matrix product reaches 1190); the matrix cores are busy 44 % of the cycles counted, the vector units 45 %, LDS conflicts
 // are 3 %.  2048 rows over a context of 6144 in int8 293 us, 810 TFLOP/s.  64-wide heads have room for two workgroups
-// to a CU, and the exponentials weigh twice as much: five prompts of up to 2047 rows under a window of 512, e4m3 with one scale, 46 us,
+// to a CU, and the exponentials weigh twice as much: five prompts of up to 2047 rows under a window of 512, e4m3 with one scale, 43.5 us,
 // vector units busy 59 %, matrix cores 19.
 // Slower at 8192 rows: four waves (489 us), the next tile's logits ahead of this one's softmax (795, registers spill), the
 // halves of a workgroup in opposite phases over three buffers (578), higher priority for half the waves (449 against 448).
@@ -1016,13 +1016,16 @@ __global__ __launch_bounds__(64 * NW, HEAD == 64 ? 4 : 2) void window_flash_kern
 #pragma unroll
         for (int k = 0; k < KS; k++) s[rt] = mfma32<MT>(*reinterpret_cast<const u32x4*>(st0 + (rt * KS + k) * 1024), qf[k], s[rt]);
       }
-      __builtin_amdgcn_sched_group_barrier(0x100, 6, 0);
+      // operand reads ahead of the products: six, or three in the 128 registers that 64-wide heads leave (five prompts under a
+      // window of 512: 48.5 us, with four or six of them 51)
+      constexpr int AHEAD = HEAD == 64 ? 3 : 6;
+      __builtin_amdgcn_sched_group_barrier(0x100, AHEAD, 0);
 #pragma unroll
-      for (int k = 0; k < 2 * KS - 6; k++) {
+      for (int k = 0; k < 2 * KS - AHEAD; k++) {
         __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
         __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
       }
-      __builtin_amdgcn_sched_group_barrier(0x008, 6, 0);
+      __builtin_amdgcn_sched_group_barrier(0x008, AHEAD, 0);
     }
     float f[4];
     if constexpr (!SCALED) {
