@@ -689,7 +689,7 @@ __global__ __launch_bounds__(64 * NW, 2) void window_rows_kernel(const WindowPar
 // softmax no product runs.  8192 rows of 32 heads of 128 under a window of 4096, bf16: 430 to 475 us from card to card, 870 to 960 TFLOP/s of what is visible
 // (a large matrix product reaches 1190); the matrix cores are busy 44 % of the cycles counted, the vector units 45 %, LDS conflicts
 // are 3 %.  2048 rows over a context of 6144 in int8 293 us, 810 TFLOP/s.  64-wide heads have room for two workgroups
-// to a CU, and the exponentials weigh twice as much: five prompts of up to 2047 rows under a window of 512, e4m3 with one scale, 43.5 us,
+// to a CU, and the exponentials weigh twice as much: five prompts of up to 2047 rows under a window of 512, e4m3 with one scale, 40 us,
 // vector units busy 59 %, matrix cores 19.
 // Slower at 8192 rows: four waves (489 us), the next tile's logits ahead of this one's softmax (795, registers spill), the
 // halves of a workgroup in opposite phases over three buffers (578), higher priority for half the waves (449 against 448).
@@ -1149,9 +1149,18 @@ __global__ __launch_bounds__(64 * NW, HEAD == 64 ? 4 : 2) void window_flash_kern
     }
   };
   int n = 0;
-  for (; n < in0; n++) step(n, std::false_type());
-  for (; n < in1; n++) step(n, std::true_type());
-  for (; n < tiles; n++) step(n, std::false_type());
+  if constexpr (HEAD == 64) {
+    // the masked step stands once in the code: 35 KB instead of 45, and short walks are bound by fetching it (five prompts under a
+    // window of 512 47.7 -> 44.4 us).  At 128 the compiler then finds worse registers: 2048 rows over 6144 296 -> 330 us.
+    while (n < tiles) {
+      for (; n >= in0 && n < in1; n++) step(n, std::true_type());
+      if (n < tiles) step(n++, std::false_type());
+    }
+  } else {
+    for (; n < in0; n++) step(n, std::false_type());
+    for (; n < in1; n++) step(n, std::true_type());
+    for (; n < tiles; n++) step(n, std::false_type());
+  }
 
   // ---- out ----------------------------------------------------------------------------------------------------------------
   l = pair_sum(l);
