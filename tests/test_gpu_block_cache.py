@@ -508,6 +508,16 @@ def test_values_next_to_nothing(form):
         assert torch.isfinite(cpu(b.run())).all()
 
 
+@pytest.mark.parametrize("bound", [1, 3, 20])
+def test_query_longer_than_its_bound(bound):
+    """As many rows as the bound says are certain, whatever else the batch holds."""
+    b = Batch([(100, 30), (3000, 2), (50, 1)], 8, 2, 64, 16, "block_int8", torch.bfloat16, seed=24)
+    want, tolerance = b.reference()
+    got = cpu(b.run(max_query_len=bound)).double()
+    first = torch.tensor([j < bound for _, n in b.lens for j in range(n)])
+    assert ((got[:b.rows] - want).abs() <= tolerance)[first].all()
+
+
 def test_one_scale_that_is_no_number():
     """Rows that see nothing stay zero whatever the scale is."""
     b = Batch([(0, 3), (20, 2), (0, 300)], 4, 2, 64, 16, "fp8", torch.bfloat16, seed=17)

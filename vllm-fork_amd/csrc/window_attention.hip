@@ -1149,9 +1149,10 @@ __global__ __launch_bounds__(64 * NW, HEAD == 64 ? 4 : 2) void window_flash_kern
     }
   };
   int n = 0;
-  if constexpr (HEAD == 64) {
+  if constexpr (HEAD == 64 || KV == KV16) {
     // the masked step stands once in the code: 35 KB instead of 45, and short walks are bound by fetching it (five prompts under a
-    // window of 512 47.7 -> 44.4 us).  At 128 the compiler then finds worse registers: 2048 rows over 6144 296 -> 330 us.
+    // window of 512 47.7 -> 44.4 us, 8192 rows in bf16 444 -> 440).  With codes of 128-wide heads the compiler then finds worse
+    // registers: 2048 rows over 6144 296 -> 330 us.
     while (n < tiles) {
       for (; n >= in0 && n < in1; n++) step(n, std::true_type());
       if (n < tiles) step(n++, std::false_type());
@@ -1373,7 +1374,7 @@ static int launch_window(WindowParams p, const WindowPlan& w, int part_rows, hip
     p.split_tiles = a.splits == 1 ? INT_MAX : a.split_tiles;
     p.part_rows = kind ? 0 : part_rows;
     p.min_cols = kind && !w.all_flash ? w.row_cols + 1 : 0;
-    p.max_cols = kind ? INT_MAX : w.row_cols;
+    p.max_cols = kind || !w.flash.col_tiles ? INT_MAX : w.row_cols;
     p.lds_cols = std::min(16, p.longest_cols);
     const dim3 grid((unsigned)groups(a)), wg(64 * a.waves);
     const size_t lds = (size_t)a.waves * p.lds_cols * (HEAD + 4) * sizeof(float);
