@@ -16,7 +16,7 @@
 //
 // Bound by HBM for prompts: 8192 tokens of 32 query and 8 kv heads of 128, int8, 35 to 39 us for 185 MB, 4.7 to 5.3 TB/s, what a large copy
 // reaches.  A decode step is a chain of round trips: slots, then rows, angles, scales and the block, then the stores: 6.9 us for
-// one token, 7.5 for 64; 508 tokens with half of a 64-wide head rotated (the general form) 11.8.
+// one token, 7.5 for 64; 508 tokens with half of a 64-wide head rotated 9.7.
 #include "common.h"
 
 // one rounding per operation: the results equal a sequence of separate fp32 multiplications and additions
@@ -309,7 +309,9 @@ __device__ inline u32x4 byte_mask(uint32_t m) {
 // FORM_WHOLE: NeoX pairing over the whole head, 16-bit angles of the model's type, aligned rows; FORM_NONE: no rotation, aligned
 // rows -- nearly every call, in kernels that the general form's code (60 KB) does not weigh on: 47 -> 35 us for 8192 prompt
 // tokens of 32 + 8 heads, 8.1 -> 6.7 us for one token.  Under FORM_WHOLE a lane holds 8 elements of K and their 8 partners.
-enum { FORM_ANY = 0, FORM_WHOLE = 1, FORM_NONE = 2 };
+// FORM_PART: the other rotations that turn runs of 16, aligned rows: 8192 tokens with half of each head in pairs 68 -> 62 us, 64 decode
+// tokens 9.1 -> 7.8 (with registers for three workgroups to a CU instead of two, as the two forms above, 59 and 9.8).
+enum { FORM_ANY = 0, FORM_WHOLE = 1, FORM_NONE = 2, FORM_PART = 3 };
 template <typename DT, bool INT8, int HEAD, int FORM>
 __device__ __forceinline__ void append_run(const AppendParams& p, int t, uint64_t here, int blk, int offset, int pos, int h,
                                            unsigned char* stage, int lane) {
@@ -359,14 +361,14 @@ __device__ __forceinline__ void append_run(const AppendParams& p, int t, uint64_
       k.a = *reinterpret_cast<const u32x4*>(kr + 8 * chunk);
       k.b = *reinterpret_cast<const u32x4*>(kr + HEAD / 2 + 8 * chunk);
       rotate8<DT>(k.a, k.b, *reinterpret_cast<const u32x4*>(angle), *reinterpret_cast<const u32x4*>(angle + HEAD / 2));
-    } else if (p.rot_mode == ROT_ANY) {
+    } else if (FORM == FORM_ANY && p.rot_mode == ROT_ANY) {
       k = rotate16_any<DT>(kr, d0, p, at);
     } else {
-      k = load16(kr + d0, p.aligned);
+      k = load16(kr + d0, FORM != FORM_ANY || p.aligned);
       if (turns) {
         Angles a;
         load_angles(a, p, at, d0);
-        const Row16 other = halves ? load16(kr + d0 + partner, p.aligned) : k;
+        const Row16 other = halves ? load16(kr + d0 + partner, FORM != FORM_ANY || p.aligned) : k;
         k = rotate16<DT>(k, other, a, halves, first_half);
       }
     }
@@ -485,13 +487,14 @@ __device__ __forceinline__ void append_run(const AppendParams& p, int t, uint64_
 }
 
 // The query of one token by one wave, 64 / (HEAD / 16) heads a pass: the general form, 16 elements of a head per lane.
-template <typename DT, int HEAD>
+template <typename DT, int HEAD, int FORM>
 __device__ inline void rotate_query(const AppendParams& p, int t, int lane) {
   constexpr int LPT = HEAD / 16, TPP = 64 / LPT;
   const int chunk = lane % LPT, sub = lane / LPT, d0 = chunk * 16;
   const bool turns = (p.rot_mode == ROT_HALVES || p.rot_mode == ROT_PAIRS) && d0 < p.rot;
   const bool halves = p.rot_mode == ROT_HALVES, first_half = d0 < p.rot / 2;
   const int partner = turns && halves ? (first_half ? p.rot / 2 : -(p.rot / 2)) : 0;
+  const bool aligned = FORM != FORM_ANY || p.aligned;
   const uint16_t* q = p.q + (int64_t)t * p.q_stride;
   uint16_t* out = p.q_out + (int64_t)t * p.q_out_stride;
   const int pos = p.rot_mode == ROT_NONE ? 0 : position(p, t);
@@ -501,17 +504,17 @@ __device__ inline void rotate_query(const AppendParams& p, int t, int lane) {
     const int h = min(h0 + sub, p.num_heads - 1);
     const uint16_t* x = q + (int64_t)h * HEAD;
     Row16 r;
-    if (p.rot_mode == ROT_ANY) {
+    if (FORM == FORM_ANY && p.rot_mode == ROT_ANY) {
       r = rotate16_any<DT>(x, d0, p, pos);
     } else {
-      r = load16(x + d0, p.aligned);
+      r = load16(x + d0, aligned);
       if (turns) {
-        const Row16 other = halves ? load16(x + d0 + partner, p.aligned) : r;
+        const Row16 other = halves ? load16(x + d0 + partner, aligned) : r;
         r = rotate16<DT>(r, other, a, halves, first_half);
       }
     }
     // (in place, a lane's partner has been read by now: the store needs what the same instructions loaded)
-    if (h0 + sub < p.num_heads) store16(out + (int64_t)h * HEAD + d0, r, p.aligned);
+    if (h0 + sub < p.num_heads) store16(out + (int64_t)h * HEAD + d0, r, aligned);
   }
 }
 
@@ -556,7 +559,7 @@ __device__ inline void rotate_query_whole(const AppendParams& p, int t, int lane
 }
 
 template <typename DT, bool INT8, int HEAD, int FORM>
-__global__ __launch_bounds__(256, FORM == FORM_ANY ? 2 : 3) void rope_and_cache_blocks_kernel(const AppendParams p) {
+__global__ __launch_bounds__(256, FORM == FORM_ANY || FORM == FORM_PART ? 2 : 3) void rope_and_cache_blocks_kernel(const AppendParams p) {
   extern __shared__ __attribute__((aligned(16))) unsigned char stage[];   // [4 waves][HEAD][block size]
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -566,7 +569,7 @@ __global__ __launch_bounds__(256, FORM == FORM_ANY ? 2 : 3) void rope_and_cache_
     if (t < p.num_tokens) {
       if constexpr (FORM == FORM_WHOLE) rotate_query_whole<DT, HEAD>(p, t, lane);
       else if constexpr (FORM == FORM_NONE) copy_query<HEAD>(p, t, lane);
-      else rotate_query<DT, HEAD>(p, t, lane);
+      else rotate_query<DT, HEAD, FORM>(p, t, lane);
     }
     return;
   }
@@ -620,7 +623,7 @@ __global__ __launch_bounds__(256, FORM == FORM_ANY ? 2 : 3) void rope_and_cache_
   // Lane i looks at token t0 - 1 + i: whether a run begins at one of the wave's positions, and (all but always) the whole of it.
   int slot;
   const int tl = t0 - 1 + lane, blk = block_at(tl, slot);
-  const bool rotates = FORM == FORM_WHOLE || (FORM == FORM_ANY && p.rot_mode != ROT_NONE);
+  const bool rotates = FORM == FORM_WHOLE || FORM == FORM_PART || (FORM == FORM_ANY && p.rot_mode != ROT_NONE);
   const int pos = rotates && tl >= 0 && tl < p.num_tokens ? position(p, tl) : 0;
   const int before = __shfl_up(blk, 1, 64);
   uint64_t heads = __ballot(lane > 0 && lane <= p.tokens_per_wave && blk >= 0 && blk != before);
@@ -722,12 +725,13 @@ extern "C" int mi355q_rope_and_cache_blocks(const int64_t* positions, const void
   const dim3 grid(p.kv_groups + q_groups), wg(256);
   const bool i8 = code_type == MI355Q_KV_INT8;
   const bool whole = p.rot_mode == ROT_HALVES && rot_dim == head_size && p.aligned && cos_dtype == dtype;
-  const bool none = p.rot_mode == ROT_NONE && p.aligned;
+  const bool none = p.rot_mode == ROT_NONE && p.aligned, part = (p.rot_mode == ROT_HALVES || p.rot_mode == ROT_PAIRS) && p.aligned;
 #define LAUNCH(DT, I8, HD, FM) hipLaunchKernelGGL((rope_and_cache_blocks_kernel<DT, I8, HD, FM>), grid, wg, lds, s, p)
 #define BY_FORM(DT, I8, HD)                      \
   do {                                           \
     if (whole) LAUNCH(DT, I8, HD, FORM_WHOLE);   \
     else if (none) LAUNCH(DT, I8, HD, FORM_NONE); \
+    else if (part) LAUNCH(DT, I8, HD, FORM_PART); \
     else LAUNCH(DT, I8, HD, FORM_ANY);           \
   } while (0)
 #define BY_HEAD(DT, I8)                          \
