@@ -1327,7 +1327,9 @@ static WindowPlan window_plan(int num_seqs, int num_rows, int num_heads, int num
     // side by side in the grid).  What is shorter than two stretches stays whole: 64 contexts up to 4096 in four stretches took 84 us,
     // whole 71; 32 decode rows under a window of 4096 in two 91, whole 84.
     const int64_t stretches = groups <= 64 ? 256 / groups : std::max<int64_t>(256 / groups, std::clamp<int64_t>(std::min(tiles / 64, 16384 / groups), 1, 32));
-    window_cut(w.rows, tiles, stretches, (tiles <= 4 * w.rows.waves ? 4 : 2) * w.rows.waves);
+    // A stretch has a tile for each wave at least, and two for each stay whole: the join is a launch of 4 us.  One sequence, in a
+    // graph: 1000 tokens whole 11.1 us, in two 11.9; 2000 whole 15.7, in four 11.8; 4000 in four 13.9, in eight 12.2; 8000 15.8 and 14.0.
+    window_cut(w.rows, tiles, stretches, (tiles <= 2 * w.rows.waves ? 2 : 1) * w.rows.waves);
   }
   if (prompts) {
     // Column tiles of the whole batch at most.  (Sequences times the longest one's tiles were 445 us for 200 decode rows and
