@@ -687,10 +687,10 @@ __global__ __launch_bounds__(64 * NW, 2) void window_rows_kernel(const WindowPar
 //
 // Bound by the matrix cores and the exponentials in turn: a SIMD holds two waves of 128-wide heads, and while both are in their
 // softmax no product runs.  8192 rows of 32 heads of 128 under a window of 4096, bf16: 430 to 475 us from card to card, 870 to 960 TFLOP/s of what is visible
-// (a large matrix product reaches 1190); the matrix cores are busy 44 % of the cycles counted, the vector units 45 %, LDS conflicts
+// (a large matrix product reaches 1190); the matrix cores are busy 45 % of the cycles counted, the vector units 47 %, LDS conflicts
 // are 3 %.  2048 rows over a context of 6144 in int8 293 us, 810 TFLOP/s.  64-wide heads have room for two workgroups
 // to a CU, and the exponentials weigh twice as much: five prompts of up to 2047 rows under a window of 512, e4m3 with one scale, 40 us,
-// vector units busy 59 %, matrix cores 19.
+// vector units busy 60 %, matrix cores 22.
 // Slower at 8192 rows: four waves (489 us), the next tile's logits ahead of this one's softmax (795, registers spill), the
 // halves of a workgroup in opposite phases over three buffers (578), higher priority for half the waves (449 against 448).
 // ---------------------------------------------------------------------------------------------------------------------
