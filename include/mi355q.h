@@ -758,7 +758,7 @@ int mi355q_rope_and_cache_blocks(const int64_t* positions, const void* query, in
  * mi355q_reshape_and_cache, the caches of mi355q_rope_and_cache_blocks have one for each.
  * Only pages that some row sees are looked up (those behind the window may have been given away); a page number outside
  * [0, num_blocks) reads as tokens that nobody sees.  query_start_loc int32 [num_seqs + 1], or NULL: one row each.
- * max_query_len bounds the query lengths (of a longer one only that many rows are certain); max_seq_len only chooses how
+ * max_query_len bounds the query lengths (of a longer one only its first max_query_len rows are certain); max_seq_len only chooses how
  * the work is cut.
  * workspace: device scratch of mi355q_paged_window_attention_workspace_bytes(...) bytes (0: may be NULL), used by this
  * call alone; nothing in it has to be cleared.  head_size 64 or 128; 1 to 16 query heads to a kv head; block_size a

@@ -518,6 +518,27 @@ def test_query_longer_than_its_bound(bound):
     assert ((got[:b.rows] - want).abs() <= tolerance)[first].all()
 
 
+@pytest.mark.parametrize("form", ["auto", "block_int8"])
+@pytest.mark.parametrize("lens,bound", [
+    ([(0, 300), (50, 20), (10, 1)], 20),             # one query of several column tiles where the bound says one
+    ([(0, 300)], 20), ([(7, 200), (0, 20)], 20), ([(0, 20), (30, 500), (90, 3), (5, 17)], 20),
+    ([(4200, 400), (5000, 33), (20, 1)], 33),        # contexts in stretches
+    ([(3, 1), (0, 700), (40, 130), (8, 129)], 130),
+])
+def test_query_of_more_column_tiles_than_its_bound(form, lens, bound):
+    """The rows within the bound are certain in every sequence, in a batch whose prompts take more column tiles than announced."""
+    b = Batch(lens, 8, 2, 64, 16, form, torch.bfloat16, seed=25)
+    want, tolerance = b.reference()
+    first = torch.tensor([j < bound for _, n in lens for j in range(n)])
+    for window in (0, 100):
+        if window:
+            b.window, b.sinks = window, 3
+            want, tolerance = b.reference()
+        got = cpu(b.run(max_query_len=bound)).double()
+        assert torch.equal(got[b.rows:], torch.full_like(got[b.rows:], 3.0))
+        assert ((got[:b.rows] - want).abs() <= tolerance)[first].all()
+
+
 def test_one_scale_that_is_no_number():
     """Rows that see nothing stay zero whatever the scale is."""
     b = Batch([(0, 3), (20, 2), (0, 300)], 4, 2, 64, 16, "fp8", torch.bfloat16, seed=17)
@@ -550,6 +571,7 @@ def test_scale_zero_and_pages_out_of_range():
         b.tables[0, 2], b.tables[1, 5] = -1, b.blocks
         b.dev["tables"] = b.tables.to(DEV)
         b.check()
+
 
 
 @pytest.mark.parametrize("form", FORMS)

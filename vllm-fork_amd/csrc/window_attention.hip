@@ -63,7 +63,8 @@ struct WindowParams {
   int splits, split_tiles;      // the context in stretches of split_tiles 64-token tiles, at most `splits` of them
   int part_rows;                // decode rows: room for so many rows of a sequence (0: rows as they are numbered)
   int col_tiles;                // decode rows: column tiles of the longest query
-  int longest_cols;             // columns of the longest query, at most WA_ROWS_COLS
+  int longest_cols;             // columns of the longest query as the caller announced it (rows kernel: at most WA_ROWS_COLS); a
+                                // longer query is served so far
   int lds_cols;                 // rows kernel: columns of a 16-column tile that any sequence has
   int min_cols, max_cols;       // sequences with fewer or more columns (rows x heads per kv head) are another launch's
 };
@@ -88,7 +89,7 @@ __device__ inline Slot slot_of(const WindowParams& p, int slot) {
   for (int s0 = 0; s0 < p.num_seqs; s0 += 64) {
     const int start = from, qlen = to - from;
     if (s0 + 64 < p.num_seqs) from = first_row(s0 + 64 + lane), to = first_row(s0 + 65 + lane);   // on their way meanwhile
-    const int cols = min(qlen, p.num_rows - start) * p.group;
+    const int cols = min(min(qlen, p.num_rows - start) * p.group, p.longest_cols);   // (the grid has room for no more than was announced)
     const int n = start < 0 || cols < p.min_cols ? 0 : (max(cols, 0) + COLS - 1) / COLS;
     int upto = n;
 #pragma unroll
@@ -753,7 +754,7 @@ __global__ __launch_bounds__(64 * NW, HEAD == 64 ? 4 : 2) void window_flash_kern
   if (slot.seq < 0) return;
   const int seq = slot.seq, ct = slot.ct, start = slot.start, qlen = slot.qlen;
   const int G = p.group;
-  const int cols = min(qlen, p.num_rows - start) * G;
+  const int cols = min(min(qlen, p.num_rows - start) * G, p.longest_cols);
   const int seq_len = sload(p.seq_lens + seq);
   const int c0 = ct * COLS, c1 = min(c0 + COLS, cols) - 1;
   const int pos0 = seq_len - qlen + c0 / G, pos1 = seq_len - qlen + c1 / G;
@@ -1235,7 +1236,7 @@ __global__ __launch_bounds__(256) void window_merge_kernel(const WindowParams p)
     start = p.starts ? sload(p.starts + seq) : seq;
     qlen = p.starts ? sload(p.starts + seq + 1) - start : 1;
   }
-  const int all = min(qlen, p.num_rows - start) * p.group, cols = FLASH ? all : min(all, p.longest_cols);
+  const int all = min(qlen, p.num_rows - start) * p.group, cols = min(all, p.longest_cols);
   if (start < 0 || c >= cols || all > p.max_cols) return;
   const int seq_len = sload(p.seq_lens + seq);
   const int c0 = c / COLS * COLS, c1 = min(c0 + COLS, cols) - 1;
@@ -1369,6 +1370,7 @@ static int launch_window(WindowParams p, const WindowPlan& w, int part_rows, hip
     return groups(a) * 64 * a.waves < (int64_t)1 << 32 && (a.splits <= 1 || merges(a) * 256 < (int64_t)1 << 32);
   };
   MI355Q_REQUIRE(fits(w.rows) && fits(w.flash), "paged_window_attention: too many workgroups");
+  const int announced = p.longest_cols;
   for (int kind = 0; kind < 2; kind++) {
     const WindowPart& a = kind ? w.flash : w.rows;
     if (!a.col_tiles) continue;
@@ -1377,6 +1379,7 @@ static int launch_window(WindowParams p, const WindowPlan& w, int part_rows, hip
     p.part_rows = kind ? 0 : part_rows;
     p.min_cols = kind && !w.all_flash ? w.row_cols + 1 : 0;
     p.max_cols = kind || !w.flash.col_tiles ? INT_MAX : w.row_cols;
+    p.longest_cols = kind ? announced : std::min(announced, w.row_cols);
     p.lds_cols = std::min(16, p.longest_cols);
     const dim3 grid((unsigned)groups(a)), wg(64 * a.waves);
     const size_t lds = (size_t)a.waves * p.lds_cols * (HEAD + 4) * sizeof(float);
@@ -1472,7 +1475,7 @@ extern "C" int mi355q_paged_window_attention(void* out, int64_t out_stride, cons
   p.page_magic = pieces == 1 ? 0 : (int)(((1ull << 32) + pieces - 1) / pieces);
   p.window = std::min(window, 1 << 30), p.sinks = sinks;
   const int part_rows = window_part_rows(w, num_seqs, num_rows, max_query_len, p.group);
-  p.longest_cols = (int)std::min<int64_t>((int64_t)max_query_len * p.group, w.row_cols);
+  p.longest_cols = (int)std::min<int64_t>((int64_t)max_query_len * p.group, INT_MAX);
   p.out16 = ((uintptr_t)out & 15) == 0 && out_stride % 8 == 0;
   hipStream_t s = (hipStream_t)stream;
 #define BY_KV(DT, HD)                                                                                                     \
