@@ -573,6 +573,35 @@ def test_scale_zero_and_pages_out_of_range():
         b.check()
 
 
+def swap_blocks(b, i, j):
+    """Pages i and j of a batch's cache change places, in the tables too."""
+    for t in (b.k, b.v, b.kc, b.vc) + ((b.dev["ks"], b.dev["vs"]) if b.form.startswith("block") else ()):
+        t[[i, j]] = t[[j, i]]
+    at_i, at_j = b.tables == i, b.tables == j
+    b.tables[at_i], b.tables[at_j] = j, i
+    b.dev["tables"] = b.tables.to(DEV)
+
+
+@pytest.mark.parametrize("form", FORMS)
+@pytest.mark.parametrize("window,sinks", [(0, 0), (150, 20)])
+def test_pages_out_of_range_show_nothing_of_block_0(form, window, sinks):
+    """A page outside the cache is nobody's, also where block 0 holds nothing but NaN, in tiles that every row sees whole: decode
+    rows, drafts, prompt rows, a context in several stretches."""
+    for lens in ([(300, 1), (290, 5), (4500, 1)], [(300, 1), (310, 40), (150, 100)]):
+        b = Batch(lens, 8, 2, 64, 16, form, torch.bfloat16, window=window, sinks=sinks, seed=26)
+        used = set(b.tables.flatten().tolist())
+        swap_blocks(b, 0, next(n for n in range(b.blocks) if n not in used))
+        for s, (c, n) in enumerate(lens):
+            for i, page in enumerate(range(1 + s, (c + n) // 16, 7)):
+                b.tables[s, page] = [-1, b.blocks, 1 << 30, -(1 << 31)][i % 4]
+        b.dev["tables"] = b.tables.to(DEV)
+        nan = {"auto": 0x7fc0, "fp8": 0x7f, "block_fp8": 0xff, "block_int8": 0x80}[form]
+        for t in (b.kc, b.vc):
+            t.view(torch.int16 if form == "auto" else torch.uint8)[0] = nan
+        if form.startswith("block"):
+            b.dev["ks"][0] = b.dev["vs"][0] = float("nan")
+        b.check()
+
 
 @pytest.mark.parametrize("form", FORMS)
 @pytest.mark.parametrize("window,sinks", [(0, 0), (70, 4)])

@@ -538,6 +538,16 @@ __global__ __launch_bounds__(64 * NW, 2) void window_rows_kernel(const WindowPar
       bad = __any(clear_v(tg, lim, ok));
       left_out |= bad;
     }
+    if constexpr (INNER && KV != KVI8) {
+      if (ok_tile != 15) {               // a page outside the cache: block 0 was fetched in its place, and 0 times its NaN is one
+#pragma unroll
+        for (int d = 0; d < DT16; d++)
+#pragma unroll
+          for (int h = 0; h < VP; h++)
+#pragma unroll
+            for (int e = 0; e < 4; e++) vf[d][h][e] = ok ? vf[d][h][e] : 0u;
+      }
+    }
     if (INNER || KV == KVI8 || !bad) {
 #pragma unroll
       for (int d = 0; d < DT16; d++)
