@@ -761,7 +761,7 @@ int mi355q_rope_and_cache_blocks(const int64_t* positions, const void* query, in
  * max_query_len bounds the query lengths (of a longer one only its first max_query_len rows are certain); max_seq_len only chooses how
  * the work is cut.
  * workspace: device scratch of mi355q_paged_window_attention_workspace_bytes(...) bytes (0: may be NULL), used by this
- * call alone; nothing in it has to be cleared.  head_size 64 or 128; 1 to 16 query heads to a kv head; block_size a
+ * call alone; nothing in it has to be cleared.  (The size is 0 too for bounds that the call refuses.)  head_size 64 or 128; 1 to 16 query heads to a kv head; block_size a
  * multiple of 16 up to 256.
  * Stands for the reference's windowed attention (sliding_window of AttentionImpl, vllm/v1/attention/backends/
  * rocm_attn.py:271-300; ops/prefix_prefill.py SLIDING_WINDOW); visible first tokens and block scales have no counterpart there.

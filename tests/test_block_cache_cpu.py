@@ -89,6 +89,20 @@ def test_every_batch_has_a_plan_of_bounded_scratch():
         assert got % ((head + 2) * 4) == 0 and got <= max(32 * rows * kvh * group, 256 * 256 * 2) * (head + 2) * 4
 
 
+@pytest.mark.parametrize("heads,kv_heads", [(4, 8), (1, 2), (5, 2), (34, 2), (0, 1), (1, 0), (-4, 2), (4, -2), (-4, -2), (1, 1 << 30)])
+def test_heads_that_do_not_fit_are_refused(heads, kv_heads):
+    """Also where the size of the scratch is asked for, before the attention has seen them."""
+    L = _lib.lib()
+    for window in (0, 100):
+        for longest in (1, 5, 300):
+            assert L.mi355q_paged_window_attention_workspace_bytes(1, 3, heads, kv_heads, 128, longest, 1 << 17, window, 4, _lib.KV_INT8) == 0
+            refused(L.mi355q_paged_window_attention, ATTEND, "query heads", num_heads=heads, num_kv_heads=kv_heads, window=window,
+                    max_query_len=longest)
+    for bad in (dict(window=-1), dict(sinks=-1), dict(window=-(1 << 31))):
+        bounds = dict(seqs=1, rows=1, heads=4, kv_heads=2, head=128, longest=1, context=1 << 17, window=0, sinks=0, kv=_lib.KV_INT8)
+        assert L.mi355q_paged_window_attention_workspace_bytes(*{**bounds, **bad}.values()) == 0
+
+
 def test_nothing_to_attend_is_no_error():
     f = _lib.lib().mi355q_paged_window_attention
     assert f(*{**ATTEND, "num_rows": 0}.values()) == _lib.OK and f(*{**ATTEND, "num_seqs": 0}.values()) == _lib.OK

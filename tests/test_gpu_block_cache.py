@@ -539,6 +539,16 @@ def test_query_of_more_column_tiles_than_its_bound(form, lens, bound):
         assert ((got[:b.rows] - want).abs() <= tolerance)[first].all()
 
 
+@pytest.mark.parametrize("heads", [1, 4, 12, 136])
+def test_query_heads_that_do_not_fit_the_cache(heads):
+    """Fewer query heads than kv heads, no whole number to each, more than 16 to each: an error, before anything is sized by them."""
+    b = Batch([(100, 1), (60, 3)], 16, 8, 64, 16, "block_int8", torch.bfloat16, seed=27)
+    q = torch.zeros(b.rows, heads, 64, dtype=torch.bfloat16, device=DEV)
+    for window in (0, 50):
+        with pytest.raises(RuntimeError, match="query heads"):
+            b.run(query=q, out=torch.empty_like(q), sliding_window=window)
+
+
 def test_one_scale_that_is_no_number():
     """Rows that see nothing stay zero whatever the scale is."""
     b = Batch([(0, 3), (20, 2), (0, 300)], 4, 2, 64, 16, "fp8", torch.bfloat16, seed=17)

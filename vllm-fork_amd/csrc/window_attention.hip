@@ -1423,9 +1423,15 @@ static int launch_window(WindowParams p, const WindowPlan& w, int part_rows, hip
 
 using namespace mi355q;
 
+static bool heads_fit(int num_heads, int num_kv_heads) {
+  return num_heads > 0 && num_kv_heads > 0 && num_heads % num_kv_heads == 0 && num_heads / num_kv_heads <= 16;
+}
+
 extern "C" size_t mi355q_paged_window_attention_workspace_bytes(int num_seqs, int num_rows, int num_heads, int num_kv_heads, int head_size,
                                                                 int max_query_len, int max_seq_len, int window, int sinks, int kv_type) {
-  if (num_seqs <= 0 || num_rows <= 0 || num_kv_heads <= 0 || num_heads <= 0 || max_query_len <= 0 || max_seq_len <= 0) return 0;
+  // (bounds that the attention itself refuses need no scratch; the plan divides by the heads to a kv head)
+  if (num_seqs <= 0 || num_rows <= 0 || !heads_fit(num_heads, num_kv_heads) || max_query_len <= 0 || max_seq_len <= 0 || window < 0 || sinks < 0)
+    return 0;
   const WindowPlan w = window_plan(num_seqs, num_rows, num_heads, num_kv_heads, kv_type, max_query_len, max_seq_len, window, sinks);
   return (size_t)window_partials(w, num_seqs, num_rows, num_heads, num_kv_heads, max_query_len) * (head_size + 2) * sizeof(float);
 }
@@ -1445,7 +1451,7 @@ extern "C" int mi355q_paged_window_attention(void* out, int64_t out_stride, cons
   MI355Q_REQUIRE(out && query && key_cache && value_cache && block_tables && seq_lens, "paged_window_attention: null pointer");
   MI355Q_REQUIRE(kv_type == MI355Q_KV_16 || (k_scale && v_scale), "paged_window_attention: an 8-bit cache needs k_scale / v_scale");
   MI355Q_REQUIRE(head_size == 64 || head_size == 128, "paged_window_attention: head_size %d (64 or 128)", head_size);
-  MI355Q_REQUIRE(num_heads > 0 && num_kv_heads > 0 && num_heads % num_kv_heads == 0 && num_heads / num_kv_heads <= 16,
+  MI355Q_REQUIRE(heads_fit(num_heads, num_kv_heads),
                  "paged_window_attention: %d query heads over %d kv heads (1 to 16 to each)", num_heads, num_kv_heads);
   MI355Q_REQUIRE(block_size >= 16 && block_size <= 256 && block_size % 16 == 0, "paged_window_attention: block size %d (a multiple of 16 up to 256)", block_size);
   MI355Q_REQUIRE(num_blocks > 0 && max_blocks_per_seq > 0 && (int64_t)max_blocks_per_seq * block_size < (int64_t)1 << 30,

@@ -1435,6 +1435,8 @@ def paged_window_attention(out: torch.Tensor, query: torch.Tensor, key_cache: to
     blocks, kvh, bs, strides = _paged_cache(what, key_cache, value_cache, D, element)
     if kvh != num_kv_heads:
         raise RuntimeError(f"{what}: {num_kv_heads} kv heads over a cache of {kvh}")
+    if kvh == 0 or H % kvh or not 1 <= H // kvh <= 16:
+        raise RuntimeError(f"{what}: {H} query heads over {kvh} kv heads (1 to 16 to each)")
     scales = (None, None, 0, 0)
     if element == 1:
         if k_scale is None or v_scale is None:
