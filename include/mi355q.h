@@ -734,7 +734,11 @@ enum { MI355Q_KV_16 = 0, MI355Q_KV_FP8 = 1, MI355Q_KV_INT8 = 2 };
  *   Writing offset 0 restarts a block.  A value that is not finite makes the scale NaN.
  * slot_mapping int64 [num_tokens]; slots outside [0, num_blocks * block_size) are skipped (their query is rotated all the
  * same).  The tokens of one block follow one another in slot_mapping, as a scheduler lays a sequence's new tokens (skipped
- * ones may stand between them); of several with the same slot the last one stays.  Positions are clamped to the table's max_position rows.
+ * ones may stand between them); of several with the same slot the last one stays.  A block's tokens are taken 64 positions of
+ * slot_mapping at a time: where skipped or repeated ones stretch them over more (a block without such holds 64 at most), the call
+ * does what one call for each stretch would, the next beginning at the block's first token 64 positions or more behind the last
+ * one's beginning.  Codes may then be rounded more than once, and a stretch that goes back to an earlier offset makes what the
+ * call itself wrote from there on void, as a call would.  Positions are clamped to the table's max_position rows.
  * head_size 64 or 128, block_size 16, 32, 48 or 64; rows of 16-byte alignment take the wide loads, others work too.
  * No counterpart in the reference, whose 8-bit caches have one scale per tensor or per head
  * (csrc/cache_kernels.cu:254-400; rope and cache write in one hook: vllm/v1/attention/backends/rocm_attn.py:522-562).

@@ -224,6 +224,34 @@ def test_append_one_slot_named_many_times():
     run_append(c, qkv, 1, KVH, D, torch.arange(150), angles(D, 150, torch.float16), D, True, slots)
 
 
+@pytest.mark.parametrize("form", ["block_int8", "block_fp8"])
+@pytest.mark.parametrize("T", [400, 900])
+def test_append_of_a_block_stretched_over_many_positions(form, T):
+    """What the header says of a block whose tokens take more than 64 positions: the call does what a call for each stretch does --
+    on the way up, back to offset 0, back to an offset between, with slots named again; other blocks beside it."""
+    H, KVH, D, bs = 2, 2, 64, 16
+    slots = [-1] * T
+    for at, slot in [(0, 21), (1, 22), (63, 23), (64, 24), (90, 16), (91, 30), (170, 18), (171, 17), (233, 18), (234, 31), (235, 40), (236, 41),
+                     (310, 32), (330, 50), (331, 51), (T - 1, 49)]:
+        slots[at] = slot
+    one, many = Cache(5, KVH, D, bs, form, seed=3), Cache(5, KVH, D, bs, form, seed=3)
+    qkv, pos, cs = qkv_rows(T, H, KVH, D, torch.bfloat16, 15), torch.arange(T), angles(D, T, torch.bfloat16)
+    run_append(one, qkv, H, KVH, D, pos, cs, D, True, slots)
+    calls, begin, block = [], None, None
+    for t, slot in enumerate(slots):
+        if slot < 0:
+            continue
+        if slot // bs != block or t >= begin + 64:
+            calls.append([-1] * T)
+            begin, block = t, slot // bs
+        calls[-1][t] = slot
+    assert len(calls) == 8
+    for call in calls:
+        run_append(many, qkv, H, KVH, D, pos, cs, D, True, call)
+    for name in ("kc", "vc", "ks", "vs"):
+        assert torch.equal(getattr(one, name), getattr(many, name)), name
+
+
 def test_append_unaligned_rows_and_strided_scales():
     H, KVH, D, bs = 3, 2, 64, 16
     c = Cache(5, KVH, D, bs, "block_int8")

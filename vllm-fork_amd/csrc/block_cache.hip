@@ -8,6 +8,8 @@
 //   s_new = max(s_old, max |x| * (1 / QMAX))     over the call's tokens in b
 //   codes at offsets < first become round(c * (s_old / s_new)) where s_new > s_old
 //   new codes are round(x / s_new), 0 where s_new is 0; other offsets keep their bytes.
+// A run of tokens that skipped or repeated slots stretch over more than 64 positions (a lane each) is appended 64 positions at a
+// time, as so many calls would: each stretch is a call's tokens in what is said above.
 // A value that is not finite makes its block's scale NaN: reads of the block are NaN until it is restarted.
 //
 // The tokens of one block follow one another in slot_mapping (tokens without a slot may stand between them), so a block's

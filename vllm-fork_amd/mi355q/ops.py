@@ -1321,7 +1321,8 @@ def rope_and_cache_blocks(positions: torch.Tensor, query: torch.Tensor, key: tor
     the cache takes it rotated.  kv_cache_dtype "block_int8" or "block_fp8"; k_scales / v_scales fp32 [blocks, kv_heads].
     A block's scale grows with its tokens (earlier codes are rescaled) and starts over when offset 0 is written.
     slot_mapping int64 [T]: negative slots and slots past the cache are skipped; the tokens of one block follow one
-    another (skipped ones may stand between them).  Not idempotent on `query` when in place, and tokens must be appended in their order."""
+    another (skipped ones may stand between them; where these or repeated slots stretch a block's tokens over more than 64
+    positions, each 64 are appended as by a call of their own).  Not idempotent on `query` when in place, and tokens must be appended in their order."""
     what = "rope_and_cache_blocks"
     index = _one_device(what, key, positions, query, value, cos_sin_cache, key_cache, value_cache, k_scales, v_scales, slot_mapping, query_out)
     T = slot_mapping.numel()
