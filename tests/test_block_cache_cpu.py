@@ -6,7 +6,7 @@ import pytest
 import torch
 
 from mi355q import _lib, ops
-from mi355q.plugin.attention import Attention, Mi355AttentionBackend, Mi355AttentionImpl
+from mi355q.plugin.attention import Attention, Mi355AttentionBackend, Mi355AttentionImpl, Mi355AttentionMetadata
 
 _BUFFER = ctypes.create_string_buffer(4096)
 PTR = (ctypes.addressof(_BUFFER) + 63) & ~63   # never read: every call below is refused
@@ -145,6 +145,19 @@ def test_attention_layer_arguments():
     layer = Attention(8, 128, 0.1, 2, cache_dtype="block_fp8", sliding_window=64)
     layer.process_weights_after_loading()
     assert layer.impl.block_scaled and not hasattr(layer, "k_scale") and layer.kv_scales is None
+
+
+@pytest.mark.parametrize("form", ["block_int8", "block_fp8"])
+def test_layer_without_its_scales_says_so(form):
+    layer = Attention(4, 64, 0.1, 2, cache_dtype=form)
+    layer.kv_cache = torch.zeros(Mi355AttentionBackend.get_kv_cache_shape(3, 16, 2, 64), dtype=torch.uint8)
+    q, k = torch.zeros(2, 256, dtype=torch.bfloat16), torch.zeros(2, 128, dtype=torch.bfloat16)
+    i32 = dict(dtype=torch.int32)
+    md = Mi355AttentionMetadata(2, 2, torch.tensor([0, 2], **i32), 2, torch.tensor([2], **i32), torch.zeros(1, 1, **i32), torch.arange(2))
+    for call in (lambda: layer(q, k, k, md), lambda: layer.impl.forward(layer, q, k, k, layer.kv_cache, md, torch.empty_like(q)),
+                 lambda: layer.impl.do_rope_and_kv_cache_update(layer, q, k, k, torch.arange(2), torch.zeros(4, 64), True, layer.kv_cache, md.slot_mapping)):
+        with pytest.raises(RuntimeError, match="kv_scales"):
+            call()
 
 
 def test_registered_operators_have_schemas_and_fakes():

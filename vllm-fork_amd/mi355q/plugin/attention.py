@@ -210,7 +210,12 @@ class Mi355AttentionImpl:
 
     def _scales(self, layer):
         """(k, v) scales of the layer: one value each, or [blocks, kv_heads]."""
-        return (layer.kv_scales[0], layer.kv_scales[1]) if self.block_scaled else (layer._k_scale, layer._v_scale)
+        if not self.block_scaled:
+            return layer._k_scale, layer._v_scale
+        if getattr(layer, "kv_scales", None) is None:
+            raise RuntimeError(f"a {self.kv_cache_dtype} cache needs layer.kv_scales beside it: fp32 zeros of "
+                               "Mi355AttentionBackend.get_kv_scales_shape(num_blocks, num_kv_heads)")
+        return layer.kv_scales[0], layer.kv_scales[1]
 
     # -- contract ----------------------------------------------------------
     def do_kv_cache_update(self, layer, key, value, kv_cache, slot_mapping) -> None:
