@@ -577,6 +577,16 @@ def test_query_heads_that_do_not_fit_the_cache(heads):
             b.run(query=q, out=torch.empty_like(q), sliding_window=window)
 
 
+def test_workspace_in_pieces_is_refused():
+    """Elements that do not lie side by side, or are one element many times over, are no room for the kernels."""
+    b = Batch([(2999, 1), (700, 3)], 4, 1, 128, 16, "block_int8", torch.bfloat16, seed=14)
+    need = ops.paged_window_attention_workspace_bytes(2, b.rows + 1, 4, 1, 128, b.max_query, b.max_len, b.form)
+    for ws in (torch.empty(2 * need, dtype=torch.uint8, device=DEV)[::2], torch.empty(1, dtype=torch.uint8, device=DEV).expand(need)):
+        assert ws.numel() == need
+        with pytest.raises(RuntimeError, match="contiguous"):
+            b.run(workspace=ws)
+
+
 def test_one_scale_that_is_no_number():
     """Rows that see nothing stay zero whatever the scale is."""
     b = Batch([(0, 3), (20, 2), (0, 300)], 4, 2, 64, 16, "fp8", torch.bfloat16, seed=17)

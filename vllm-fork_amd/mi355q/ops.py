@@ -1458,6 +1458,8 @@ def paged_window_attention(out: torch.Tensor, query: torch.Tensor, key_cache: to
     if need:
         if workspace is None:
             workspace, room = torch.empty(need, dtype=torch.uint8, device=query.device), need
+        elif not workspace.is_contiguous():
+            raise RuntimeError(f"{what}: workspace must be contiguous")
         else:
             room = workspace.numel() * workspace.element_size()
     _launch(index, L.mi355q_paged_window_attention, out.data_ptr(), os_[0], query.data_ptr(), qs[0], key_cache.data_ptr(),
