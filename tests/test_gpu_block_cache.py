@@ -755,6 +755,32 @@ def test_rows_that_see_nothing():
 
 
 @pytest.mark.parametrize("form", ["block_int8", "block_fp8"])
+@pytest.mark.parametrize("window,sinks", [(0, 0), (40, 3)])
+@pytest.mark.parametrize("factor", [2.0 ** 24, 2.0 ** 40, 2.0 ** 90])
+def test_values_of_another_size_where_a_row_does_not_see_them(form, window, sinks, factor):
+    """Blocks whose V is larger by far, ahead of a row or behind its window: the row is held to the largest value that it sees itself.
+    Prompts, chunks, drafts of one and of two column tiles, decode rows beside them; a wave that meets such a block first and walks on."""
+    def louder(b, s, page):
+        b.v[int(b.tables[s, page])] *= factor
+        b.dev["vs"][int(b.tables[s, page])] *= factor
+
+    for D, bs in ((64, 16), (128, 32)):
+        for lens in ([(0, 300), (130, 90), (70, 1)], [(200, 12), (300, 4), (62, 5), (190, 1)]):
+            b = Batch(lens, 8, 2, D, bs, form, torch.bfloat16, window=window, sinks=sinks, seed=28, loud=0.3)
+            for s, (c, n) in enumerate(lens):
+                for page in {(c + n - 1) // bs, (c + n // 2) // bs} - {0}:
+                    louder(b, s, page)
+            b.check()
+    if window:
+        b = Batch([(5, 1)] * 40 + [(2000, 40)], 2, 2, 64, 16, form, torch.bfloat16, window=1200, sinks=sinks, seed=29, loud=0.3)
+        louder(b, 40, 800 // 16)
+        b.check()
+        b = Batch([(2000, 300)], 2, 2, 64, 16, form, torch.bfloat16, window=1200, sinks=sinks, seed=29, loud=0.3)
+        louder(b, 0, 816 // 16)
+        b.check()
+
+
+@pytest.mark.parametrize("form", ["block_int8", "block_fp8"])
 def test_scales_far_apart(form):
     """Blocks whose V scales differ by factors of up to e^30: the probabilities in between keep their bits."""
     b = Batch([(700, 1), (300, 6)], 4, 2, 128, 16, form, torch.bfloat16, seed=11, loud=6.0)

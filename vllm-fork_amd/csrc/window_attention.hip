@@ -14,7 +14,8 @@
 // largest.  K's and V's block scales stay outside the products, for the 16 tokens of a lane group lie in one block.  K's is
 // one factor per lane on the logits.  V's is taken relative to the largest V scale met so far (vref, rescaled like the running
 // maximum), so that fp16 holds it: for decode rows one factor per lane on the probabilities; for prompts a power of two, exact
-// on V's codes, and the rest in [1, 2), which goes into the exponent of the probabilities.  One scale for the whole cache
+// on V's codes, and the rest in [1, 2), which goes into the exponent of the probabilities.  Where it is too small for that (the
+// larger one may be of tokens that other rows see) it goes onto the products, in fp32, which holds scales 2^100 apart.  One scale for the whole cache
 // goes into the softmax scale and into the result.  Scales are 0 or more, or NaN.
 #include <limits.h>
 #include <math.h>
@@ -219,15 +220,15 @@ __device__ inline u32x4 only(u32x4 v, bool here, int n) {
 // group g = lane / 16 holds after S^T are tokens 16 g .. 16 g + 15: one block, one scale, and the B operand of O^T as
 // they stand; V comes in its own order, 16 tokens of a head dim per lane.
 //
-// Probabilities are 2^(x - m + 15) here (the largest fits fp16 once V's relative scale, at most 1/2, has been applied): what
-// a block whose scale is 10^-8 of the largest adds still has all its bits.
+// Probabilities are 2^(x - m + 15) here, times V's relative scale, which is at most 1 and, down to 2^-12, leaves the largest ones
+// all their bits.  Tiles with smaller ones (but zeros) are multiplied a token at a time, the scale put onto the products in fp32.
 //
 // Measured, 32 heads over 8 kv heads of 128: 32 rows under a window of 4096 in bf16 84 us, 4.8 TB/s (a large copy reaches 5.1; the
 // matrix cores are busy 5 % of the time); 32 rows of 100 to 4095 tokens in int8 33 us, 3.6 TB/s, the longest sequence's workgroup
 // ends last; two rows of 131072 and 50001 tokens, 64 heads, e4m3, 68 us and 5 us for the join, 4.4 TB/s; 16 drafts of
 // five rows over 500 to 3500 tokens, int8, 22.6 and 4.2 us; one row of 1001 tokens 11 us, round trips.
 // ---------------------------------------------------------------------------------------------------------------------
-constexpr float WA_ROWS_SHIFT = 15.0f;
+constexpr float WA_ROWS_SHIFT = 15.0f, WA_RLEAST = 0x1p-12f;
 
 template <typename DT, int KV, int HEAD, int NCT, int NW>
 __global__ __launch_bounds__(64 * NW, 2) void window_rows_kernel(const WindowParams p) {
@@ -441,7 +442,9 @@ __global__ __launch_bounds__(64 * NW, 2) void window_rows_kernel(const WindowPar
   };
 
   // One tile.  INNER: every column sees every token of it, if its pages exist.
-  bool left_out = false;               // a tile whose V holds an infinity or NaN that only some columns may see
+  // a tile left out: V holds an infinity or NaN that only some columns may see, or its scale would leave fp16 probabilities too few bits
+  // (the reference may be of tokens that other columns see)
+  bool left_out = false;
   auto step = [&](auto inner) {
     constexpr bool INNER = decltype(inner)::value;
     const int t0 = span.base(tile), lim = span.limit(tile), tg = t0 + 16 * g;
@@ -477,6 +480,9 @@ __global__ __launch_bounds__(64 * NW, 2) void window_rows_kernel(const WindowPar
     // the sum of weights over what is rounded for the product, where V's scale leaves it its bits
     const bool rounded = KV == KV16 || __all(r >= 0x1p-10f);
     const float less = KV == KV16 ? 1.f : __builtin_amdgcn_rcpf(r);
+    const bool apart = KV != KV16 && __any(r > 0.f && r < WA_RLEAST);
+    left_out |= apart;
+    const float rp = apart ? 0.f : r;
     u32x4 pf[NCT][2];
 #pragma unroll
     for (int n = 0; n < NCT; n++) {
@@ -523,7 +529,7 @@ __global__ __launch_bounds__(64 * NW, 2) void window_rows_kernel(const WindowPar
       }
 #pragma unroll
       for (int i = 0; i < 8; i++) {
-        uint32_t w = KV == KV16 ? pack_p<MT>(x[2 * i], x[2 * i + 1]) : pack_p<MT>(x[2 * i] * r, x[2 * i + 1] * r);
+        uint32_t w = KV == KV16 ? pack_p<MT>(x[2 * i], x[2 * i + 1]) : pack_p<MT>(x[2 * i] * rp, x[2 * i + 1] * rp);
         sum = add_pair<MT>(w, sum);
         // (a NaN scale reaches only the columns that see its tokens)
         if (!INNER && KV != KV16) w &= ((seen >> (2 * i)) & 1 ? 0xffffu : 0u) | ((seen >> (2 * i)) & 2 ? 0xffff0000u : 0u);
@@ -573,48 +579,67 @@ __global__ __launch_bounds__(64 * NW, 2) void window_rows_kernel(const WindowPar
     while (tile < in1) step(std::true_type());
     while (tile < end) step(std::false_type());
 
-    // tiles left out: once more, one token at a time, added to the columns that see it
-    if (KV != KVI8 && left_out) {
+    // tiles left out: once more, one token at a time, added to the columns that see it.  Which they were: the same reference, from the start
+    if (__builtin_expect(left_out, false)) {
+      float ref = 0.f, inv = 1.f;
       for (tile = begin + wave; tile < end; tile += NW) {
-        if (tile >= in0 && tile < in1) continue;
         look_up(tile);
+        const bool ok = (at_ok >> g) & 1, inner = tile >= in0 && tile < in1;
+        const float vs = KV == KV16 ? 1.f : __shfl(at_vs, g, 64);
+        bool again = false;
+        if constexpr (KV != KV16) {
+          const float vtop = group_max(vs);
+          if (__any(vtop > ref)) ref = fmaxf(2.f * vtop, 0x1p-125f), inv = 1.f / ref;
+          const float r = ok ? vs * inv : 1.f;
+          again = __any(r > 0.f && r < WA_RLEAST);
+        }
+        if (!again && (KV == KVI8 || inner)) continue;
         load_k(0);
         load_v(0);
         const int lim = span.limit(tile), tg = span.base(tile) + 16 * g;
-        const bool ok = (at_ok >> g) & 1;
-        if (!__any(clear_v(tg, lim, ok))) continue;
-        f32x4 s[NCT][4];
-        logits(s);
-        const float ks = KV == KV16 ? 1.f : __shfl(at_ks, g, 64), vs = KV == KV16 ? 1.f : __shfl(at_vs, g, 64);
-        const float r = KV == KV16 || !ok ? 1.f : vs * vinv;
-        uint32_t seen[NCT];
-        u32x4 pf[NCT][2];
+        if (!__any(clear_v(tg, lim, ok)) && !again) continue;
+        const float ks = KV == KV16 ? 1.f : __shfl(at_ks, g, 64);
+        uint32_t zero;
+        auto fresh = [&]() { asm volatile("v_mov_b32 %0, 0" : "=v"(zero)); };   // keeps widened operands out of registers across loops
 #pragma unroll
         for (int n = 0; n < NCT; n++) {
-          seen[n] = sees(n, tg, lim, ok);
+          fresh();
+          const uint32_t seen = sees(n, tg, lim, ok);
           const float f = qscale[n] * ks, ms = (m[n] == -INFINITY ? 0.f : m[n]) - WA_ROWS_SHIFT;
+          u32x4 pf[2];
 #pragma unroll
-          for (int i = 0; i < 8; i++)
-            pf[n][i >> 2][i & 3] = pack2<MT>(exp2_fast(s[n][i >> 1][2 * (i & 1)] * f - ms) * r, exp2_fast(s[n][i >> 1][2 * (i & 1) + 1] * f - ms) * r);
-        }
+          for (int T = 0; T < 4; T++) {
+            f32x4 s = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int ds = 0; ds < DS; ds++) {
+              u32x4 a;
+              if constexpr (EB == 1) a = widen8<KV>(kf[T][ds >> 1] ^ u32x4{zero, zero, zero, zero}, ds & 1);
+              else a = kf[T][ds];
+              s = mfma16<MT>(a, qf[n][ds], s);
+            }
+#pragma unroll
+            for (int i = 0; i < 2; i++) pf[T >> 1][2 * (T & 1) + i] = pack2<MT>(exp2_fast(s[2 * i] * f - ms), exp2_fast(s[2 * i + 1] * f - ms));
+          }
 #pragma unroll 1
-        for (int k = 0; k < 64; k++) {
-          const int i = k & 15;
-          const bool here = g == k >> 4;
-          uint32_t zero;
-          asm volatile("v_mov_b32 %0, 0" : "=v"(zero));   // keeps widened operands out of registers across the loop
-#pragma unroll
-          for (int n = 0; n < NCT; n++) {
-            const bool counts = (__shfl((int)seen[n], (k & 48) + col, 64) >> i) & 1;
+          for (int k = 0; k < 64; k++) {
+            const int i = k & 15;
+            const bool here = g == k >> 4;
+            const float factor = KV == KV16 ? 1.f : __shfl(vs * vinv, k & 48, 64);
+            const bool counts = (__shfl((int)seen, (k & 48) + col, 64) >> i) & 1;
+            fresh();
 #pragma unroll
             for (int d = 0; d < DT16; d++) {
-              f32x4 x = o[n][d];
+              f32x4 x = KV == KV16 ? o[n][d] : f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
               for (int h = 0; h < 2; h++) {
                 u32x4 v;
                 if constexpr (EB == 1) v = widen8<KV>(vf[d][0] ^ u32x4{zero, zero, zero, zero}, h);
                 else v = vf[d][h] ^ u32x4{zero, zero, zero, zero};
-                x = mfma16<MT>(only<MT>(v, here, i - 8 * h), only<MT>(pf[n][h], here, i - 8 * h), x);
+                x = mfma16<MT>(only<MT>(v, here, i - 8 * h), only<MT>(pf[h], here, i - 8 * h), x);
+              }
+              if constexpr (KV != KV16) {
+#pragma unroll
+                for (int e = 0; e < 4; e++) x[e] = __builtin_fmaf(x[e], factor, o[n][d][e]);
               }
               if (counts) o[n][d] = x;
             }
@@ -694,7 +719,8 @@ __global__ __launch_bounds__(64 * NW, 2) void window_rows_kernel(const WindowPar
 // of each 16-token stretch are tokens 8 h .. 8 h + 7 of it (h = lane / 32), the B operand of O^T as they stand.  A stretch lies
 // in one block, so K's scale is wave-uniform per 8 registers and joins the factor of the exponent.  V's scale is a power of two
 // times a number in [1, 2): the power, relative to that of the largest scale met so far and with 2^7 in hand, goes into the
-// widened codes, exactly (down to scales of 2^-30 of the largest); the number goes into the exponent of the probabilities.
+// widened codes, exactly (down to scales of 2^-21 of the largest, below that onto the products, a token at a time; e4m3 codes have bits down
+// to 2^-9, and fp16 numbers down to 2^-24); the number goes into the exponent of the probabilities.
 //
 // Bound by the matrix cores and the exponentials in turn: a SIMD holds two waves of 128-wide heads, and while both are in their
 // softmax no product runs.  8192 rows of 32 heads of 128 under a window of 4096, bf16: 430 to 475 us from card to card, 870 to 960 TFLOP/s of what is visible
@@ -726,7 +752,7 @@ __device__ inline float pair_sum(float v) {
   auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
   return __uint_as_float(r[0]) + __uint_as_float(r[1]);
 }
-constexpr float WA_VSHIFT = 128.0f;
+constexpr float WA_VSHIFT = 128.0f, WA_VLEAST = 0x1p-14f;
 
 template <typename DT, int KV, int HEAD, int NW>
 __global__ __launch_bounds__(64 * NW, HEAD == 64 ? 4 : 2) void window_flash_kernel(const WindowParams p) {
@@ -746,8 +772,9 @@ __global__ __launch_bounds__(64 * NW, HEAD == 64 ? 4 : 2) void window_flash_kern
   struct Chunk {
     u32x4 at[4 * CHUNK];      // per stretch: block offset (64 bits), token offset in the block, tokens somebody sees
     float ks[SCALES];
-    float vpow[SCALES], vlog[SCALES], vinv[SCALES];   // V's scale: 2^7 power / vref, log2 and reciprocal of the rest
-    int ok[CHUNK];            // per tile: stretches whose page exists and that begin before the end
+    float vpow[SCALES], vlog[SCALES], vinv[SCALES];   // V's scale: 2^7 power / vref (1 where vfac has it), log2 and reciprocal of the rest
+    float vfac[SCALES];       // the power where fp16 would not hold its products with the codes, else 1
+    int ok[CHUNK];            // per tile: stretches whose page exists and that begin before the end; 16: some vfac is not 1
     float vref;               // a power of two above every scale so far
   };
   __shared__ __attribute__((aligned(1024))) unsigned char lds[LDS];
@@ -871,7 +898,12 @@ __global__ __launch_bounds__(64 * NW, HEAD == 64 ? 4 : 2) void window_flash_kern
         const uint32_t bits = __float_as_uint(v[i]);
         const bool split = v[i] > 0x1p-100f && v[i] < INFINITY;      // (else as it is: zero, next to it, or a NaN that stays one)
         const float rest = split ? __uint_as_float((bits & 0x007fffffu) | 0x3f800000u) : 1.f;
-        ch.vpow[n] = split ? __uint_as_float(bits & 0x7f800000u) * inv : v[i] * inv + (v[i] - v[i]);
+        const float power = split ? __uint_as_float(bits & 0x7f800000u) * inv : v[i] * inv + (v[i] - v[i]);
+        const bool apart = power > 0.f && power < WA_VLEAST;
+        ch.vpow[n] = apart ? 1.f : power;
+        ch.vfac[n] = apart ? power : 1.f;
+        const uint64_t some = __ballot(apart);
+        if ((lane & 3) == 0 && ((some >> lane) & 15)) ch.ok[n >> 2] |= 16;
         ch.vlog[n] = __builtin_amdgcn_logf(rest);
         ch.vinv[n] = 1.f / rest;
       }
@@ -1004,6 +1036,8 @@ __global__ __launch_bounds__(64 * NW, HEAD == 64 ? 4 : 2) void window_flash_kern
     if (tiles > 1) request(1);
   }
 
+  int state = SCALED && tiles > 0 ? __builtin_amdgcn_readfirstlane(chunks[0].ok[0]) : 0;   // `ok` of the tile to come
+
   // One tile.  INNER: every column of the workgroup sees every token of it, if its pages exist.
   auto step = [&](int n, auto inner) {
     constexpr bool INNER = decltype(inner)::value;
@@ -1013,7 +1047,8 @@ __global__ __launch_bounds__(64 * NW, HEAD == 64 ? 4 : 2) void window_flash_kern
     const unsigned char* st0 = lds + (n & 1) * STAGE + lane * 16;
     const Chunk& ch = chunk_of(n);
     const int t0 = INNER ? 0 : span.base(begin + n), lim = INNER ? 0 : span.limit(begin + n);
-    const int ok_tile = __builtin_amdgcn_readfirstlane(ch.ok[n % CHUNK]);
+    const int next = SCALED ? chunk_of(n + 1).ok[(n + 1) % CHUNK] : 0, ok_tile = SCALED ? state & 15 : __builtin_amdgcn_readfirstlane(ch.ok[n % CHUNK]);
+    const bool apart = SCALED && state > 15;
     bool idle = wc0 > wc1;
     // does any of the wave's columns see any of it?
     if constexpr (!INNER) idle = idle || t0 > wpos1 || (p.window && t0 + 63 <= wpos0 - p.window && t0 >= p.sinks) || ok_tile == 0;
@@ -1047,6 +1082,7 @@ __global__ __launch_bounds__(64 * NW, HEAD == 64 ? 4 : 2) void window_flash_kern
 #pragma unroll
       for (int j = 0; j < 4; j++) f[j] = qscale * ks[j];
     }
+    if constexpr (SCALED) state = __builtin_amdgcn_readfirstlane(next);
     if (n + 1 < tiles) {
       deliver(n + 1);
       if (n + 2 < tiles) request(n + 2);
@@ -1129,7 +1165,32 @@ __global__ __launch_bounds__(64 * NW, HEAD == 64 ? 4 : 2) void window_flash_kern
 
     // ---- O^T += V^T P^T -------------------------------------------------------------------------------------------------
     const unsigned char* vt = st0 + KBYTES;
-    if (INNER || bad_tile[n & 1] != n + 1) {
+    if (!INNER && __builtin_expect(bad_tile[n & 1] == n + 1 || apart, false)) {
+      // an infinity or NaN that some columns may see and others must not, or scales too far apart for fp16: one token at a time,
+      // scaled in fp32 and added where it is seen
+#pragma unroll 1
+      for (int k = 0; k < 64; k++) {
+        const int st = k >> 4, i = k & 7, t = t0 + k;
+        const bool here = half == ((k >> 3) & 1);
+        const bool counts = t < lim && t <= pos && (!p.window || t > pos - p.window || t < p.sinks) && ((ok_tile >> st) & 1);
+        const u32x4 pb = only<MT>(st == 0 ? pf[0] : st == 1 ? pf[1] : st == 2 ? pf[2] : pf[3], here, i);
+#pragma unroll
+        for (int d = 0; d < DTL; d++) {
+          const u32x4 a = only<MT>(*reinterpret_cast<const u32x4*>(vt + (d * 4 + st) * 1024), here, i);
+          f32x16 r;
+          if constexpr (SCALED) {
+            r = mfma32<MT>(a, pb, f32x16{});
+            const float factor = ch.vfac[n % CHUNK * 4 + st];
+#pragma unroll
+            for (int e = 0; e < 16; e++) r[e] = __builtin_fmaf(r[e], factor, o[d][e]);
+          } else {
+            r = mfma32<MT>(a, pb, o[d]);
+          }
+#pragma unroll
+          for (int e = 0; e < 16; e++) o[d][e] = counts ? r[e] : o[d][e];
+        }
+      }
+    } else {
 #pragma unroll
       for (int d = 0; d < DTL; d++)
 #pragma unroll
@@ -1141,36 +1202,22 @@ __global__ __launch_bounds__(64 * NW, HEAD == 64 ? 4 : 2) void window_flash_kern
         __builtin_amdgcn_sched_group_barrier(0x100, 1, 1);
       }
       __builtin_amdgcn_sched_group_barrier(0x008, 4, 1);
-    } else {
-      // an infinity or NaN that some columns may see and others must not: one token at a time, added where it is seen
-#pragma unroll 1
-      for (int k = 0; k < 64; k++) {
-        const int st = k >> 4, i = k & 7, t = t0 + k;
-        const bool here = half == ((k >> 3) & 1);
-        const bool counts = t < lim && t <= pos && (!p.window || t > pos - p.window || t < p.sinks) && ((ok_tile >> st) & 1);
-        const u32x4 pb = only<MT>(st == 0 ? pf[0] : st == 1 ? pf[1] : st == 2 ? pf[2] : pf[3], here, i);
-#pragma unroll
-        for (int d = 0; d < DTL; d++) {
-          const u32x4 a = only<MT>(*reinterpret_cast<const u32x4*>(vt + (d * 4 + st) * 1024), here, i);
-          const f32x16 r = mfma32<MT>(a, pb, o[d]);
-#pragma unroll
-          for (int e = 0; e < 16; e++) o[d][e] = counts ? r[e] : o[d][e];
-        }
-      }
     }
   };
+  // a tile of scales too far apart goes through the masked step
+  auto inner = [&](int n) { return n >= in0 && n < in1 && (!SCALED || __builtin_expect(state < 16, true)); };
   int n = 0;
   if constexpr (HEAD == 64 || KV == KV16) {
     // the masked step stands once in the code: 35 KB instead of 45, and short walks are bound by fetching it (five prompts under a
     // window of 512 47.7 -> 44.4 us, 8192 rows in bf16 444 -> 440).  With codes of 128-wide heads the compiler then finds worse
     // registers: 2048 rows over 6144 296 -> 330 us.
     while (n < tiles) {
-      for (; n >= in0 && n < in1; n++) step(n, std::true_type());
+      for (; inner(n); n++) step(n, std::true_type());
       if (n < tiles) step(n++, std::false_type());
     }
   } else {
     for (; n < in0; n++) step(n, std::false_type());
-    for (; n < in1; n++) step(n, std::true_type());
+    for (; inner(n); n++) step(n, std::true_type());
     for (; n < tiles; n++) step(n, std::false_type());
   }
 
