@@ -756,8 +756,8 @@ int mi355q_rope_and_cache_blocks(const int64_t* positions, const void* query, in
  * Causal attention of rows of any query length over the paged cache, with an optional sliding window and first tokens
  * that stay visible: row j of sequence s stands at p = seq_lens[s] - query_len[s] + j and sees token t where
  *   t <= p and (window == 0 or t > p - window or t < sinks).
- * A row that sees nothing is written as zeros; rows behind the last sequence are not touched.  kv_type MI355Q_KV_16:
- * cache of dtype elements (k_scale / v_scale unused); MI355Q_KV_FP8 / MI355Q_KV_INT8: codes whose scale is read at
+ * A row that sees nothing (or whose logits are all minus infinity) is written as zeros; rows behind the last sequence are
+ * not touched.  kv_type MI355Q_KV_16: cache of dtype elements (k_scale / v_scale unused); MI355Q_KV_FP8 / MI355Q_KV_INT8: codes whose scale is read at
  * [block * scale_block_stride + kv_head * scale_head_stride], 0 or more or NaN -- strides 0 give the one-scale cache of
  * mi355q_reshape_and_cache, the caches of mi355q_rope_and_cache_blocks have one for each.
  * Only pages that some row sees are looked up (those behind the window may have been given away); a page number outside
@@ -765,8 +765,11 @@ int mi355q_rope_and_cache_blocks(const int64_t* positions, const void* query, in
  * max_query_len bounds the query lengths (of a longer one only its first max_query_len rows are certain); max_seq_len only chooses how
  * the work is cut.
  * workspace: device scratch of mi355q_paged_window_attention_workspace_bytes(...) bytes (0: may be NULL), used by this
- * call alone; nothing in it has to be cleared.  (The size is 0 too for bounds that the call refuses.)  head_size 64 or 128; 1 to 16 query heads to a kv head; block_size a
- * multiple of 16 up to 256.
+ * call alone; nothing in it has to be cleared.  (The size is 0 too for bounds that the call refuses.)  head_size 64 or
+ * 128; 1 to 16 query heads to a kv head; block_size a multiple of 16 up to 256.
+ * Sums, maxima and products are held in fp32; probabilities are rounded to dtype (16-bit caches) or fp16 (8-bit ones) for
+ * the product with V, and summed as rounded; bf16 queries of 8-bit caches are brought to fp16 by a power of two for each
+ * row and head.
  * Stands for the reference's windowed attention (sliding_window of AttentionImpl, vllm/v1/attention/backends/
  * rocm_attn.py:271-300; ops/prefix_prefill.py SLIDING_WINDOW); visible first tokens and block scales have no counterpart there.
  */

@@ -754,6 +754,21 @@ def test_rows_that_see_nothing():
         assert torch.equal(cpu(b2.run())[3:5], got[3:5])
 
 
+def test_logits_of_minus_infinity():
+    """A row whose logits are all minus infinity is zeros; next to finite ones such a token weighs nothing."""
+    b = Batch([(100, 1), (30, 200), (60, 3)], 4, 2, 64, 16, "auto", torch.float16, seed=30)
+    b.dev["q"].abs_().add_(0.5)
+    lost = [int(p) for p in b.tables[0, :7]] + [int(b.tables[1, 1]), int(b.tables[2, 2])]
+    for page in lost:
+        b.kc[page, :, 0, :, 0] = -torch.inf
+    b.tables[1, 1] = b.tables[2, 2] = -1                # to the formula, tokens of no weight are tokens that nobody sees
+    b.q = cpu(b.dev["q"])
+    want, bound = b.reference()
+    got = cpu(b.run()).double()
+    assert torch.equal(got[0], torch.zeros_like(got[0]))
+    assert ((got[1:b.rows] - want[1:]).abs() <= bound[1:]).all()
+
+
 @pytest.mark.parametrize("form", ["block_int8", "block_fp8"])
 @pytest.mark.parametrize("window,sinks", [(0, 0), (40, 3)])
 @pytest.mark.parametrize("factor", [2.0 ** 24, 2.0 ** 40, 2.0 ** 90])
