@@ -16,9 +16,10 @@
 // work belongs to the wave of the run's first token: the largest magnitude is known before anything is encoded, no
 // atomics, no second launch, and the result does not depend on any order of execution.
 //
-// Bound by HBM for prompts: 8192 tokens of 32 query and 8 kv heads of 128, int8, 35 to 39 us for 185 MB, 4.7 to 5.3 TB/s, what a large copy
-// reaches.  A decode step is a chain of round trips: slots, then rows, angles, scales and the block, then the stores: 6.9 us for
-// one token, 7.5 for 64; 508 tokens with half of a 64-wide head rotated 9.7.
+// Bound by HBM for prompts: 8192 tokens of 32 query and 8 kv heads of 128, int8, 186.8 MB in 38 to 40 us, 4.7 to 4.9 TB/s, where two
+// batches take turns, 45 us, 4.2 TB/s, over eight, of which the caches hold nothing (a large copy reaches 5.15).  A decode step is a
+// chain of round trips: slots, then rows, angles, scales and the block, then the stores: 6 to 7 us for one token, 6.5 to 8 for 64; 508
+// tokens with half of a 64-wide head rotated 9.6.
 #include "common.h"
 
 // one rounding per operation: the results equal a sequence of separate fp32 multiplications and additions
@@ -309,10 +310,13 @@ __device__ inline u32x4 byte_mask(uint32_t m) {
 // turned in LDS, so that the cache takes 16 tokens of a head dim at once.  What the block held (needed where the scale
 // grows, and around the new tokens of V) is requested together with the new rows: a decode step is three round trips.
 // FORM_WHOLE: NeoX pairing over the whole head, 16-bit angles of the model's type, aligned rows; FORM_NONE: no rotation, aligned
-// rows -- nearly every call, in kernels that the general form's code (60 KB) does not weigh on: 47 -> 35 us for 8192 prompt
-// tokens of 32 + 8 heads, 8.1 -> 6.7 us for one token.  Under FORM_WHOLE a lane holds 8 elements of K and their 8 partners.
-// FORM_PART: the other rotations that turn runs of 16, aligned rows: 8192 tokens with half of each head in pairs 68 -> 62 us, 64 decode
-// tokens 9.1 -> 7.8 (with registers for three workgroups to a CU instead of two, as the two forms above, 59 and 9.8).
+// rows -- nearly every call, in kernels that the general form's code (60 KB) does not weigh on.  Over eight batches in turn, in a graph,
+// general form and this: 8192 prompt tokens of 32 + 8 heads 89 and 45 us, without rotation 61 and 46; one token 7.8 and 5.8, 6.4 and 5.6.
+// Under FORM_WHOLE a lane holds 8 elements of K and their 8 partners.
+// FORM_PART: the other rotations that turn runs of 16, aligned rows: half of each head in pairs 81 and 75 us, in halves 89 and 81, 64
+// decode tokens 8.2 and 6.9, 8.5 and 7.1: the query has one pass on its way where FORM_WHOLE has four, and in halves every run is
+// read once more for its partners.  (One batch again and again 62 us and, for 64 tokens, 7.8; with registers for three workgroups to
+// a CU instead of two, as the two forms above have, 59 and 9.8.)
 enum { FORM_ANY = 0, FORM_WHOLE = 1, FORM_NONE = 2, FORM_PART = 3 };
 template <typename DT, bool INT8, int HEAD, int FORM>
 __device__ __forceinline__ void append_run(const AppendParams& p, int t, uint64_t here, int blk, int offset, int pos, int h,
@@ -715,7 +719,10 @@ extern "C" int mi355q_rope_and_cache_blocks(const int64_t* positions, const void
   const int pieces = block_size / 16;
   p.page_magic = pieces == 1 ? 0 : (int)(((1ull << 32) + pieces - 1) / pieces);
   // a wave looks at one position where a step holds few tokens (every one begins a run of its own), at 8 where they come
-  // as prompts: most positions then continue a run, and waves that find nothing to begin are pure dispatch
+  // as prompts: most positions then continue a run, and waves that find nothing to begin are pure dispatch.  The slots are on the
+  // device, so the number of tokens has to tell.  One position and eight, int8, 32 + 8 heads of 128, in a graph: decode rows 64 6.4 and
+  // 32.5 us, 512 12.3 and 27.7, 1024 21.8 and 30.3, 2048 38.0 and 36.6; a prompt of 64 6.4 and 6.3, 512 12.9 and 7.0, 1024 21.4 and
+  // 8.1, 8192 144 and 36.6.  (A decode batch of 600 rows pays 14 us for what a prompt of that length gains 7.)
   p.tokens_per_wave = num_tokens <= 512 ? 1 : 8;
   const int64_t units = ((int64_t)num_tokens + p.tokens_per_wave - 1) / p.tokens_per_wave * num_kv_heads;
   const int64_t kv_groups = (units + 3) / 4;

@@ -28,7 +28,6 @@
 namespace mi355q {
 
 typedef __attribute__((ext_vector_type(2))) _Float16 wa_f16x2;
-typedef __attribute__((ext_vector_type(2))) __bf16 wa_bf16x2;
 
 constexpr float WA_LOG2E = 1.44269504088896f;
 // Probabilities are kept as 2^(x - m + 6): fp16 then resolves a probability down to 2^-30 of the largest, and the running
@@ -78,7 +77,6 @@ __device__ inline T sload(const T* p) {
   return *(const __attribute__((address_space(4))) T*)(uintptr_t)p;
 }
 
-// what a sequence's rows [first column, last column] see: sink tokens [0, sink_end) and [low, end), 64 at a time
 // Prompt rows: column tile `slot` of the batch, counted over the sequences that have any (seq < 0: there are fewer).  The grid
 // is as large as num_rows allows, not sequences times the longest: every wave counts for itself, a sequence per lane.
 struct Slot { int seq, ct, start, qlen; };
@@ -114,6 +112,7 @@ __device__ inline int64_t part_row(const WindowParams& p, int seq, int start, in
   return p.part_rows ? (int64_t)seq * p.part_rows + (row - start) : row;
 }
 
+// what a sequence's rows [first column, last column] see: sink tokens [0, sink_end) and [low, end), 64 at a time
 struct Span {
   int sink_end, low, end, sink_tiles, tiles;
   __device__ inline int base(int i) const { return i < sink_tiles ? 64 * i : low + 64 * (i - sink_tiles); }
@@ -223,10 +222,10 @@ __device__ inline u32x4 only(u32x4 v, bool here, int n) {
 // Probabilities are 2^(x - m + 15) here, times V's relative scale, which is at most 1 and, down to 2^-12, leaves the largest ones
 // all their bits.  Tiles with smaller ones (but zeros) are multiplied a token at a time, the scale put onto the products in fp32.
 //
-// Measured, 32 heads over 8 kv heads of 128: 32 rows under a window of 4096 in bf16 84 us, 4.8 TB/s (a large copy reaches 5.1; the
-// matrix cores are busy 5 % of the time); 32 rows of 100 to 4095 tokens in int8 33 us, 3.6 TB/s, the longest sequence's workgroup
-// ends last; two rows of 131072 and 50001 tokens, 64 heads, e4m3, 68 us and 5 us for the join, 4.4 TB/s; 16 drafts of
-// five rows over 500 to 3500 tokens, int8, 22.6 and 4.2 us; one row of 1001 tokens 11 us, round trips.
+// Measured, 32 heads over 8 kv heads of 128: 32 rows under a window of 4096 in bf16 83 us, 468.6 MB, 5.6 TB/s (a large read reaches 6.0;
+// the matrix cores are busy 5 % of the time); 32 rows of 100 to 4095 tokens in int8 34 us, 138.3 MB, 4.1 TB/s, the longest sequence's
+// workgroup ends last; two rows of 131072 and 50002 tokens, 64 heads, e4m3, 68.5 us and 4.8 us for the join, 371.3 MB, 5.1 TB/s; 16 drafts
+// of five rows over 500 to 3500 tokens, int8, 23.0 and 4.2 us, 67.1 MB, 2.5 TB/s; one row of 1001 tokens 11 us, round trips.
 // ---------------------------------------------------------------------------------------------------------------------
 constexpr float WA_ROWS_SHIFT = 15.0f, WA_RLEAST = 0x1p-12f;
 
@@ -723,11 +722,12 @@ __global__ __launch_bounds__(64 * NW, 2) void window_rows_kernel(const WindowPar
 // to 2^-9, and fp16 numbers down to 2^-24); the number goes into the exponent of the probabilities.
 //
 // Bound by the matrix cores and the exponentials in turn: a SIMD holds two waves of 128-wide heads, and while both are in their
-// softmax no product runs.  8192 rows of 32 heads of 128 under a window of 4096, bf16: 430 to 475 us from card to card, 870 to 960 TFLOP/s of what is visible
-// (a large matrix product reaches 1190); the matrix cores are busy 45 % of the cycles counted, the vector units 47 %, LDS conflicts
-// are 3 %.  2048 rows over a context of 6144 in int8 293 us, 810 TFLOP/s.  64-wide heads have room for two workgroups
-// to a CU, and the exponentials weigh twice as much: five prompts of up to 2047 rows under a window of 512, e4m3 with one scale, 40 us,
-// vector units busy 60 %, matrix cores 22.
+// softmax no product runs.  8192 rows of 32 heads of 128 under a window of 4096, bf16: 431 to 475 us from card to card, 870 to 960
+// TFLOP/s of what is visible (a large matrix product reaches 1190 to 1230); the matrix cores are busy 45 % of the cycles counted, the
+// vector units 46 %, LDS conflicts are 3 %.  2048 rows over a context of 6144 and 700 of their own, int8, with a decode row's two launches
+// 292 to 313 us, 780 to 837 TFLOP/s.  64-wide heads have room for two workgroups to a CU, and the exponentials weigh twice as much: five
+// prompts of up to 2047 rows under a window of 512, e4m3 with one scale, 40 us behind each other (44 on an idle card), vector units
+// busy 61 %, matrix cores 22.
 // Slower at 8192 rows: four waves (489 us), the next tile's logits ahead of this one's softmax (795, registers spill), the
 // halves of a workgroup in opposite phases over three buffers (578), higher priority for half the waves (449 against 448).
 // ---------------------------------------------------------------------------------------------------------------------
@@ -1387,6 +1387,7 @@ static WindowPlan window_plan(int num_seqs, int num_rows, int num_heads, int num
     const int64_t stretches = groups <= 64 ? 256 / groups : std::max<int64_t>(256 / groups, std::clamp<int64_t>(std::min(tiles / 64, 16384 / groups), 1, 32));
     // A stretch has a tile for each wave at least, and two for each stay whole: the join is a launch of 4 us.  One sequence, in a
     // graph: 1000 tokens whole 11.1 us, in two 11.9; 2000 whole 15.7, in four 11.8; 4000 in four 13.9, in eight 12.2; 8000 15.8 and 14.0.
+    // (Calls one by one from Python are bound by the host, and the join is a second launch there: 2000 tokens whole 20 us, in four 24.)
     window_cut(w.rows, tiles, stretches, (tiles <= 2 * w.rows.waves ? 2 : 1) * w.rows.waves);
   }
   if (prompts) {
