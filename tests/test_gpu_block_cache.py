@@ -754,6 +754,20 @@ def test_rows_that_see_nothing():
         assert torch.equal(cpu(b2.run())[3:5], got[3:5])
 
 
+@pytest.mark.parametrize("form", ["block_int8", "block_fp8"])
+@pytest.mark.parametrize("lens", [[(9000, 80)], [(9000, 5)], [(8150, 1), (9100, 9)]])
+def test_values_of_another_size_on_long_walks(form, lens):
+    """The same where a workgroup walks a long context whole: the larger values come last, or first and are left behind by the window."""
+    for window, at in ((0, lambda c, n: c + n // 2), (5000, lambda c, n: c + n // 2 - 5000), (0, lambda c, n: 4000), (5000, lambda c, n: c - 300)):
+        b = Batch(lens, 8, 2, 64, 16, form, torch.bfloat16, window=window, sinks=2, seed=31, loud=0.3)
+        for s, (c, n) in enumerate(lens):
+            page = int(b.tables[s, at(c, n) // 16])
+            b.v[page] *= 2.0 ** 40
+            b.dev["vs"][page] *= 2.0 ** 40
+        b.check(b.run(max_seq_len=64))
+        b.check()
+
+
 def test_logits_of_minus_infinity():
     """A row whose logits are all minus infinity is zeros; next to finite ones such a token weighs nothing."""
     b = Batch([(100, 1), (30, 200), (60, 3)], 4, 2, 64, 16, "auto", torch.float16, seed=30)
