@@ -46,6 +46,15 @@ def test_more_than_a_launch_holds_is_refused():
     refused(_lib.lib().mi355q_paged_window_attention, ATTEND, "too many", num_seqs=1 << 24, num_rows=1 << 24, max_query_len=1)
 
 
+def test_sizes_whose_products_pass_64_bits_are_refused():
+    """Workgroups times threads wrap around to a small number, or to none."""
+    many = 1 << 30
+    refused(_lib.lib().mi355q_rope_and_cache_blocks, APPEND, "too many", num_tokens=1 << 26, num_kv_heads=many, block_stride=many * 128 * 16)
+    for heads, longest in ((many, 1), (many, 64), (1 << 25, 1), ((1 << 31) - 1, (1 << 31) - 1)):
+        refused(_lib.lib().mi355q_paged_window_attention, ATTEND, "too many", num_seqs=many, num_rows=many, num_heads=heads, num_kv_heads=heads,
+                max_query_len=longest)
+
+
 def test_nothing_to_append_is_no_error():
     assert _lib.lib().mi355q_rope_and_cache_blocks(*{**APPEND, "num_tokens": 0}.values()) == _lib.OK
 

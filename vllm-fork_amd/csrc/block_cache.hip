@@ -727,7 +727,7 @@ extern "C" int mi355q_rope_and_cache_blocks(const int64_t* positions, const void
   const int64_t units = ((int64_t)num_tokens + p.tokens_per_wave - 1) / p.tokens_per_wave * num_kv_heads;
   const int64_t kv_groups = (units + 3) / 4;
   const int q_groups = num_heads ? (int)(((int64_t)num_tokens + 3) / 4) : 0;
-  MI355Q_REQUIRE((kv_groups + q_groups) * 256 < (int64_t)1 << 32, "rope_and_cache_blocks: %d tokens are too many for a launch", num_tokens);
+  MI355Q_REQUIRE(kv_groups + q_groups < (int64_t)1 << 24, "rope_and_cache_blocks: %d tokens are too many for a launch", num_tokens);
   p.kv_groups = (int)kv_groups;
   const size_t lds = (size_t)4 * head_size * block_size;
   hipStream_t s = (hipStream_t)stream;

@@ -1419,6 +1419,15 @@ static WindowPlan window_plan(int num_seqs, int num_rows, int num_heads, int num
   return w;
 }
 
+// a launch has fewer than 2^32 threads (taken apart by divisions: the products may pass 64 bits)
+static bool window_fits(const WindowPlan& w, int num_seqs, int num_kv_heads) {
+  auto fits = [&](const WindowPart& a, int64_t tiles) {
+    const int64_t most = ((int64_t)1 << 32) - 1, of_tile = std::max<int64_t>((int64_t)a.splits * 64 * a.waves, a.splits > 1 ? a.cols / 4 * 256 : 0);
+    return !a.col_tiles || tiles <= most / num_kv_heads / a.col_tiles / of_tile;
+  };
+  return fits(w.rows, num_seqs) && fits(w.flash, 1);
+}
+
 // Partial sums of decode rows: room for so many rows of a sequence, or (0) for the rows as they are numbered, if that is less.
 static int window_part_rows(const WindowPlan& w, int num_seqs, int num_rows, int max_query_len, int G) {
   const int64_t of_seq = (std::min<int64_t>((int64_t)max_query_len * G, w.row_cols) + G - 1) / G;
@@ -1438,10 +1447,6 @@ static int launch_window(WindowParams p, const WindowPlan& w, int part_rows, hip
   auto tiles = [&](const WindowPart& a) { return (int64_t)(&a == &w.rows ? p.num_seqs : 1) * p.num_kv_heads * a.col_tiles; };
   auto groups = [&](const WindowPart& a) { return tiles(a) * a.splits; };
   auto merges = [&](const WindowPart& a) { return tiles(a) * (a.cols / 4); };
-  auto fits = [&](const WindowPart& a) {      // a launch has fewer than 2^32 threads
-    return groups(a) * 64 * a.waves < (int64_t)1 << 32 && (a.splits <= 1 || merges(a) * 256 < (int64_t)1 << 32);
-  };
-  MI355Q_REQUIRE(fits(w.rows) && fits(w.flash), "paged_window_attention: too many workgroups");
   const int announced = p.longest_cols;
   for (int kind = 0; kind < 2; kind++) {
     const WindowPart& a = kind ? w.flash : w.rows;
@@ -1495,6 +1500,7 @@ extern "C" size_t mi355q_paged_window_attention_workspace_bytes(int num_seqs, in
   if (num_seqs <= 0 || num_rows <= 0 || !heads_fit(num_heads, num_kv_heads) || max_query_len <= 0 || max_seq_len <= 0 || window < 0 || sinks < 0)
     return 0;
   const WindowPlan w = window_plan(num_seqs, num_rows, num_heads, num_kv_heads, kv_type, max_query_len, max_seq_len, window, sinks);
+  if (!window_fits(w, num_seqs, num_kv_heads)) return 0;
   return (size_t)window_partials(w, num_seqs, num_rows, num_heads, num_kv_heads, max_query_len) * (head_size + 2) * sizeof(float);
 }
 
@@ -1528,6 +1534,7 @@ extern "C" int mi355q_paged_window_attention(void* out, int64_t out_stride, cons
                  "paged_window_attention: caches and query rows must be 16-byte aligned");
   MI355Q_REQUIRE(((uintptr_t)out & 3) == 0 && out_stride % 2 == 0, "paged_window_attention: output rows must be 4-byte aligned");
   const WindowPlan w = window_plan(num_seqs, num_rows, num_heads, num_kv_heads, kv_type, max_query_len, max_seq_len, window, sinks);
+  MI355Q_REQUIRE(window_fits(w, num_seqs, num_kv_heads), "paged_window_attention: too many workgroups");
   const int64_t partials = window_partials(w, num_seqs, num_rows, num_heads, num_kv_heads, max_query_len);
   const size_t need = (size_t)partials * (head_size + 2) * sizeof(float);
   if (need && (!workspace || workspace_bytes < need))
